@@ -457,6 +457,58 @@ int asme_ws_linear_residual_ln(const float* X, int64_t M, int64_t K, const float
                                const float* ln_w, const float* ln_b, float eps, float* s_out, float* ln_out,
                                float* stats, void* stream);
 
+/* ---- Operators over long histories.  `dtype`: the storage of the tensors declared void* -- 0 fp32, 1 bf16 (arithmetic,
+ * statistics and sums are fp32 either way, each output rounded once).  Tensors declared float* are fp32. */
+
+/* Distillation (csrc/distill.hip), next to asme_cross_entropy_*: the KL divergence of softmax(logits / temperature) over
+ * the catalogue from softmax(teacher / temperature) over row r's list ids[r][0..top) (entries outside [0, V) are absent;
+ * an item twice on a list counts twice), times temperature^2, mean over the rows whose list is not empty (NaN if none).
+ * logits (n, V) rows ld apart; ids, teacher (n, top), top <= 1024.  out[0] = loss, out[1] = rows with a list; state
+ * (n, 2) and prob (n, top) are for the backward.  Workspace: bytes from the *_workspace query. */
+int64_t asme_distill_xent_workspace(int64_t n, int64_t V);
+int asme_distill_xent_fwd(const void* logits, int64_t ld, int64_t n, int64_t V, const int64_t* ids,
+                          const float* teacher, int64_t top, float temperature, int dtype, float* state, float* prob,
+                          void* workspace, int64_t ws_bytes, float* out, void* stream);
+/* dlogits (rows ld_d apart; not logits itself) = dloss[0] times the gradient; rows without a list: 0.  stats = the
+ * forward's out. */
+int asme_distill_xent_bwd(const void* logits, int64_t ld, int64_t n, int64_t V, const int64_t* ids, int64_t top,
+                          float temperature, int dtype, const float* state, const float* prob, const float* stats,
+                          const float* dloss, void* dlogits, int64_t ld_d, void* stream);
+
+/* Gated residual between two norms (csrc/gatednorm.hip), next to asme_residual_ln_*:
+ *   s = residual_scale * res + gate * Npost(y);  z = Npre(s)
+ * over n rows of dim <= 8192 values; N = LayerNorm, or root-mean-square norm (rms = 1), with weight and nullable bias.
+ * gate (nullable): n / rows_per_gate rows, each for rows_per_gate consecutive rows.  pre_w null: no z.  stats (n, 4). */
+int asme_gated_residual_norm_fwd(const void* res, const void* y, const void* gate, int64_t rows_per_gate,
+                                 const float* post_w, const float* post_b, const float* pre_w, const float* pre_b,
+                                 int64_t n, int64_t dim, float residual_scale, float eps, int rms, int dtype,
+                                 void* s_out, void* z_out, float* stats, void* stream);
+/* bytes; rows_per_gate = n without a gate or with rows_per_gate 1 */
+int64_t asme_gated_residual_norm_bwd_workspace(int64_t n, int64_t dim, int64_t rows_per_gate);
+/* ds, dz (nullable): gradients of s and z.  dres, dy, dgate and dw (4, dim: post_w, post_b, pre_w, pre_b) nullable. */
+int asme_gated_residual_norm_bwd(const void* res, const void* y, const void* gate, int64_t rows_per_gate,
+                                 const float* post_w, const float* post_b, const float* pre_w, int64_t n, int64_t dim,
+                                 float residual_scale, int rms, int dtype, const float* stats, const void* ds,
+                                 const void* dz, void* dres, void* dy, void* dgate, float* dw, void* workspace,
+                                 int64_t ws_bytes, void* stream);
+
+/* Serving window attention (csrc/windowcache.hip).  Cache of a sequence: cache_k, cache_v (batch, kv_heads, slots,
+ * head_dim), slots = sinks + window; position p in slot p while p < sinks, then in sinks + (p - sinks) mod window.
+ * step: stores the new token's k, v (batch, kv_heads, head_dim) at position lengths[b] (tokens before this one; negative:
+ * the sequence takes no step, its output is 0 and its cache stays) and writes out (batch, heads, head_dim) = the
+ * attention of q (the same shape) to everything the cache then holds.  lengths stay as they are (several layers share
+ * them).  head_dim 16, 32, 64 or 128; heads a multiple of kv_heads; pointers 16-byte aligned. */
+int64_t asme_window_step_workspace(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t slots);
+int asme_window_step(const void* q, const void* k, const void* v, void* cache_k, void* cache_v, const int64_t* lengths,
+                     int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t slots, int64_t sinks,
+                     float scale, int dtype, void* workspace, int64_t ws_bytes, void* out, void* stream);
+/* fill: positions 0 .. min(lengths[b], seq_len) - 1 of a prompt (element strides of batch, token and head given; a
+ * head's values adjacent) into the slots they end up in; slots that no position falls on stay as they are. */
+int asme_window_cache_fill(const void* k, const void* v, int64_t k_batch, int64_t k_token, int64_t k_head,
+                           int64_t v_batch, int64_t v_token, int64_t v_head, const int64_t* lengths, int64_t batch,
+                           int64_t seq_len, int64_t kv_heads, int64_t head_dim, int64_t slots, int64_t sinks, int dtype,
+                           void* cache_k, void* cache_v, void* stream);
+
 /* ---- NARM encoders (csrc/narm.hip).  Global encoder: one nn.GRU layer, batch_first, h_0 = 0
  * (core/models/narm/components.py:32-56; the reference packs the padded batch, the recurrence is causal so the
  * valid positions are identical).  Hidden size padded to hp (multiple of 16, <= 128; padded gate rows/columns and

@@ -1,0 +1,455 @@
+// The end of one block and the start of the next in one pass, next to residual + LayerNorm (norm.hip): the block's output
+// normed, gated and added to a scaled residual, and the sum normed for the next block.
+//
+//   branch = Npost(y);  s = a * res + gate * branch;  z = Npre(s)
+//   N(x) = (x - mean) r * w + b, r = 1 / sqrt(var + eps);  root-mean-square form: mean = 0, r = 1 / sqrt(mean x^2 + eps)
+//   backward of (ds, dz), x^ the normalised rows of y (post) and s (pre):
+//     d    = ds + Npre'(dz);          Npre'(g) = r (h - mean(h) - x^ mean(h x^)), h = g w (rms: without mean(h))
+//     dres = a d;  dgate = d * branch;  dy = Npost'(d * gate);  dw, db: column sums of g x^ and g
+//
+// gate: none, or one row of `dim` values for every rows_per_gate consecutive rows (all rows: a gate per channel; one
+// sequence's rows: a gate per sequence; 1: a gate per element).
+// Memory bound: forward reads res, y and writes s, z; backward reads res, y, ds, dz and writes dres, dy (s is formed
+// again from res and y, in fp32, instead of being read back rounded).  Every row is held in registers, at most 8 values a
+// thread, by as many threads as that takes (16 .. 1024, so a row's sums are shuffles within a wave up to 512 values and
+// one LDS exchange between waves beyond).  Weights stay in registers over a workgroup's rows.  Column sums: registers
+// over a workgroup's rows, then partial rows summed in a fixed order -- no atomics.
+#include "elem.h"
+
+using namespace asme;
+
+namespace {
+
+constexpr int kMaxDim = 8192;
+constexpr int kPer = 8;  // values per thread
+
+// values i = 0..7 of thread t of a row: VEC: whole 16-byte vectors, else single elements kPer apart in threads
+template <class T, int TPR, bool VEC>
+struct Row {
+    static constexpr int TPRv = TPR;
+    static constexpr int kBlock = TPR > 256 ? TPR : 256;
+    static constexpr int kSlots = TPR >= 64 ? (TPR > 64 ? 1 : kBlock / 64) : kBlock / TPR;  // rows at a time
+    static constexpr int kThreads = TPR > 64 ? TPR : 256;
+    static constexpr int E = VEC ? Elem<T>::V : 1;
+    static __device__ __forceinline__ int col(int t, int i) { return ((i / E) * TPR + t) * E + i % E; }
+    static __device__ __forceinline__ void load(const T* p, int t, int D, float (&x)[kPer]) {
+        if constexpr (VEC) {
+#pragma unroll
+            for (int c = 0; c < kPer / E; ++c) {
+                float v[E];
+                const int j = (c * TPR + t) * E;
+                if (j < D) Elem<T>::load(p + j, v);
+#pragma unroll
+                for (int e = 0; e < E; ++e) x[c * E + e] = j < D ? v[e] : 0.f;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) x[i] = i * TPR + t < D ? Elem<T>::get(p + i * TPR + t) : 0.f;
+        }
+    }
+    static __device__ __forceinline__ void store(T* p, int t, int D, const float (&x)[kPer]) {
+        if constexpr (VEC) {
+#pragma unroll
+            for (int c = 0; c < kPer / E; ++c) {
+                float v[E];
+                const int j = (c * TPR + t) * E;
+#pragma unroll
+                for (int e = 0; e < E; ++e) v[e] = x[c * E + e];
+                if (j < D) Elem<T>::store(p + j, v);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kPer; ++i)
+                if (i * TPR + t < D) Elem<T>::put(p + i * TPR + t, x[i]);
+        }
+    }
+    static __device__ __forceinline__ void load_f32(const float* p, int t, int D, float def, float (&x)[kPer]) {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const int j = col(t, i);
+            x[i] = p && j < D ? p[j] : (j < D ? def : 0.f);
+        }
+    }
+    // N sums over the row's threads, in every one of them.  Rows of more than one wave: through `red` (2 x N x 16 floats,
+    // alternating halves, so one barrier a call is enough); `flip` counts the calls.
+    template <int N>
+    static __device__ __forceinline__ void sum(float (&v)[N], float* red, int& flip) {
+        constexpr int W = TPR < 64 ? TPR : 64;
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+#pragma unroll
+            for (int o = W / 2; o >= 1; o >>= 1) v[k] += __shfl_xor(v[k], o, 64);
+        if constexpr (TPR > 64) {
+            float* r = red + (flip & 1) * 32;
+            ++flip;
+            if ((threadIdx.x & 63) == 0)
+#pragma unroll
+                for (int k = 0; k < N; ++k) r[k * 16 + (threadIdx.x >> 6)] = v[k];
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < N; ++k) {
+                v[k] = 0.f;
+#pragma unroll
+                for (int w = 0; w < TPR / 64; ++w) v[k] += r[k * 16 + w];
+            }
+        }
+    }
+};
+
+struct Args {
+    const void *res, *y, *gate;
+    const float *post_w, *post_b, *pre_w, *pre_b;
+    int64_t n, rows_per_gate;
+    int D;
+    float scale, eps;
+    int rms;
+    void *s, *z;
+    float* stats;  // (n, 4): mean and r of y, mean and r of s
+    // backward
+    const void *ds, *dz;
+    void *dres, *dy, *dgate;
+    float* part;       // (grid, 4, D): post_w, post_b, pre_w, pre_b
+    float* gate_part;  // (items, D) when a gate's rows are split over items
+    int64_t subs, sub_rows, items;
+};
+
+// mean and 1 / deviation of the row's values (two passes over registers)
+template <class R>
+__device__ __forceinline__ void moments(const float (&x)[kPer], int t, int D, float eps, int rms, float* red, int& flip,
+                                        float& mean, float& r) {
+    mean = 0.f;
+    if (!rms) {
+        float v[1] = {0.f};
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) v[0] += x[i];
+        R::template sum<1>(v, red, flip);
+        mean = v[0] / (float)D;
+    }
+    float v[1] = {0.f};
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const float c = R::col(t, i) < D ? x[i] - mean : 0.f;
+        v[0] = fmaf(c, c, v[0]);
+    }
+    R::template sum<1>(v, red, flip);
+    r = 1.f / sqrtf(v[0] / (float)D + eps);
+}
+
+template <class T, class R>
+__global__ __launch_bounds__(R::kThreads) void fwd_kernel(Args a) {
+    __shared__ float red[64];
+    int flip = 0;
+    const int t = threadIdx.x % R::TPRv, slot = R::kSlots > 1 ? threadIdx.x / R::TPRv : 0, D = a.D;
+    float pw[kPer], pb[kPer], qw[kPer], qb[kPer];
+    R::load_f32(a.post_w, t, D, 1.f, pw);
+    R::load_f32(a.post_b, t, D, 0.f, pb);
+    R::load_f32(a.pre_w, t, D, 1.f, qw);
+    R::load_f32(a.pre_b, t, D, 0.f, qb);
+    // (every thread of a workgroup makes the same number of turns: the row sums may hold a barrier)
+    for (int64_t base = (int64_t)blockIdx.x * R::kSlots; base < a.n; base += (int64_t)gridDim.x * R::kSlots) {
+        const int64_t row = min(base + slot, a.n - 1);
+        const bool live = base + slot < a.n;
+        float x[kPer], s[kPer], m, r;
+        R::load((const T*)a.y + row * D, t, D, x);
+        R::load((const T*)a.res + row * D, t, D, s);
+        float g[kPer];
+        if (a.gate) R::load((const T*)a.gate + row / a.rows_per_gate * D, t, D, g);
+        moments<R>(x, t, D, a.eps, a.rms, red, flip, m, r);
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const float b = fmaf((x[i] - m) * r, pw[i], pb[i]);
+            s[i] = a.gate ? fmaf(g[i], b, a.scale * s[i]) : fmaf(a.scale, s[i], b);
+        }
+        if (live) R::store((T*)a.s + row * D, t, D, s);
+        float m2 = 0.f, r2 = 0.f;
+        if (a.pre_w) {
+            // columns behind the row hold b's 0, not a number of the row
+            moments<R>(s, t, D, a.eps, a.rms, red, flip, m2, r2);
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) s[i] = fmaf((s[i] - m2) * r2, qw[i], qb[i]);
+            if (live) R::store((T*)a.z + row * D, t, D, s);
+        }
+        if (live && t == 0) *reinterpret_cast<float4*>(a.stats + row * 4) = make_float4(m, r, m2, r2);
+    }
+}
+
+// the workgroup's column sums of one accumulator over its row slots -> out[0..D)
+template <class R, class Put>
+__device__ __forceinline__ void column_sums(const float (&acc)[kPer], int t, int slot, int D, float* buf, Put&& put) {
+    if constexpr (R::kSlots == 1) {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i)
+            if (R::col(t, i) < D) put(R::col(t, i), acc[i]);
+    } else {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) buf[(slot * R::TPRv + t) * kPer + i] = acc[i];
+        __syncthreads();
+        // buf[slot][thread][value]: one (thread, value) pair per column
+        for (int c = threadIdx.x; c < R::TPRv * kPer; c += R::kThreads) {
+            float v = 0.f;
+#pragma unroll
+            for (int k = 0; k < R::kSlots; ++k) v += buf[k * R::TPRv * kPer + c];
+            const int j = R::col(c / kPer, c % kPer);
+            if (j < D) put(j, v);
+        }
+    }
+}
+
+// GATE: 0 none, 1 a row of its own for every row (dgate written at once), 2 shared by rows_per_gate rows.
+// Items: rows_per_gate rows (all rows without a shared gate) in `subs` pieces of sub_rows; a workgroup takes items
+// blockIdx.x, + gridDim.x, ...: a shared gate's sums are closed at the end of each item, the weights' at the end of all.
+template <class T, class R, int GATE>
+__global__ __launch_bounds__(R::kThreads) void bwd_kernel(Args a) {
+    __shared__ float red[64];
+    __shared__ float buf[R::kSlots > 1 ? R::kSlots * R::TPRv * kPer : 1];
+    int flip = 0;
+    const int t = threadIdx.x % R::TPRv, slot = R::kSlots > 1 ? threadIdx.x / R::TPRv : 0, D = a.D;
+    const float inv_d = 1.f / (float)D, centre = a.rms ? 0.f : 1.f;
+    float pw[kPer], pb[kPer], qw[kPer];
+    R::load_f32(a.post_w, t, D, 1.f, pw);
+    R::load_f32(a.post_b, t, D, 0.f, pb);
+    R::load_f32(a.pre_w, t, D, 1.f, qw);
+    float acc[4][kPer], gacc[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) acc[0][i] = acc[1][i] = acc[2][i] = acc[3][i] = gacc[i] = 0.f;
+    for (int64_t item = blockIdx.x; item < a.items; item += gridDim.x) {
+        const int64_t group = item / a.subs, first = (item % a.subs) * a.sub_rows;
+        const int64_t begin = group * a.rows_per_gate + first;
+        const int64_t end = group * a.rows_per_gate + min(a.rows_per_gate, first + a.sub_rows);
+        for (int64_t base = begin; base < end; base += R::kSlots) {
+            const bool live = base + slot < end;
+            const int64_t row = live ? base + slot : end - 1;
+            const float4 st = *reinterpret_cast<const float4*>(a.stats + row * 4);
+            float y[kPer], s[kPer], d[kPer], g[kPer], dz[kPer];
+            R::load((const T*)a.y + row * D, t, D, y);
+            R::load((const T*)a.res + row * D, t, D, s);
+            if (a.ds) R::load((const T*)a.ds + row * D, t, D, d);
+            if (a.dz) R::load((const T*)a.dz + row * D, t, D, dz);
+            if (GATE == 1) R::load((const T*)a.gate + row * D, t, D, g);
+            if (GATE == 2) R::load((const T*)a.gate + group * D, t, D, g);
+            float br[kPer];
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                if (!live || !a.ds) d[i] = 0.f;
+                const bool in = R::col(t, i) < D;
+                y[i] = in ? (y[i] - st.x) * st.y : 0.f;
+                br[i] = fmaf(y[i], pw[i], pb[i]);
+                s[i] = GATE ? fmaf(g[i], br[i], a.scale * s[i]) : fmaf(a.scale, s[i], br[i]);
+                s[i] = in ? (s[i] - st.z) * st.w : 0.f;
+            }
+            if (a.dz) {
+                float v[2] = {0.f, 0.f};
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) {
+                    if (!live) dz[i] = 0.f;
+                    acc[2][i] = fmaf(dz[i], s[i], acc[2][i]);
+                    acc[3][i] += dz[i];
+                    dz[i] *= qw[i];
+                    v[0] = fmaf(dz[i], s[i], v[0]);
+                    v[1] += dz[i];
+                }
+                R::template sum<2>(v, red, flip);
+                v[0] *= inv_d;
+                v[1] *= inv_d * centre;
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) d[i] = fmaf(dz[i] - fmaf(s[i], v[0], v[1]), st.w, d[i]);
+            }
+            if (a.dres && live) {
+                float o[kPer];
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) o[i] = a.scale * d[i];
+                R::store((T*)a.dres + row * D, t, D, o);
+            }
+            if (GATE == 1 && a.dgate) {
+                float o[kPer];
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) o[i] = d[i] * br[i];
+                if (live) R::store((T*)a.dgate + row * D, t, D, o);
+            }
+            float v[2] = {0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                if (R::col(t, i) >= D) d[i] = 0.f;
+                if (GATE == 2) gacc[i] = fmaf(d[i], br[i], gacc[i]);
+                const float db = GATE ? d[i] * g[i] : d[i];
+                acc[0][i] = fmaf(db, y[i], acc[0][i]);
+                acc[1][i] += db;
+                d[i] = db * pw[i];
+                v[0] = fmaf(d[i], y[i], v[0]);
+                v[1] += d[i];
+            }
+            if (a.dy) {
+                R::template sum<2>(v, red, flip);
+                v[0] *= inv_d;
+                v[1] *= inv_d * centre;
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) d[i] = (d[i] - fmaf(y[i], v[0], v[1])) * st.y;
+                if (live) R::store((T*)a.dy + row * D, t, D, d);
+            }
+        }
+        if (GATE == 2 && a.dgate) {
+            if (a.subs == 1)
+                column_sums<R>(gacc, t, slot, D, buf,
+                               [&](int j, float v) { Elem<T>::put((T*)a.dgate + group * D + j, v); });
+            else
+                column_sums<R>(gacc, t, slot, D, buf, [&](int j, float v) { a.gate_part[item * D + j] = v; });
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) gacc[i] = 0.f;
+        }
+    }
+    if (a.part)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            column_sums<R>(acc[k], t, slot, D, buf,
+                           [&](int j, float v) { a.part[((int64_t)blockIdx.x * 4 + k) * D + j] = v; });
+}
+
+// out[g][j] = sum over m < rows of part[g * rows + m][j], j < width: 64 columns x 16 row lanes a workgroup, then the
+// lanes' sums in order
+template <class T>
+__global__ __launch_bounds__(1024) void column_reduce_kernel(const float* __restrict__ part, int64_t rows, int64_t width,
+                                                             int64_t col_groups, T* __restrict__ out) {
+    __shared__ float buf[16][64];
+    const int64_t g = blockIdx.x / col_groups, j = blockIdx.x % col_groups * 64 + (threadIdx.x & 63);
+    const int lane = threadIdx.x >> 6;
+    float v = 0.f;
+    if (j < width)
+        for (int64_t m = lane; m < rows; m += 16) v += part[(g * rows + m) * width + j];
+    buf[lane][threadIdx.x & 63] = v;
+    __syncthreads();
+    if (lane == 0 && j < width) {
+        for (int k = 1; k < 16; ++k) v += buf[k][threadIdx.x];
+        Elem<T>::put(out + g * width + j, v);
+    }
+}
+
+bool aligned(std::initializer_list<const void*> ps) {
+    for (const void* p : ps)
+        if ((uintptr_t)p & 15) return false;
+    return true;
+}
+
+// f(Row<...>{}) for a checked dim: the fewest threads a row that hold it at 8 values each
+template <class T, class F>
+void with_row(int64_t D, bool vec, F&& f) {
+    auto pick = [&](auto v) {
+        constexpr bool VEC = decltype(v)::value;
+        if (D <= 16 * kPer) f(Row<T, 16, VEC>{});
+        else if (D <= 32 * kPer) f(Row<T, 32, VEC>{});
+        else if (D <= 64 * kPer) f(Row<T, 64, VEC>{});
+        else if (D <= 128 * kPer) f(Row<T, 128, VEC>{});
+        else if (D <= 256 * kPer) f(Row<T, 256, VEC>{});
+        else if (D <= 512 * kPer) f(Row<T, 512, VEC>{});
+        else f(Row<T, 1024, VEC>{});
+    };
+    if (vec) pick(std::true_type{});
+    else pick(std::false_type{});
+}
+
+// rows at a time and workgroups that fill the chip for a row layout
+int64_t slots_of(int64_t D) { return D <= 128 ? 16 : D <= 256 ? 8 : D <= 512 ? 4 : 1; }
+int64_t threads_of(int64_t D) {
+    return D <= 512 ? 256 : D <= 1024 ? 128 : D <= 2048 ? 256 : D <= 4096 ? 512 : 1024;
+}
+int64_t resident(int64_t D) { return 256 * 1024 / threads_of(D); }  // 16 waves per CU
+
+struct Plan {
+    int64_t subs, sub_rows, items, grid;
+};
+// pieces of the backward: the rows of a shared gate (else all rows) cut so that there are enough items to fill the chip,
+// each a whole number of turns; the grid (and with it the partial rows) is at most what runs at once
+Plan plan(int64_t n, int64_t rows_per_gate, int64_t D) {
+    const int64_t groups = n / rows_per_gate, slots = slots_of(D), fill = resident(D);
+    Plan p;
+    const int64_t turns = (rows_per_gate + slots - 1) / slots;
+    int64_t subs = std::min(turns, std::max<int64_t>(1, fill / groups));
+    p.sub_rows = (turns + subs - 1) / subs * slots;
+    p.subs = (rows_per_gate + p.sub_rows - 1) / p.sub_rows;
+    p.items = groups * p.subs;
+    p.grid = std::min(p.items, fill);
+    return p;
+}
+
+bool sizes_ok(int64_t n, int64_t D, int64_t rows_per_gate) {
+    return n >= 1 && D >= 1 && D <= kMaxDim && n <= (1ll << 40) / D && rows_per_gate >= 1 && rows_per_gate <= n &&
+           n % rows_per_gate == 0;
+}
+
+}  // namespace
+
+ASME_API int asme_gated_residual_norm_fwd(const void* res, const void* y, const void* gate, int64_t rows_per_gate,
+                                          const float* post_w, const float* post_b, const float* pre_w,
+                                          const float* pre_b, int64_t n, int64_t dim, float residual_scale, float eps,
+                                          int rms, int dtype, void* s_out, void* z_out, float* stats, void* stream) {
+    ASME_CHECK_ARG(res && y && post_w && s_out && stats, "asme_gated_residual_norm_fwd: null pointer");
+    ASME_CHECK_ARG(!pre_w || z_out, "asme_gated_residual_norm_fwd: z_out missing");
+    ASME_CHECK_ARG(dtype_ok(dtype), "asme_gated_residual_norm_fwd: dtype is 0 (fp32) or 1 (bf16)");
+    ASME_CHECK_ARG(sizes_ok(n, dim, gate ? rows_per_gate : 1), "asme_gated_residual_norm_fwd: bad size");
+    ASME_CHECK_ARG(eps >= 0.f, "asme_gated_residual_norm_fwd: eps >= 0");
+    Args a{};
+    a.res = res, a.y = y, a.gate = gate, a.post_w = post_w, a.post_b = post_b, a.pre_w = pre_w, a.pre_b = pre_b;
+    a.n = n, a.rows_per_gate = gate ? rows_per_gate : 1, a.D = (int)dim, a.scale = residual_scale, a.eps = eps;
+    a.rms = rms, a.s = s_out, a.z = z_out, a.stats = stats;
+    with_dtype(dtype, [&](auto e) {
+        using T = decltype(e);
+        with_row<T>(dim, dim % Elem<T>::V == 0 && aligned({res, y, gate, s_out, z_out}), [&](auto r) {
+            using R = decltype(r);
+            const int64_t turns = (n + R::kSlots - 1) / R::kSlots;
+            hipLaunchKernelGGL((fwd_kernel<T, R>), dim3((unsigned)std::min(turns, 2 * resident(dim))),
+                               dim3(R::kThreads), 0, (hipStream_t)stream, a);
+        });
+    });
+    ASME_LAUNCH_CHECK("asme_gated_residual_norm_fwd");
+}
+
+// bytes; 0 for sizes that the calls refuse
+ASME_API int64_t asme_gated_residual_norm_bwd_workspace(int64_t n, int64_t dim, int64_t rows_per_gate) {
+    if (!sizes_ok(n, dim, rows_per_gate)) return 0;
+    const Plan p = plan(n, rows_per_gate, dim);
+    return (p.grid * 4 + (p.subs > 1 ? p.items : 0)) * dim * 4;
+}
+
+// rows_per_gate: as in the forward; n (all rows) without a gate or with a gate row for every row (gate_rows = 1)
+ASME_API int asme_gated_residual_norm_bwd(const void* res, const void* y, const void* gate, int64_t rows_per_gate,
+                                          const float* post_w, const float* post_b, const float* pre_w, int64_t n,
+                                          int64_t dim, float residual_scale, int rms, int dtype, const float* stats,
+                                          const void* ds, const void* dz, void* dres, void* dy, void* dgate,
+                                          float* dw, void* workspace, int64_t ws_bytes, void* stream) {
+    ASME_CHECK_ARG(res && y && post_w && stats && workspace, "asme_gated_residual_norm_bwd: null pointer");
+    ASME_CHECK_ARG(!dz || pre_w, "asme_gated_residual_norm_bwd: dz without the norm's weight");
+    ASME_CHECK_ARG(!dgate || gate, "asme_gated_residual_norm_bwd: dgate without a gate");
+    ASME_CHECK_ARG(dtype_ok(dtype), "asme_gated_residual_norm_bwd: dtype is 0 (fp32) or 1 (bf16)");
+    ASME_CHECK_ARG(sizes_ok(n, dim, gate ? rows_per_gate : 1), "asme_gated_residual_norm_bwd: bad size");
+    const bool shared = gate && rows_per_gate > 1;
+    const int64_t rows = shared ? rows_per_gate : n;
+    ASME_CHECK_ARG(ws_bytes >= asme_gated_residual_norm_bwd_workspace(n, dim, rows),
+                   "asme_gated_residual_norm_bwd: workspace too small");
+    const Plan p = plan(n, rows, dim);
+    Args a{};
+    a.res = res, a.y = y, a.gate = gate, a.post_w = post_w, a.post_b = post_b, a.pre_w = pre_w;
+    a.n = n, a.rows_per_gate = rows, a.D = (int)dim, a.scale = residual_scale, a.rms = rms;
+    a.stats = const_cast<float*>(stats), a.ds = ds, a.dz = dz, a.dres = dres, a.dy = dy, a.dgate = dgate;
+    a.part = dw ? (float*)workspace : nullptr;
+    a.gate_part = (float*)workspace + p.grid * 4 * dim;
+    a.subs = p.subs, a.sub_rows = p.sub_rows, a.items = p.items;
+    hipStream_t st = (hipStream_t)stream;
+    const unsigned cg = (unsigned)((dim + 63) / 64), cg4 = (unsigned)((4 * dim + 63) / 64);
+    with_dtype(dtype, [&](auto e) {
+        using T = decltype(e);
+        with_row<T>(dim, dim % Elem<T>::V == 0 && aligned({res, y, gate, ds, dz, dres, dy, dgate}), [&](auto r) {
+            using R = decltype(r);
+            const dim3 grid((unsigned)p.grid), block(R::kThreads);
+            if (!gate) hipLaunchKernelGGL((bwd_kernel<T, R, 0>), grid, block, 0, st, a);
+            else if (!shared) hipLaunchKernelGGL((bwd_kernel<T, R, 1>), grid, block, 0, st, a);
+            else hipLaunchKernelGGL((bwd_kernel<T, R, 2>), grid, block, 0, st, a);
+        });
+        if (shared && dgate && p.subs > 1)
+            hipLaunchKernelGGL(column_reduce_kernel<T>, dim3((unsigned)(p.items / p.subs) * cg), dim3(1024), 0, st,
+                               a.gate_part, p.subs, dim, (int64_t)cg, (T*)dgate);
+    });
+    if (dw)
+        hipLaunchKernelGGL(column_reduce_kernel<float>, dim3(cg4), dim3(1024), 0, st, a.part, p.grid, 4 * dim,
+                           (int64_t)cg4, dw);
+    ASME_LAUNCH_CHECK("asme_gated_residual_norm_bwd");
+}

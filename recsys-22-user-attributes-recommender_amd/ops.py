@@ -15,6 +15,7 @@ from dataclasses import dataclass
 from typing import List, Optional, Sequence, Tuple
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import call, ptr, stream
@@ -48,6 +49,33 @@ def _f32(t: torch.Tensor) -> torch.Tensor:
 
 def _i64(t: torch.Tensor) -> torch.Tensor:
     return t.to(torch.int64).contiguous()
+
+
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1}  # the `dtype` argument of the C ABI
+
+
+def _dtype_code(t: torch.Tensor) -> int:
+    if t.dtype not in _DTYPES:
+        raise TypeError(f"expected a float32 or bfloat16 tensor, got {t.dtype}")
+    return _DTYPES[t.dtype]
+
+
+def _alike(like: torch.Tensor, dtype: Optional[torch.dtype] = None, **tensors):
+    """every given tensor on `like`'s device and (where `dtype` is given) of that dtype; like is on a ROCm device"""
+    ptr(like)
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if t.device != like.device:
+            raise ValueError(f"{name} is on {t.device}, expected {like.device}")
+        if dtype is not None and t.dtype != dtype:
+            raise TypeError(f"{name} is {t.dtype}, expected {dtype}")
+
+
+def _ws_bytes(name: str, *sizes, device) -> Tuple[Optional[torch.Tensor], int]:
+    """a workspace of the size a *_workspace query names"""
+    n = int(getattr(_lib.load(), name)(*sizes))
+    return (torch.empty(n, device=device, dtype=torch.uint8), n) if n else (None, 0)
 
 
 def _reduce_partials(part: torch.Tensor, width: int) -> torch.Tensor:
@@ -1443,6 +1471,95 @@ def residual_ln(res, y, norm: Optional[torch.nn.LayerNorm], p_a: float, p_b: flo
     return _ResidualLNFn.apply(res, y, norm.weight, norm.bias, norm.eps, p_a, p_b)
 
 
+class _GatedResidualNormFn(torch.autograd.Function):
+    """s = residual_scale * res + gate * Npost(y);  z = Npre(s)  (csrc/gatednorm.hip)"""
+
+    @staticmethod
+    def forward(ctx, res, y, gate, post_w, post_b, pre_w, pre_b, rows_per_gate: int, residual_scale: float, eps: float,
+                rms: bool):
+        ctx.set_materialize_grads(False)
+        n, D = res.shape
+        s = torch.empty_like(res)
+        z = torch.empty_like(res) if pre_w is not None else None
+        stats = torch.empty(n, 4, device=res.device, dtype=torch.float32)
+        with torch.cuda.device(res.device):
+            call("asme_gated_residual_norm_fwd", ptr(res), ptr(y), ptr(gate), rows_per_gate, ptr(post_w), ptr(post_b),
+                 ptr(pre_w), ptr(pre_b), n, D, residual_scale, eps, int(rms), _dtype_code(res), ptr(s), ptr(z),
+                 ptr(stats), stream())
+        ctx.save_for_backward(res, y, gate, post_w, post_b, pre_w, stats)
+        ctx.meta = (rows_per_gate, residual_scale, rms, pre_b is not None)
+        return s, z
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, ds, dz):
+        res, y, gate, post_w, post_b, pre_w, stats = ctx.saved_tensors
+        rows_per_gate, residual_scale, rms, has_pre_b = ctx.meta
+        n, D = res.shape
+        need = ctx.needs_input_grad
+        ds, dz = (None if g is None else _aligned(g) for g in (ds, dz))
+        if ds is None and dz is None:
+            return (None,) * 11
+        dres = torch.empty_like(res) if need[0] else None
+        dy = torch.empty_like(res) if need[1] else None
+        dgate = torch.empty_like(gate) if need[2] else None
+        dw = torch.empty(4, D, device=res.device, dtype=torch.float32) if any(need[3:7]) else None
+        with torch.cuda.device(res.device):
+            shared = n if gate is None or rows_per_gate == 1 else rows_per_gate
+            ws, nb = _ws_bytes("asme_gated_residual_norm_bwd_workspace", n, D, shared, device=res.device)
+            call("asme_gated_residual_norm_bwd", ptr(res), ptr(y), ptr(gate), rows_per_gate, ptr(post_w), ptr(post_b),
+                 ptr(pre_w), n, D, residual_scale, int(rms), _dtype_code(res), ptr(stats), ptr(ds), ptr(dz), ptr(dres),
+                 ptr(dy), ptr(dgate), ptr(dw), ptr(ws), nb, stream())
+        w = [dw[i] if need[3 + i] else None for i in range(4)] if dw is not None else [None] * 4
+        return (dres, dy, dgate, w[0], w[1], w[2], w[3], None, None, None, None)
+
+
+def gated_residual_norm(res: torch.Tensor, y: torch.Tensor, post_w: torch.Tensor,
+                        post_b: Optional[torch.Tensor] = None, pre_w: Optional[torch.Tensor] = None,
+                        pre_b: Optional[torch.Tensor] = None, gate: Optional[torch.Tensor] = None,
+                        residual_scale: float = 1.0, eps: float = 1e-5, rms: bool = False):
+    """The end of a block and the start of the next: (s, z) with
+        s = residual_scale * res + gate * Npost(y),   z = Npre(s)   (None without pre_w)
+    over the last axis (up to 8192 values), N a LayerNorm or (rms=True) a root-mean-square norm with weight and optional
+    bias.  gate: None, one value per channel (D,), or of res's rank with the trailing axes before the channels 1 --
+    (B, 1, D): a gate per sequence -- or of res's shape; it multiplies as it is (a tanh or sigmoid is the caller's).
+    res, y and gate of one dtype, float32 or bfloat16; the norms' weights of any floating type, their sums float32.
+    Differentiable once in everything but residual_scale and eps."""
+    D = res.shape[-1]
+    if res.shape != y.shape or res.dim() < 1:
+        raise ValueError(f"res {tuple(res.shape)} and y {tuple(y.shape)} differ")
+    if not 1 <= D <= 8192:
+        raise ValueError(f"{D} channels: expected 1 to 8192")
+    if pre_w is None and pre_b is not None:
+        raise ValueError("pre_b without pre_w")
+    if not (math.isfinite(residual_scale) and 0.0 <= eps < math.inf):
+        raise ValueError(f"residual_scale {residual_scale}, eps {eps}: expected finite numbers, eps >= 0")
+    _dtype_code(res)
+    _alike(res, res.dtype, y=y, gate=gate)
+    weights = dict(post_w=post_w, post_b=post_b, pre_w=pre_w, pre_b=pre_b)
+    _alike(res, **weights)
+    for name, w in weights.items():
+        if w is not None and (w.shape != (D,) or not w.is_floating_point()):
+            raise ValueError(f"{name} {tuple(w.shape)} of {w.dtype}: expected {D} floating values")
+    n = res.numel() // D
+    per = 1
+    if gate is not None:
+        lead = gate.shape[:-1] if gate.dim() > 1 else (1,) * (res.dim() - 1)
+        same = next((i for i, (a, b) in enumerate(zip(lead, res.shape)) if a != b), len(lead))
+        if gate.shape[-1:] != (D,) or len(lead) != res.dim() - 1 or any(a != 1 for a in lead[same:]):
+            raise ValueError(f"gate {tuple(gate.shape)} for rows {tuple(res.shape)}: expected ({D},), the rows' shape, "
+                             "or that with 1 in trailing axes before the channels")
+        per = n // max(1, gate.numel() // D)
+    if n == 0:
+        zero = res + y * post_w.to(y.dtype)
+        return zero, (zero if pre_w is not None else None)
+    s, z = _GatedResidualNormFn.apply(
+        _aligned(res).view(n, D), _aligned(y).view(n, D), None if gate is None else _aligned(gate).view(-1, D),
+        *(None if w is None else w.float().contiguous() for w in weights.values()), per, float(residual_scale),
+        float(eps), bool(rms))
+    return s.view(res.shape), (None if z is None else z.view(res.shape))
+
+
 class _GeluDropoutFn(torch.autograd.Function):
     """dropout(GELU_erf(x)) (transformer_layers.py:217-220; ffn_modifier.py:24-26 with p = 0)"""
 
@@ -1531,6 +1648,92 @@ def attention(qkv, key_valid, heads: int, causal: bool, p_drop: float = 0.0, ker
     """kernels: the kernel family (asme_attention_fwd_kernels): 0 automatic (the product path); 1 streaming only and
     2 resident with the recomputing dQ pass for the kernel tests and A/B timing"""
     return _AttentionFn.apply(qkv, key_valid, heads, causal, p_drop, kernels)
+
+
+def window_cache_fill(cache_k: torch.Tensor, cache_v: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                      lengths: torch.Tensor, sinks: int = 0):
+    """Lay prompts into ring caches (asme_window_cache_fill), in place: k, v (B, L, kv_heads, head_dim), of which
+    sequence b has lengths[b] tokens from position 0; cache_k, cache_v (B, kv_heads, sinks + window, head_dim).  Slots
+    that no position of a prompt falls on stay as they are (window_attention_step does not read them)."""
+    _check_cache(cache_k, cache_v, sinks)
+    B, KV, slots, D = cache_k.shape
+    if k.dim() != 4 or k.shape != v.shape or k.shape[0] != B or k.shape[2:] != (KV, D):
+        raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)}: expected (batch {B}, length, {KV}, {D})")
+    _alike(cache_k, cache_k.dtype, k=k, v=v)
+    _alike(cache_k, lengths=lengths)
+    if lengths.shape != (B,):
+        raise ValueError(f"lengths {tuple(lengths.shape)}: expected ({B},)")
+    if B == 0 or k.shape[1] == 0:
+        return
+    k, v = _strided_heads(k.detach()), _strided_heads(v.detach())
+    with torch.cuda.device(cache_k.device):
+        call("asme_window_cache_fill", ptr(k), ptr(v), *k.stride()[:3], *v.stride()[:3], ptr(_i64(lengths)), B,
+             k.shape[1], KV, D, slots, sinks, _dtype_code(cache_k), ptr(cache_k), ptr(cache_v), stream())
+
+
+def window_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache_k: torch.Tensor,
+                          cache_v: torch.Tensor, lengths: torch.Tensor, sinks: int = 0,
+                          scale: Optional[float] = None) -> torch.Tensor:
+    """One new token per sequence against its ring cache (asme_window_step): stores k, v (B, kv_heads, head_dim) as
+    position lengths[b] -- the tokens before this one; negative: the sequence takes no step -- and returns the attention
+    (B, heads, head_dim) of q to what the cache then holds, the row that window_attention gives that position.  The
+    caches (B, kv_heads, sinks + window, head_dim) change in place; `lengths` does not (the layers of a model share it:
+    add 1 once per token).  No gradients."""
+    _check_cache(cache_k, cache_v, sinks)
+    B, KV, slots, D = cache_k.shape
+    if q.dim() != 3 or q.shape[0] != B or q.shape[2] != D or q.shape[1] == 0 or q.shape[1] % KV:
+        raise ValueError(f"q {tuple(q.shape)}: expected ({B}, a multiple of {KV}, {D})")
+    if k.shape != (B, KV, D) or v.shape != (B, KV, D):
+        raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)}: expected ({B}, {KV}, {D})")
+    _alike(cache_k, cache_k.dtype, q=q, k=k, v=v)
+    _alike(cache_k, lengths=lengths)
+    if lengths.shape != (B,):
+        raise ValueError(f"lengths {tuple(lengths.shape)}: expected ({B},)")
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, cache_k, cache_v)):
+        raise RuntimeError("window_attention_step has no gradient: call it under torch.no_grad()")
+    q, k, v = (_aligned(t) for t in (q, k, v))
+    out = torch.empty_like(q)
+    if B == 0:
+        return out
+    with torch.cuda.device(q.device):
+        ws, nb = _ws_bytes("asme_window_step_workspace", B, q.shape[1], KV, D, slots, device=q.device)
+        call("asme_window_step", ptr(q), ptr(k), ptr(v), ptr(cache_k), ptr(cache_v), ptr(_i64(lengths)), B, q.shape[1],
+             KV, D, slots, sinks, D ** -0.5 if scale is None else scale, _dtype_code(q), ptr(ws), nb, ptr(out),
+             stream())
+    return out
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """t contiguous, from a 16-byte boundary on"""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _strided_heads(t: torch.Tensor) -> torch.Tensor:
+    """(B, L, heads, head_dim) with adjacent head values and every row on a 16-byte boundary, copied only if it is not"""
+    per = 16 // t.element_size()
+    ok = t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(s % per == 0 and s >= 0 for s in t.stride()[:3])
+    return t if ok else t.contiguous().clone() if t.is_contiguous() else t.contiguous()
+
+
+_HEAD_DIMS = (16, 32, 64, 128)
+
+
+def _check_cache(cache_k, cache_v, sinks: int):
+    if cache_k.dim() != 4 or cache_k.shape != cache_v.shape:
+        raise ValueError(f"caches {tuple(cache_k.shape)} and {tuple(cache_v.shape)}: expected two of (batch, kv_heads, "
+                         "sinks + window, head_dim)")
+    if cache_k.shape[3] not in _HEAD_DIMS:
+        raise ValueError(f"head_dim {cache_k.shape[3]}: expected one of {_HEAD_DIMS}")
+    if not 0 <= sinks < cache_k.shape[2]:
+        raise ValueError(f"sinks {sinks}: expected 0 <= sinks < {cache_k.shape[2]} slots")
+    _dtype_code(cache_k)
+    _alike(cache_k, cache_k.dtype, cache_v=cache_v)
+    for c in (cache_k, cache_v):
+        if not c.is_contiguous() or c.data_ptr() % 16:
+            raise ValueError("the caches are contiguous, from a 16-byte boundary on")
+    if cache_k.numel() and cache_k.data_ptr() == cache_v.data_ptr():
+        raise ValueError("cache_k and cache_v are the same memory")
 
 
 # ------------------------------------------------------------------------------------ heads / losses
@@ -1654,6 +1857,67 @@ class _CrossEntropyFn(torch.autograd.Function):
 
 def cross_entropy(logits, targets, ignore_index: int):
     return _CrossEntropyFn.apply(logits, targets, ignore_index)
+
+
+class _DistillFn(torch.autograd.Function):
+    """tau^2 KL(teacher's list || softmax over the catalogue), mean over the rows with a list (csrc/distill.hip)."""
+
+    @staticmethod
+    def forward(ctx, x, ids, teacher, temperature: float):
+        n, V = x.shape
+        top = ids.shape[1]
+        state = torch.empty(n, 2, device=x.device, dtype=torch.float32)
+        prob = torch.empty(n, top, device=x.device, dtype=torch.float32)
+        out = torch.empty(2, device=x.device, dtype=torch.float32)
+        with torch.cuda.device(x.device):
+            ws, nb = _ws_bytes("asme_distill_xent_workspace", n, V, device=x.device)
+            call("asme_distill_xent_fwd", ptr(x), x.stride(0), n, V, ptr(ids), ptr(teacher), top, temperature,
+                 _dtype_code(x), ptr(state), ptr(prob), ptr(ws), nb, ptr(out), stream())
+        ctx.save_for_backward(x, ids, state, prob, out)
+        ctx.temperature = temperature
+        return out[0]
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dloss):
+        x, ids, state, prob, out = ctx.saved_tensors
+        n, V = x.shape
+        g = torch.empty(n, V, device=x.device, dtype=x.dtype)
+        with torch.cuda.device(x.device):
+            call("asme_distill_xent_bwd", ptr(x), x.stride(0), n, V, ptr(ids), ids.shape[1], ctx.temperature,
+                 _dtype_code(x), ptr(state), ptr(prob), ptr(out), ptr(_f32(dloss.reshape(1))), ptr(g), V, stream())
+        return g, None, None, None
+
+
+def distill_cross_entropy(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits: torch.Tensor,
+                          temperature: float = 1.0) -> torch.Tensor:
+    """Distillation from a teacher's best items: for logits (..., V) and the teacher's lists teacher_ids,
+    teacher_logits (..., k <= 1024; e.g. of catalog_topk), the scalar
+        temperature^2 * KL(softmax(teacher_logits / temperature) over the list || softmax(logits / temperature) over V),
+    mean over the rows whose list is not empty (NaN when all are).  Entries whose id is not in [0, V) (-1 ends a shorter
+    list) are absent; an item twice on a list counts twice.  The gradient goes to `logits`; the teacher takes none.
+    logits float32 or bfloat16, the loss float32."""
+    V, top = logits.shape[-1], teacher_ids.shape[-1]
+    if teacher_ids.shape != teacher_logits.shape or teacher_ids.shape[:-1] != logits.shape[:-1]:
+        raise ValueError(f"logits {tuple(logits.shape)}, teacher_ids {tuple(teacher_ids.shape)} and teacher_logits "
+                         f"{tuple(teacher_logits.shape)}: expected (..., V) and twice (..., k)")
+    if not 1 <= top <= 1024 or V < 1:
+        raise ValueError(f"{V} items and lists of {top}: expected at least one item and 1 to 1024 entries")
+    if teacher_ids.is_floating_point() or teacher_ids.dtype == torch.bool:
+        raise TypeError(f"teacher_ids are whole numbers, got {teacher_ids.dtype}")
+    if not 0.0 < temperature < math.inf:
+        raise ValueError(f"temperature {temperature}: expected a positive number")
+    if torch.is_grad_enabled() and teacher_logits.requires_grad:
+        raise ValueError("distill_cross_entropy gives the teacher no gradient: detach teacher_logits")
+    _dtype_code(logits)
+    _alike(logits, teacher_ids=teacher_ids, teacher_logits=teacher_logits)
+    x = logits.reshape(-1, V)
+    if x.shape[0] == 0:
+        return x.float().sum() * math.nan  # the mean over no rows
+    if x.stride(1) != 1 or x.stride(0) < V:
+        x = x.contiguous()
+    return _DistillFn.apply(x, _i64(teacher_ids).reshape(-1, top), teacher_logits.float().reshape(-1, top).contiguous(),
+                            float(temperature))
 
 
 def linear_xent_ok(hidden: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None) -> bool:
