@@ -1650,6 +1650,125 @@ def attention(qkv, key_valid, heads: int, causal: bool, p_drop: float = 0.0, ker
     return _AttentionFn.apply(qkv, key_valid, heads, causal, p_drop, kernels)
 
 
+def _strides(*ts):
+    """the (batch, token, head) element strides of (B, L, heads, head_dim) tensors as a host array"""
+    return (ctypes_i64 * (3 * len(ts)))(*(x for t in ts for x in t.stride()[:3]))
+
+
+def _window_forward(q, k, v, valid, window, sinks, causal, scale, with_state):
+    B, L, H, D = q.shape
+    out = torch.empty(B, L, H, D, device=q.device, dtype=q.dtype)
+    state = torch.empty(B, H, L, 2, device=q.device, dtype=torch.float32) if with_state else None
+    with torch.cuda.device(q.device):
+        call("asme_window_attention_fwd", ptr(q), ptr(k), ptr(v), ptr(out), _strides(q, k, v, out), ptr(valid), B, H,
+             k.shape[2], L, D, window, sinks, int(causal), scale, _dtype_code(q), ptr(state), stream())
+    return out, state
+
+
+def _window_backward(q, k, v, valid, out, state, dout, grads, window, sinks, causal, scale):
+    B, L, H, D = q.shape
+    dout = _strided_heads(dout)
+    with torch.cuda.device(q.device):
+        ws, nb = _ws_bytes("asme_window_attention_bwd_workspace", B, H, k.shape[2], L, D, window, sinks, _dtype_code(q),
+                           device=q.device)
+        call("asme_window_attention_bwd", ptr(q), ptr(k), ptr(v), ptr(out), ptr(dout), *(ptr(g) for g in grads),
+             _strides(q, k, v, out, dout, *grads), ptr(valid), B, H, k.shape[2], L, D, window, sinks, int(causal),
+             scale, _dtype_code(q), ptr(state), ptr(ws), nb, stream())
+
+
+class _WindowAttentionFn(torch.autograd.Function):
+    """Sliding-window attention with sinks (csrc/window.hip) on separate q, k, v."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, valid, *how):
+        out, state = _window_forward(q, k, v, valid, *how, any(ctx.needs_input_grad[:3]))
+        ctx.save_for_backward(q, k, v, valid, out, state)
+        ctx.how = how
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        q, k, v, valid, out, state = ctx.saved_tensors
+        grads = [torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in (q, k, v)]
+        _window_backward(q, k, v, valid, out, state, dout, grads, *ctx.how)
+        return (*grads, *([None] * (1 + len(ctx.how))))
+
+
+class _WindowAttentionQKVFn(torch.autograd.Function):
+    """The same on one (B, L, heads + 2 kv_heads, head_dim) projection; its gradient is one buffer too."""
+
+    @staticmethod
+    def forward(ctx, qkv, valid, heads: int, *how):
+        kv = (qkv.shape[2] - heads) // 2
+        out, state = _window_forward(*qkv.split((heads, kv, kv), 2), valid, *how, ctx.needs_input_grad[0])
+        ctx.save_for_backward(qkv, valid, out, state)
+        ctx.how, ctx.parts = how, (heads, kv, kv)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        qkv, valid, out, state = ctx.saved_tensors
+        grad = torch.empty(qkv.shape, device=qkv.device, dtype=qkv.dtype)
+        _window_backward(*qkv.split(ctx.parts, 2), valid, out, state, dout, grad.split(ctx.parts, 2), *ctx.how)
+        return (grad, None, None, *([None] * len(ctx.how)))
+
+
+def _check_window(q, heads: int, kv_heads: int, D: int, window: int, sinks: int, valid, scale):
+    if heads < 1 or kv_heads < 1 or heads % kv_heads:
+        raise ValueError(f"{heads} query heads for {kv_heads} key heads: expected a multiple")
+    if D not in _HEAD_DIMS:
+        raise ValueError(f"head_dim {D}: expected one of {_HEAD_DIMS}")
+    if window < 1 or sinks < 0:
+        raise ValueError(f"window {window}, sinks {sinks}: expected window >= 1, sinks >= 0")
+    if scale is not None and not 0.0 < scale < math.inf:
+        raise ValueError(f"scale {scale}: expected a positive number")
+    if valid is not None and (valid.shape != q.shape[:2] or valid.dtype not in (torch.bool, torch.uint8)):
+        raise ValueError(f"valid {tuple(valid.shape)} of {valid.dtype}: expected {tuple(q.shape[:2])} of bool")
+    _dtype_code(q)
+    _alike(q, valid=valid)
+    return D ** -0.5 if scale is None else float(scale)
+
+
+def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: int, sinks: int = 0,
+                     causal: bool = True, valid: Optional[torch.Tensor] = None,
+                     scale: Optional[float] = None) -> torch.Tensor:
+    """Attention over a sliding window with sinks: query i of a sequence sees key j iff 0 <= i - j < window or
+    (j < sinks and j <= i); without `causal` iff |i - j| < window or j < sinks.  q (B, L, heads, head_dim), k and v
+    (B, L, kv_heads, head_dim), heads a multiple of kv_heads, head_dim 16, 32, 64 or 128, float32 or bfloat16; views
+    with adjacent head values are read in place.  valid (B, L): positions that are not valid (padding) are neither
+    query nor key, whatever they hold; their rows of the output and of the gradients are 0.  scale: 1/sqrt(head_dim).
+    Valid positions hold finite numbers (a NaN there reaches other rows of its tile).  Returns (B, L, heads, head_dim)."""
+    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or k.shape[:2] != q.shape[:2] or k.shape[3] != q.shape[3]:
+        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}: expected (B, L, heads, head_dim) "
+                         "and twice (B, L, kv_heads, head_dim)")
+    scale = _check_window(q, q.shape[2], k.shape[2], q.shape[3], window, sinks, valid, scale)
+    _alike(q, q.dtype, k=k, v=v)
+    if q.numel() == 0:
+        return q * 1
+    return _WindowAttentionFn.apply(*(_strided_heads(t) for t in (q, k, v)), None if valid is None else as_u8(valid),
+                                    int(window), int(sinks), bool(causal), scale)
+
+
+def window_attention_qkv(qkv: torch.Tensor, heads: int, window: int, sinks: int = 0, causal: bool = True,
+                         valid: Optional[torch.Tensor] = None, scale: Optional[float] = None) -> torch.Tensor:
+    """window_attention on a fused projection qkv (B, L, (heads + 2 kv_heads) * head_dim) with heads = kv_heads, the
+    layout ops.attention takes; returns (B, L, heads * head_dim)."""
+    if qkv.dim() != 3 or heads < 1 or qkv.shape[2] % (3 * heads):
+        raise ValueError(f"qkv {tuple(qkv.shape)}: expected (B, L, 3 * {heads} * head_dim)")
+    B, L = qkv.shape[:2]
+    D = qkv.shape[2] // (3 * heads)
+    scale = _check_window(qkv, heads, heads, D, window, sinks, valid, scale)
+    if qkv.numel() == 0:
+        return qkv[..., :heads * D] * 1
+    out = _WindowAttentionQKVFn.apply(_strided_heads(qkv.view(B, L, 3 * heads, D) if qkv.is_contiguous() else
+                                                     qkv.contiguous().view(B, L, 3 * heads, D)),
+                                      None if valid is None else as_u8(valid), heads, int(window), int(sinks),
+                                      bool(causal), scale)
+    return out.view(B, L, heads * D)
+
+
 def window_cache_fill(cache_k: torch.Tensor, cache_v: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                       lengths: torch.Tensor, sinks: int = 0):
     """Lay prompts into ring caches (asme_window_cache_fill), in place: k, v (B, L, kv_heads, head_dim), of which

@@ -298,3 +298,90 @@ def test_window_cache_fill(asme, dev, dtype, b, n, kv, d, window, sinks):
             want[0][u, :, ring(p, sinks, window)], want[1][u, :, ring(p, sinks, window)] = k[u, p], v[u, p]
     asme.ops.window_cache_fill(ck, cv, k, v, lengths.cuda(), sinks=sinks)
     assert torch.equal(ck, want[0]) and torch.equal(cv, want[1])
+
+
+# ------------------------------------------------------------------------------------------------ window attention
+def seen64(n, window, sinks, causal, valid):
+    i, j = torch.arange(n)[:, None], torch.arange(n)[None]
+    if causal:
+        m = ((i - j < window) | (j < sinks)) & (j <= i)
+    else:
+        m = ((i - j).abs() < window) | (j < sinks)
+    return m[None] & valid[:, None, :] & valid[:, :, None]
+
+
+def window64(q, k, v, dout, window, sinks, causal, valid, scale):
+    """out, dq, dk, dv in 64 bits, and for each the size that its error is counted in"""
+    q, k, v, dout = (t.detach().double().cpu().transpose(1, 2) for t in (q, k, v, dout))
+    group = q.shape[1] // k.shape[1]
+    ok = valid[:, None, :, None]
+    q, k, v, dout = (torch.where(ok, t, 0.0) for t in (q, k, v, dout))
+    k, v = k.repeat_interleave(group, 1), v.repeat_interleave(group, 1)
+    m = seen64(q.shape[2], window, sinks, causal, valid)[:, None]
+    kt, vt = k.transpose(-1, -2), v.transpose(-1, -2)
+    s = (q @ kt * scale).masked_fill(~m, -math.inf)
+    p = torch.softmax(s, -1).nan_to_num(0.0)
+    out = p @ v
+    dp = dout @ vt
+    delta = (dout * out).sum(-1, keepdim=True)
+    ds = p * (dp - delta)
+    share = lambda t: t.unflatten(1, (-1, group)).sum(2)  # noqa: E731
+    res = [out, ds @ k * scale, share(ds.transpose(-1, -2) @ q * scale), share(p.transpose(-1, -2) @ dout)]
+    # a score is off by es u (its products' terms, one rounding per added k step), so p by a factor 1 + 2 es u;
+    # dP and D by 24 u of their terms
+    a = scale * (q.abs() @ kt.abs()) * m
+    es = 2 * (24 * a.amax(-1, keepdim=True) + 16)
+    dps = (dout.abs() @ vt.abs() + (dout.abs() * (p @ v.abs())).sum(-1, keepdim=True)) * m
+    dss = p * (dps * (24 + 2 * es))
+    sizes = [es * (p @ v.abs()), dss @ k.abs() * scale, share(dss.transpose(-1, -2) @ q.abs() * scale),
+             share((p * es).transpose(-1, -2) @ dout.abs())]
+    # terms of the sums over keys and queries, for sums of rounded (bf16) weights
+    terms = [p @ v.abs(), (ds.abs() @ k.abs()) * scale, share(ds.abs().transpose(-1, -2) @ q.abs() * scale),
+             share(p.transpose(-1, -2) @ dout.abs())]
+    # what the rounding of the saved output adds to D, and so to dS = P (dP - D)
+    half = (dout.abs() * out.abs()).sum(-1, keepdim=True) * p
+    more = [torch.zeros_like(out), half @ k.abs() * scale, share(half.transpose(-1, -2) @ q.abs() * scale), 0 * res[3]]
+    return tuple([t.transpose(1, 2) for t in x] for x in (res, sizes, terms, more))
+
+
+def check_window(got, dtype, q, k, v, dout, window, sinks, causal, valid, scale, n):
+    res, sizes, terms, more = window64(q, k, v, dout, window, sinks, causal, valid, scale)
+    for x, ref, size, term, extra, name in zip(got, res, sizes, terms, more, ("out", "dq", "dk", "dv")):
+        # sums over n keys or queries: n / 16 products in a row on an accumulator
+        room = size + (n / 16 + 32) * term
+        if dtype == torch.bfloat16:
+            # P and dS rounded to bf16, the output that D is formed from too: bf16 keeps 8 significant bits, so half a
+            # step is at most 2^-8 = 2^16 u of the value (1 + 2^-8 <= x < 1 + 2^-7 rounds by up to 2^-8)
+            room = room + 2.0 ** 16 * (term * (1 + 2 ** -6) + extra)
+        near(x, ref, room, 1, name)
+        assert (x[~valid.to(x.device)] == 0).all(), name
+
+
+WINDOW_CASES = [  # batch, length, heads, kv_heads, head_dim, window, sinks, causal, padding
+    (1, 1, 1, 1, 16, 1, 0, True, False), (2, 3, 2, 1, 32, 2, 1, True, True), (3, 50, 2, 2, 32, 16, 1, True, True),
+    (2, 64, 4, 2, 64, 64, 0, True, False), (2, 65, 2, 2, 128, 7, 3, True, True), (1, 200, 3, 1, 64, 64, 2, True, False),
+    (2, 257, 2, 2, 16, 31, 40, True, True), (1, 300, 2, 1, 128, 1000, 0, True, True),
+    (1, 700, 4, 1, 32, 130, 70, True, True), (2, 200, 2, 2, 64, 33, 5, False, True), (1, 513, 3, 3, 32, 1, 0, False, False),
+    (2, 70, 4, 4, 128, 5, 66, False, True), (1, 530, 4, 2, 64, 100, 13, False, True),
+    (1, 1200, 2, 1, 64, 5, 1, True, False), (1, 1031, 8, 1, 128, 257, 300, True, True),
+    (70, 17, 1, 1, 16, 4, 2, True, True)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("b,n,h,kv,d,window,sinks,causal,padding", WINDOW_CASES)
+def test_window_attention(asme, dev, dtype, b, n, h, kv, d, window, sinks, causal, padding):
+    g = torch.Generator().manual_seed(1)
+    valid = torch.ones(b, n, dtype=torch.bool)
+    if padding:  # right padding, a hole, and (of several) a sequence with nothing in it
+        valid = torch.arange(n) < torch.randint(1, n + 1, (b, 1), generator=g)
+        valid[:, n // 3] = False
+        if b > 1:
+            valid[1] = False
+    q, k, v, dout = (rand(b, n, x, d, seed=i, dtype=dtype, scale=1.5) for i, x in ((2, h), (3, kv), (4, kv), (5, h)))
+    for t, junk in ((q, math.nan), (k, math.inf), (v, math.nan), (dout, -math.inf)):
+        t[~valid.cuda()] = junk  # padding may hold anything
+    q, k, v = (t.requires_grad_() for t in (q, k, v))
+    out = asme.ops.window_attention(q, k, v, window, sinks=sinks, causal=causal,
+                                    valid=valid.cuda() if padding else None)
+    got = [out, *torch.autograd.grad(out, (q, k, v), dout)]
+    check_window(got, dtype, q, k, v, dout, window, sinks, causal, valid, d ** -0.5, n)
