@@ -99,7 +99,7 @@ __global__ __launch_bounds__(kThreads) void step_kernel(StepArgs a) {
         }
 #pragma unroll
         for (int u = 0; u < kRows; ++u) {
-            if (r0 + u * NG == to && chunk == 0) {
+            if (r0 + u * NG == to && to < end && chunk == 0) {  // (behind `end` the row is another workgroup's)
                 Elem<T>::store(ck + to * D + sub * V, kk[u]);
                 Elem<T>::store(cv + to * D + sub * V, vv[u]);
             }

@@ -282,6 +282,23 @@ def test_window_attention_step(asme, dev, dtype, b, h, kv, d, window, sinks):
         assert torch.equal(got.view(torch.int16), ref.view(torch.int16)), "the cache beside the new slot"
 
 
+@pytest.mark.parametrize("odd", [0, 1])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_window_attention_step_stores_at_every_slot(asme, dev, dtype, odd):
+    """the slots of a sequence are cut over workgroups: the new token is stored once, whichever of them it falls to"""
+    b, d, slots = 261, 64, 521
+    k, v, q = (rand(b, 1, d, seed=i, dtype=dtype) for i in (1, 2, 3))
+    ck, cv = (rand(b, 1, slots, d, seed=i, dtype=dtype) for i in (4, 5))
+    n = 2 * torch.arange(b) + odd + 521  # the ring has come round once
+    want = ck.clone(), cv.clone()
+    for u in range(b):
+        to = ring(int(n[u]), 3, slots - 3)
+        want[0][u, :, to], want[1][u, :, to] = k[u], v[u]
+    for _ in range(3):
+        asme.ops.window_attention_step(q, k, v, ck, cv, n.cuda(), sinks=3)
+        assert torch.equal(ck, want[0]) and torch.equal(cv, want[1])
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("b,n,kv,d,window,sinks", [(1, 1, 1, 16, 1, 0), (3, 9, 2, 32, 4, 2), (4, 50, 1, 64, 16, 5),
                                                    (2, 20, 3, 128, 64, 1), (5, 130, 2, 16, 31, 0)])
