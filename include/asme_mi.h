@@ -504,7 +504,8 @@ int asme_window_attention_fwd(const void* q, const void* k, const void* v, void*
                               int64_t head_dim, int64_t window, int64_t sinks, int causal, float scale, int dtype,
                               float* state, void* stream);
 int64_t asme_window_attention_bwd_workspace(int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq_len,
-                                            int64_t head_dim, int64_t window, int64_t sinks, int dtype);
+                                            int64_t head_dim, int64_t window, int64_t sinks, int causal,
+                                            int dtype);
 /* strides: of q, k, v, out, dout, dq, dk, dv (24 values); dq, dk, dv may be column blocks of one buffer */
 int asme_window_attention_bwd(const void* q, const void* k, const void* v, const void* out, const void* dout, void* dq,
                               void* dk, void* dv, const int64_t* strides, const uint8_t* valid, int64_t batch,

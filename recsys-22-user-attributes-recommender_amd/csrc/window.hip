@@ -86,7 +86,7 @@ struct Args {
     float* part;           // partial dK, dV: (key head, split block, piece, 2, rows, dim)
     int seq_len, dim, heads, kv_heads, group, window, sinks, causal;
     int blocks;            // stationary blocks of a sequence
-    int64_t items, per_xcd;
+    uint32_t items, per_xcd;  // workgroups of the pass, those of an XCD
     // dK, dV: the first `far_blocks` key blocks hold sinks, which every later query sees: cut into far_pieces pieces;
     // the others into near_pieces
     int far_blocks, far_pieces, near_pieces;
@@ -98,15 +98,15 @@ template <class T>
 struct Chunk;
 template <>
 struct Chunk<float> {
-    float4 a, b;
+    floatx4 a, b;
     __device__ __forceinline__ void load(const float* p) {
-        a = *reinterpret_cast<const float4*>(p);
-        b = *reinterpret_cast<const float4*>(p + 4);
+        a = *reinterpret_cast<const floatx4*>(p);
+        b = *reinterpret_cast<const floatx4*>(p + 4);
     }
-    __device__ __forceinline__ void zero() { a = b = make_float4(0.f, 0.f, 0.f, 0.f); }
+    __device__ __forceinline__ void zero() { a = b = floatx4{0.f, 0.f, 0.f, 0.f}; }
     __device__ __forceinline__ Frag<3> frag() const {
-        const Bf3 s = split_bf3(a, b);
-        return {s.h, s.m, s.l};
+        const float x[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+        return frag_of(x, (Frag<3>*)nullptr);
     }
 };
 template <>
@@ -127,7 +127,8 @@ struct Pass {
     static constexpr int kThreads = NW * 64;
     static constexpr int kChunks = kTS * (DP / 8);      // 16-byte chunks of one tensor's tile (per plane)
     static constexpr int kEach = 2 * kChunks / kThreads;
-    static_assert(2 * kChunks % kThreads == 0, "whole chunks per thread");
+    static constexpr int kRowStep = kThreads / (DP / 8);  // rows that the workgroup covers in one go
+    static_assert(kChunks % kThreads == 0, "a thread's first chunks are of the first tensor, the others of the second");
     // two tensors side by side in one image up to 64 columns, in an image each at 128
     static constexpr int kImages = DP == 128 ? 2 : 1;
     static constexpr int kBytes = NP * kImages * kImage;
@@ -137,31 +138,46 @@ struct Pass {
         if constexpr (DP == 128) return (plane * 2 + op) * kImage + swz(row, ch);
         return plane * kImage + swz(row, ch + op * (DP / 8));
     }
-    // bit r: streamed position t0 + r is in the sequence and valid (the same in every wave)
-    static __device__ __forceinline__ uint64_t valid_rows(const Args& a, int64_t b, int t0) {
+    // is streamed position t0 + lane in the sequence and valid (the same in every wave)?  Read with the tile and looked
+    // at when the tile is: a tile waits for one latency, not for two in a row
+    static __device__ __forceinline__ int valid_row(const Args& a, int64_t b, int t0) {
         const int pos = t0 + (threadIdx.x & 63);
-        bool ok = pos >= 0 && pos < a.seq_len;
-        if (ok && a.valid) ok = a.valid[b * a.seq_len + pos] != 0;
-        return __ballot(ok);
+        if (pos >= a.seq_len) return 0;
+        return a.valid ? a.valid[b * a.seq_len + pos] : 1;
     }
+    // the tile's rows from t0 on of two tensors (base: their first row, uniform): a 32-bit offset per chunk, the same for
+    // every whole tile.  Rows behind the sequence read its last one; put() clears them.
     static __device__ __forceinline__ void fetch(Chunk<T> (&c)[kEach], const T* x0, int64_t st0, const T* x1,
-                                                 int64_t st1, int t0, uint64_t rows, int dim) {
+                                                 int64_t st1, int t0, int seq_len, int dim) {
+        const T *b0 = x0 + t0 * st0, *b1 = x1 + t0 * st1;
+        const int ch = threadIdx.x % (DP / 8) * 8;
+        const bool in = DP > 32 || ch < dim;  // (a head of 16 leaves the second half of 32 columns empty)
+        if (t0 + kTS <= seq_len) {
 #pragma unroll
-        for (int e = 0; e < kEach; ++e) {
-            const int i = e * kThreads + threadIdx.x, op = i / kChunks, row = i % kChunks / (DP / 8), ch = i % (DP / 8);
-            if (((rows >> row) & 1) && ch * 8 < dim)
-                c[e].load((op ? x1 + (t0 + row) * st1 : x0 + (t0 + row) * st0) + ch * 8);
-            else
+            for (int e = 0; e < kEach; ++e) {
+                const uint32_t row = e % (kEach / 2) * kRowStep + threadIdx.x / (DP / 8);
                 c[e].zero();
+                if (in) c[e].load(e < kEach / 2 ? b0 + (row * (uint32_t)st0 + ch) : b1 + (row * (uint32_t)st1 + ch));
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < kEach; ++e) {
+                const uint32_t row = min(e % (kEach / 2) * kRowStep + (int)threadIdx.x / (DP / 8), seq_len - 1 - t0);
+                c[e].zero();
+                if (in) c[e].load(e < kEach / 2 ? b0 + (row * (uint32_t)st0 + ch) : b1 + (row * (uint32_t)st1 + ch));
+            }
         }
     }
-    static __device__ __forceinline__ void put(char* lds, const Chunk<T> (&c)[kEach]) {
+    static __device__ __forceinline__ void put(char* lds, Chunk<T> (&c)[kEach], uint64_t rows) {
+        const int ch = threadIdx.x % (DP / 8);
 #pragma unroll
         for (int e = 0; e < kEach; ++e) {
-            const int i = e * kThreads + threadIdx.x, op = i / kChunks, row = i % kChunks / (DP / 8), ch = i % (DP / 8);
+            const int row = e % (kEach / 2) * kRowStep + threadIdx.x / (DP / 8);
+            if (rows != ~0ull && !((rows >> row) & 1)) c[e].zero();
             const F f = c[e].frag();
 #pragma unroll
-            for (int p = 0; p < NP; ++p) *reinterpret_cast<bf16x8*>(lds + place(op, p, row, ch)) = f.p[p];
+            for (int p = 0; p < NP; ++p)
+                *reinterpret_cast<bf16x8*>(lds + place(e < kEach / 2 ? 0 : 1, p, row, ch)) = f.p[p];
         }
     }
     // stationary fragments of row `row` (null: zeros)
@@ -174,50 +190,64 @@ struct Pass {
             f[ks] = c.frag();
         }
     }
-    // X[streamed row of the 32-row half `sub`][stationary row] of tensor `op`
+    // X[streamed row of the 32-row half `sub`][stationary row] of tensor `op`.  The reads of kStep k steps are issued
+    // together, so that a product waits for the first of them and not each for its own
+    static constexpr int kStep = NP == 1 ? KS : 2;
     static __device__ __forceinline__ floatx16 score(const char* lds, int op, int sub, const F (&st)[KS]) {
         const int lane = threadIdx.x & 63, r32 = lane & 31, h = lane >> 5;
         floatx16 x;
 #pragma unroll
         for (int i = 0; i < 16; ++i) x[i] = 0.f;
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-            F A;
+        for (int k0 = 0; k0 < KS; k0 += kStep) {
+            F A[kStep];
 #pragma unroll
-            for (int p = 0; p < NP; ++p)
-                A.p[p] = *reinterpret_cast<const bf16x8*>(lds + place(op, p, 32 * sub + r32, 2 * ks + h));
-            x = product(A, st[ks], x);
+            for (int ks = 0; ks < kStep; ++ks)
+#pragma unroll
+                for (int p = 0; p < NP; ++p)
+                    A[ks].p[p] = *reinterpret_cast<const bf16x8*>(lds + place(op, p, 32 * sub + r32, 2 * (k0 + ks) + h));
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int ks = 0; ks < kStep; ++ks) x = product(A[ks], st[k0 + ks], x);
         }
         return x;
     }
     // Y^T[feature][stationary row] += streamed^T . x: rows 16 s2 + 8 (j >> 2) + 4 h + (j & 3) of the half are element j of
     // the lane's B fragment; 16-lane group (h, fh) reads rows + q x features 32 ft + 16 fh + 4 p4 .. + 3 transposed
+    static __device__ __forceinline__ void read_transposed(const char* lds, int op, int sub, int s2, F (&A)[NFT]) {
+        const int lane = threadIdx.x & 63, h = lane >> 5, fh = (lane >> 4) & 1, q = (lane & 15) >> 2, p4 = lane & 3;
+        const int lo = 32 * sub + 16 * s2 + 4 * h + q;
+#pragma unroll
+        for (int ft = 0; ft < NFT; ++ft) {
+            const int ch = 4 * ft + 2 * fh + (p4 >> 1);
+#pragma unroll
+            for (int p = 0; p < NP; ++p) {
+                const short4v a = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    (lds_short4*)(lds + place(op, p, lo, ch) + 8 * (p4 & 1)));
+                const short4v b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    (lds_short4*)(lds + place(op, p, lo + 8, ch) + 8 * (p4 & 1)));
+                typedef short short8v __attribute__((ext_vector_type(8)));
+                const short8v c = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+                A[ft].p[p] = __builtin_bit_cast(bf16x8, c);
+            }
+        }
+    }
+    static __device__ __forceinline__ F weights_of(const floatx16& x, int s2) {
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = x[8 * s2 + j];
+        return frag_of(v, (F*)nullptr);
+    }
     static __device__ __forceinline__ void gather(const char* lds, int op, int sub, const floatx16& x,
                                                   floatx16 (&y)[NFT]) {
-        const int lane = threadIdx.x & 63, h = lane >> 5, fh = (lane >> 4) & 1, q = (lane & 15) >> 2, p4 = lane & 3;
 #pragma unroll
         for (int s2 = 0; s2 < 2; ++s2) {
-            float v[8];
+            F A[NFT];
+            read_transposed(lds, op, sub, s2, A);
+            __builtin_amdgcn_sched_barrier(0);
+            const F P = weights_of(x, s2);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = x[8 * s2 + j];
-            const F P = frag_of(v, (F*)nullptr);
-            const int lo = 32 * sub + 16 * s2 + 4 * h + q;
-#pragma unroll
-            for (int ft = 0; ft < NFT; ++ft) {
-                const int ch = 4 * ft + 2 * fh + (p4 >> 1);
-                F A;
-#pragma unroll
-                for (int p = 0; p < NP; ++p) {
-                    const short4v a = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                        (lds_short4*)(lds + place(op, p, lo, ch) + 8 * (p4 & 1)));
-                    const short4v b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                        (lds_short4*)(lds + place(op, p, lo + 8, ch) + 8 * (p4 & 1)));
-                    typedef short short8v __attribute__((ext_vector_type(8)));
-                    const short8v c = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-                    A.p[p] = __builtin_bit_cast(bf16x8, c);
-                }
-                y[ft] = product(A, P, y[ft]);
-            }
+            for (int ft = 0; ft < NFT; ++ft) y[ft] = product(A[ft], P, y[ft]);
         }
     }
     // row `row` (features 32 ft + 8 i + 4 h .. + 3 of this lane's stationary row) = y * f
@@ -247,12 +277,22 @@ struct Pass {
     }
 };
 
-// Does query i see key j (both valid)?
-__device__ __forceinline__ bool sees(const Args& a, int i, int j) {
-    const int back = i - j;
-    if (a.causal) return back >= 0 && (back < a.window || j < a.sinks);
-    return (back < a.window && -back < a.window) || j < a.sinks;
+// bits 0 .. n (none for n < 0, all from n = 31 on)
+__device__ __forceinline__ uint32_t upto(int n) { return n < 0 ? 0u : n >= 31 ? ~0u : (2u << n) - 1u; }
+// bit r: query i sees key j0 + r
+__device__ __forceinline__ uint32_t keys_seen(const Args& a, int i, int j0) {
+    const uint32_t after = ~upto(i - a.window - j0), sinks = upto(a.sinks - 1 - j0);  // j > i - window; j < sinks
+    if (a.causal) return upto(i - j0) & (after | sinks);
+    return (upto(i + a.window - 1 - j0) & after) | sinks;
 }
+// bit r: query i0 + r sees key j
+__device__ __forceinline__ uint32_t queries_seen(const Args& a, int i0, int j) {
+    const uint32_t before = j < a.sinks ? ~0u : upto(j + a.window - 1 - i0);  // i < j + window, or any
+    if (a.causal) return before & ~upto(j - 1 - i0);
+    return j < a.sinks ? ~0u : before & ~upto(j - a.window - i0);
+}
+// bit of accumulator register e among the 32 rows' bits, those shifted down by 4 h
+__device__ __forceinline__ bool row_bit(uint32_t bits, int e) { return (bits >> ((e & 3) + 8 * (e >> 2))) & 1u; }
 // The block of queries i0 .. i0 + 31 and keys j0 .. j0 + 31, by its corners: 0 no pair visible, 2 every pair, 1 some
 __device__ __forceinline__ int block_seen(const Args& a, int i0, int j0) {
     const int most = i0 + 31 - j0, least = i0 - (j0 + 31);  // i - j over the block
@@ -267,9 +307,9 @@ __device__ __forceinline__ int block_seen(const Args& a, int i0, int j0) {
 
 // workgroup -> item: neighbours (blocks of the same head, which read the same streamed rows) on one XCD, so that they
 // share its L2 (the dispatcher deals workgroups round-robin over the 8 XCDs; only a matter of speed)
-__device__ __forceinline__ bool item_of(const Args& a, int64_t& item) {
-    item = (int64_t)(blockIdx.x % 8) * a.per_xcd + blockIdx.x / 8;
-    return item < a.items && (int64_t)(blockIdx.x / 8) < a.per_xcd;
+__device__ __forceinline__ bool item_of(const Args& a, uint32_t& item) {
+    item = blockIdx.x % 8 * a.per_xcd + blockIdx.x / 8;
+    return item < a.items;
 }
 
 // The streamed key tiles of queries [q0, q1): those of the sinks in front of the window's first tile, then the window's.
@@ -289,13 +329,14 @@ template <class T, int DP, int NW>
 __global__ __launch_bounds__(NW * 64) void forward_kernel(Args a) {
     using P = Pass<T, DP, NW>;
     __shared__ __attribute__((aligned(16))) char lds[P::kBytes];
-    int64_t item;
+    uint32_t item;
     if (!item_of(a, item)) return;  // (the whole workgroup)
     const int lane = threadIdx.x & 63, h = lane >> 5, r32 = lane & 31;
-    const int block = (int)(item % a.blocks), head = (int)(item / a.blocks % a.heads);
-    const int64_t b = item / a.blocks / a.heads;
+    const uint32_t row = item / (uint32_t)a.blocks;  // sequence and head
+    const int block = (int)(item - row * a.blocks), head = (int)(row % (uint32_t)a.heads);
+    const int64_t b = row / (uint32_t)a.heads;
     const int q0 = block * NW * 32, q1 = min(a.seq_len, q0 + NW * 32);
-    const int w0 = q0 + (threadIdx.x >> 6) * 32, qi = w0 + r32;
+    const int w0 = q0 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 32, qi = w0 + r32;
     const bool live = qi < a.seq_len && (!a.valid || a.valid[b * a.seq_len + qi]);
     const bool any = __ballot(live) != 0;
     typename P::F Q[P::KS];
@@ -308,26 +349,23 @@ __global__ __launch_bounds__(NW * 64) void forward_kernel(Args a) {
     const T* V = a.v.at<T>(b, head / a.group);
     const KeyTiles tiles(a, q0, q1);
     Chunk<T> next[P::kEach];
-    int i = 0, t0 = 0;
-    uint64_t rows = 0;
-    auto advance = [&]() {  // the next tile with a valid position, on its way
-        for (; i < tiles.count; ++i) {
-            t0 = tiles.start(i);
-            rows = P::valid_rows(a, b, t0);
-            if (rows) break;
-        }
-        if (i < tiles.count) P::fetch(next, K, a.k.st, V, a.v.st, t0, rows, a.dim);
+    int i = 0, t0 = 0, valid = 0;
+    auto issue = [&]() {  // tile i, on its way
+        if (i >= tiles.count) return;
+        t0 = tiles.start(i);
+        valid = P::valid_row(a, b, t0);
+        P::fetch(next, K, a.k.st, V, a.v.st, t0, a.seq_len, a.dim);
     };
-    if (__syncthreads_or(any)) advance();
+    if (__syncthreads_or(any)) issue();
     else i = tiles.count;
     while (i < tiles.count) {
         const int k0 = t0;
-        const uint64_t keys = rows;
+        const uint64_t keys = __ballot(valid != 0);
         __syncthreads();  // the last tile has been read
-        P::put(lds, next);
+        P::put(lds, next, keys);
         __syncthreads();
         ++i;
-        advance();
+        issue();
         if (!any) continue;
 #pragma unroll
         for (int sub = 0; sub < 2; ++sub) {
@@ -336,11 +374,9 @@ __global__ __launch_bounds__(NW * 64) void forward_kernel(Args a) {
             if (!seen) continue;
             floatx16 x = P::score(lds, 0, sub, Q);
             if (seen == 1 || ok != 0xFFFFFFFFu) {
+                const uint32_t bits = (ok & keys_seen(a, qi, j0)) >> (4 * h);
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const int r = acc_row(e, h);
-                    x[e] = ((ok >> r) & 1) && sees(a, qi, j0 + r) ? x[e] : -INFINITY;
-                }
+                for (int e = 0; e < 16; ++e) x[e] = row_bit(bits, e) ? x[e] : -INFINITY;
             }
             float t = x[0];
 #pragma unroll
@@ -379,13 +415,14 @@ template <class T, int DP, int NW>
 __global__ __launch_bounds__(NW * 64) void dq_kernel(Args a) {
     using P = Pass<T, DP, NW>;
     __shared__ __attribute__((aligned(16))) char lds[P::kBytes];
-    int64_t item;
+    uint32_t item;
     if (!item_of(a, item)) return;
     const int lane = threadIdx.x & 63, h = lane >> 5, r32 = lane & 31;
-    const int block = (int)(item % a.blocks), head = (int)(item / a.blocks % a.heads);
-    const int64_t b = item / a.blocks / a.heads;
+    const uint32_t row = item / (uint32_t)a.blocks;  // sequence and head
+    const int block = (int)(item - row * a.blocks), head = (int)(row % (uint32_t)a.heads);
+    const int64_t b = row / (uint32_t)a.heads;
     const int q0 = block * NW * 32, q1 = min(a.seq_len, q0 + NW * 32);
-    const int w0 = q0 + (threadIdx.x >> 6) * 32, qi = w0 + r32;
+    const int w0 = q0 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 32, qi = w0 + r32;
     const bool live = qi < a.seq_len && (!a.valid || a.valid[b * a.seq_len + qi]);
     const bool any = __ballot(live) != 0;
     typename P::F Q[P::KS], O[P::KS];
@@ -422,26 +459,23 @@ __global__ __launch_bounds__(NW * 64) void dq_kernel(Args a) {
     const T* V = a.v.at<T>(b, head / a.group);
     const KeyTiles tiles(a, q0, q1);
     Chunk<T> next[P::kEach];
-    int i = 0, t0 = 0;
-    uint64_t rows = 0;
-    auto advance = [&]() {
-        for (; i < tiles.count; ++i) {
-            t0 = tiles.start(i);
-            rows = P::valid_rows(a, b, t0);
-            if (rows) break;
-        }
-        if (i < tiles.count) P::fetch(next, K, a.k.st, V, a.v.st, t0, rows, a.dim);
+    int i = 0, t0 = 0, valid = 0;
+    auto issue = [&]() {  // tile i, on its way
+        if (i >= tiles.count) return;
+        t0 = tiles.start(i);
+        valid = P::valid_row(a, b, t0);
+        P::fetch(next, K, a.k.st, V, a.v.st, t0, a.seq_len, a.dim);
     };
-    if (__syncthreads_or(any)) advance();
+    if (__syncthreads_or(any)) issue();
     else i = tiles.count;
     while (i < tiles.count) {
         const int k0 = t0;
-        const uint64_t keys = rows;
-        __syncthreads();
-        P::put(lds, next);
+        const uint64_t keys = __ballot(valid != 0);
+        __syncthreads();  // the last tile has been read
+        P::put(lds, next, keys);
         __syncthreads();
         ++i;
-        advance();
+        issue();
         if (!any) continue;
 #pragma unroll
         for (int sub = 0; sub < 2; ++sub) {
@@ -450,16 +484,14 @@ __global__ __launch_bounds__(NW * 64) void dq_kernel(Args a) {
             if (!seen) continue;
             floatx16 x = P::score(lds, 0, sub, Q);
             const floatx16 dp = P::score(lds, 1, sub, O);
-            const bool test = seen == 1 || ok != 0xFFFFFFFFu;
+            if (seen == 1 || ok != 0xFFFFFFFFu) {
+                const uint32_t bits = (ok & keys_seen(a, qi, j0)) >> (4 * h);
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                float p = __builtin_amdgcn_exp2f(fmaf(x[e], c, -st.x)) * st.y;
-                if (test) {
-                    const int r = acc_row(e, h);
-                    p = ((ok >> r) & 1) && sees(a, qi, j0 + r) ? p : 0.f;
-                }
-                x[e] = p * (dp[e] - delta);
+                for (int e = 0; e < 16; ++e) x[e] = row_bit(bits, e) ? x[e] : -INFINITY;
             }
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+                x[e] = __builtin_amdgcn_exp2f(fmaf(x[e], c, -st.x)) * st.y * (dp[e] - delta);
             P::gather(lds, 0, sub, x, y);
         }
     }
@@ -476,13 +508,14 @@ __global__ __launch_bounds__(NW * 64) void dkv_kernel(Args a) {
     using P = Pass<T, DP, NW>;
     __shared__ __attribute__((aligned(16))) char lds[P::kBytes];
     __shared__ __attribute__((aligned(16))) float meta[3][kTS];  // maximum, 1 / sum, D of the tile's queries
-    int64_t item;
+    uint32_t item;
     if (!item_of(a, item)) return;
     const int lane = threadIdx.x & 63, h = lane >> 5, r32 = lane & 31;
     const int near = a.blocks - a.far_blocks, per_head = a.far_blocks * a.far_pieces + near * a.near_pieces;
-    const int64_t bk = item / per_head, b = bk / a.kv_heads;
-    const int kh = (int)(bk % a.kv_heads);
-    int within = (int)(item % per_head), block, piece, pieces;
+    const uint32_t bk = item / (uint32_t)per_head;
+    const int kh = (int)(bk % (uint32_t)a.kv_heads);
+    const int64_t b = bk / (uint32_t)a.kv_heads;
+    int within = (int)(item - bk * per_head), block, piece, pieces;
     if (within < a.far_blocks * a.far_pieces) {
         pieces = a.far_pieces, block = within / pieces, piece = within % pieces;
     } else {
@@ -490,7 +523,7 @@ __global__ __launch_bounds__(NW * 64) void dkv_kernel(Args a) {
         pieces = a.near_pieces, block = a.far_blocks + within / pieces, piece = within % pieces;
     }
     const int k0 = block * NW * 32, k1 = min(a.seq_len, k0 + NW * 32);
-    const int w0 = k0 + (threadIdx.x >> 6) * 32, kj = w0 + r32;
+    const int w0 = k0 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 32, kj = w0 + r32;
     const bool live = kj < a.seq_len && (!a.valid || a.valid[b * a.seq_len + kj]);
     const bool any = __ballot(live) != 0;
     const uint32_t ok = (uint32_t)__ballot(live);  // (both halves of the lanes hold the same keys)
@@ -506,68 +539,63 @@ __global__ __launch_bounds__(NW * 64) void dkv_kernel(Args a) {
     const int lo = (a.causal ? k0 : all ? 0 : max(0, k0 - a.window + 1)) / kTS * kTS;
     const int hi = all ? a.seq_len : (int)min((int64_t)a.seq_len, (int64_t)k1 - 1 + a.window);
     const int tiles = (hi - lo + kTS - 1) / kTS, steps = tiles * a.group;
-    int i = (int)((int64_t)steps * piece / pieces), t0 = 0, head = 0;
+    int i = (int)((int64_t)steps * piece / pieces), t0 = 0;
     const int last = (int)((int64_t)steps * (piece + 1) / pieces);
-    uint64_t rows = 0;
+    int valid = 0;
     Chunk<T> next[P::kEach];
     float2 st = make_float2(INFINITY, 0.f);
     float delta = 0.f;
-    auto advance = [&]() {
-        for (; i < last; ++i) {
-            t0 = lo + i % tiles * kTS;
-            rows = P::valid_rows(a, b, t0);
-            if (rows) break;
-        }
-        if (i < last) {
-            head = kh * a.group + i / tiles;
-            P::fetch(next, a.q.at<T>(b, head), a.q.st, a.dout.at<T>(b, head), a.dout.st, t0, rows, a.dim);
-            if (threadIdx.x < kTS) {
-                const int64_t at = (b * a.heads + head) * a.seq_len + t0 + threadIdx.x;
-                st = make_float2(INFINITY, 0.f), delta = 0.f;
-                if ((rows >> threadIdx.x) & 1) st = a.state[at], delta = a.delta[at];
-            }
+    auto issue = [&]() {
+        if (i >= last) return;
+        t0 = lo + i % tiles * kTS;
+        valid = P::valid_row(a, b, t0);
+        const int head = kh * a.group + i / tiles;
+        P::fetch(next, a.q.at<T>(b, head), a.q.st, a.dout.at<T>(b, head), a.dout.st, t0, a.seq_len, a.dim);
+        if (threadIdx.x < kTS) {  // (of a query that is none: (infinity, 0) and 0)
+            const int64_t at = (b * a.heads + head) * a.seq_len + t0 + threadIdx.x;
+            st = make_float2(INFINITY, 0.f), delta = 0.f;
+            if (t0 + (int)threadIdx.x < a.seq_len) st = a.state[at], delta = a.delta[at];
         }
     };
-    if (__syncthreads_or(any)) advance();
+    if (__syncthreads_or(any)) issue();
     else i = last;
     while (i < last) {
         const int q0 = t0;
-        const uint64_t queries = rows;
+        const uint64_t queries = __ballot(valid != 0);
         __syncthreads();
-        P::put(lds, next);
+        P::put(lds, next, queries);
         if (threadIdx.x < kTS) meta[0][threadIdx.x] = st.x, meta[1][threadIdx.x] = st.y, meta[2][threadIdx.x] = delta;
         __syncthreads();
         ++i;
-        advance();
+        issue();
         if (!any) continue;
 #pragma unroll
         for (int sub = 0; sub < 2; ++sub) {
             const int i0 = q0 + 32 * sub, seen = (uint32_t)(queries >> (32 * sub)) ? block_seen(a, i0, w0) : 0;
             if (!seen) continue;
             floatx16 x = P::score(lds, 0, sub, K);
-            floatx16 dp = P::score(lds, 1, sub, V);
-            const bool test = seen == 1 || ok != 0xFFFFFFFFu;
+            if (seen == 1 || ok != 0xFFFFFFFFu) {
+                const uint32_t bits = live ? queries_seen(a, i0, kj) >> (4 * h) : 0u;
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const floatx4 m = *reinterpret_cast<const floatx4*>(&meta[0][32 * sub + 8 * g + 4 * h]);
-                const floatx4 v = *reinterpret_cast<const floatx4*>(&meta[1][32 * sub + 8 * g + 4 * h]);
-                const floatx4 d = *reinterpret_cast<const floatx4*>(&meta[2][32 * sub + 8 * g + 4 * h]);
+                for (int e = 0; e < 16; ++e) x[e] = row_bit(bits, e) ? x[e] : -INFINITY;
+            }
+            const float* m = &meta[0][32 * sub + 4 * h];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float p = __builtin_amdgcn_exp2f(fmaf(x[4 * g + e], c, -m[e])) * v[e];
-                    if (test) p = live && sees(a, i0 + 8 * g + 4 * h + e, kj) ? p : 0.f;
-                    x[4 * g + e] = p;
-                    dp[4 * g + e] = p * (dp[4 * g + e] - d[e]);
-                }
+            for (int e = 0; e < 16; ++e) {
+                const int r = 8 * (e >> 2) + (e & 3);
+                x[e] = __builtin_amdgcn_exp2f(fmaf(x[e], c, -m[r])) * m[kTS + r];
             }
             P::gather(lds, 1, sub, x, yv);
+            floatx16 dp = P::score(lds, 1, sub, V);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) dp[e] = x[e] * (dp[e] - m[2 * kTS + 8 * (e >> 2) + (e & 3)]);
             P::gather(lds, 0, sub, dp, yk);
         }
     }
     if (pieces > 1) {  // fp32 rows of this piece, zeros where there is nothing
         const int64_t far = (int64_t)a.far_blocks * (a.far_pieces > 1 ? a.far_pieces : 0);
         const int64_t split = far + (int64_t)near * (a.near_pieces > 1 ? a.near_pieces : 0);
-        const int64_t slab = bk * split + (block < a.far_blocks ? (int64_t)block * a.far_pieces
+        const int64_t slab = (int64_t)bk * split + (block < a.far_blocks ? (int64_t)block * a.far_pieces
                                                                 : far + (int64_t)(block - a.far_blocks) * a.near_pieces) +
                              piece;
         float* p = a.part + (slab * 2 * NW * 32 + (kj - k0)) * a.dim;
@@ -613,10 +641,15 @@ __global__ __launch_bounds__(256) void add_pieces_kernel(Args a, int block_rows,
 // ------------------------------------------------------------------------------------------------ host
 int padded_dim(int64_t dim) { return dim <= 32 ? 32 : (int)dim; }
 
-// waves (of 32 stationary rows) per workgroup
+// Waves (of 32 stationary rows) per workgroup: eight share a streamed tile's way through LDS, at 256 registers each; four
+// (512 registers) where a pass's fragments and sums need more; two where the sequence has no more rows.
 int waves(int64_t seq_len, int dtype, int dp) {
     if (seq_len <= 64) return 2;
-    return dtype == kF32 && dp == 128 ? 4 : 8;
+    return dp == 32 || (dtype == kF32 && dp == 128) ? 4 : 8;
+}
+int waves_kv(int64_t seq_len, int dtype, int dp) {
+    if (seq_len <= 64) return 2;
+    return dp == 64 && dtype == kBF16 ? 8 : 4;
 }
 
 struct Pieces {
@@ -624,17 +657,17 @@ struct Pieces {
     int64_t slabs;  // partial slabs per key head
 };
 // key blocks are cut so that none takes much longer than the others: a block with sinks is seen by every later query
-Pieces pieces_of(int64_t batch, int64_t kv_heads, int64_t group, int64_t seq_len, int64_t window, int64_t sinks, int nw) {
+Pieces pieces_of(int64_t batch, int64_t kv_heads, int64_t group, int64_t seq_len, int64_t window, int64_t sinks,
+                 int causal, int nw) {
     const int64_t rows = nw * 32, blocks = (seq_len + rows - 1) / rows;
     Pieces p;
     p.far_blocks = (int)std::min(blocks, (sinks + rows - 1) / rows);
-    const int64_t near_steps = std::min(seq_len, rows + window) * group, far_steps = seq_len * group;
+    const int64_t reach = std::min(seq_len, rows + window * (causal ? 1 : 2));
+    const int64_t near_steps = (reach + kTS - 1) / kTS * group, far_steps = (seq_len + kTS - 1) / kTS * group;
     const int64_t have = batch * kv_heads * blocks;
-    p.near_pieces = (int)std::max<int64_t>(1, std::min<int64_t>({(512 + have - 1) / have / 2 + (have >= 512 ? 0 : 1),
-                                                                  near_steps / 512, 16}));
-    if (have >= 256) p.near_pieces = 1;
-    p.far_pieces = (int)std::max<int64_t>(
-        1, std::min<int64_t>(64, far_steps / std::max<int64_t>(512, near_steps / p.near_pieces)));
+    p.near_pieces = (int)std::max<int64_t>(1, std::min<int64_t>((512 + have - 1) / have, near_steps / 6));
+    p.far_pieces = (int)std::max<int64_t>(1, far_steps / std::max<int64_t>(6, near_steps / p.near_pieces));
+    p.near_pieces = std::min(p.near_pieces, 64), p.far_pieces = std::min(p.far_pieces, 64);
     p.slabs = (int64_t)p.far_blocks * (p.far_pieces > 1 ? p.far_pieces : 0) +
               (blocks - p.far_blocks) * (p.near_pieces > 1 ? p.near_pieces : 0);
     return p;
@@ -648,7 +681,8 @@ bool sizes_ok(int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq_len, i
 }
 
 bool strides_ok(const Tensor& t, int64_t per) {
-    return t.p && ((uintptr_t)t.p & 15) == 0 && t.sb % per == 0 && t.st % per == 0 && t.sh % per == 0;
+    return t.p && ((uintptr_t)t.p & 15) == 0 && t.sb % per == 0 && t.st % per == 0 && t.sh % per == 0 && t.st >= 0 &&
+           t.st < (1 << 23);  // (a tile's 64 rows are addressed by 32-bit offsets)
 }
 
 Args make_args(int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq_len, int64_t dim, int64_t window,
@@ -668,9 +702,10 @@ template <class F>
 void with_pass(int dtype, int dp, int nw, F&& f) {
     with_dtype(dtype, [&](auto t) {
         auto dim = [&](auto d) {
-            constexpr bool wide = sizeof(t) == 4 && decltype(d)::value == 128;
+            constexpr int most = decltype(d)::value == 32 ? 4 : 8;
             if (nw == 2) f(t, d, std::integral_constant<int, 2>{});
-            else f(t, d, std::integral_constant<int, wide ? 4 : 8>{});
+            else if (nw == 4) f(t, d, std::integral_constant<int, 4>{});
+            else f(t, d, std::integral_constant<int, most>{});
         };
         if (dp == 32) dim(std::integral_constant<int, 32>{});
         else if (dp == 64) dim(std::integral_constant<int, 64>{});
@@ -697,9 +732,9 @@ ASME_API int asme_window_attention_fwd(const void* q, const void* k, const void*
     a.state = (float2*)state;
     const int dp = padded_dim(head_dim), nw = waves(seq_len, dtype, dp);
     a.blocks = (int)((seq_len + nw * 32 - 1) / (nw * 32));
-    a.items = batch * heads * a.blocks;
-    a.per_xcd = (a.items + 7) / 8;
-    ASME_CHECK_ARG(8 * a.per_xcd < (1ll << 31), "asme_window_attention_fwd: bad size");
+    const int64_t items = batch * heads * a.blocks;
+    a.items = (uint32_t)items, a.per_xcd = (uint32_t)((items + 7) / 8);
+    ASME_CHECK_ARG(items + 8 < (1ll << 31), "asme_window_attention_fwd: bad size");
     with_pass(dtype, dp, nw, [&](auto t, auto d, auto w) {
         hipLaunchKernelGGL((forward_kernel<decltype(t), decltype(d)::value, decltype(w)::value>),
                            dim3((unsigned)(8 * a.per_xcd)), dim3(nw * 64), 0, (hipStream_t)stream, a);
@@ -709,11 +744,12 @@ ASME_API int asme_window_attention_fwd(const void* q, const void* k, const void*
 
 // bytes; 0 for sizes that the call refuses
 ASME_API int64_t asme_window_attention_bwd_workspace(int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq_len,
-                                                     int64_t head_dim, int64_t window, int64_t sinks, int dtype) {
+                                                     int64_t head_dim, int64_t window, int64_t sinks, int causal,
+                                                     int dtype) {
     if (!dtype_ok(dtype) || !sizes_ok(batch, heads, kv_heads, seq_len, head_dim, window, sinks)) return 0;
-    const int nw = waves(seq_len, dtype, padded_dim(head_dim));
+    const int nw = waves_kv(seq_len, dtype, padded_dim(head_dim));
     const Pieces p = pieces_of(batch, kv_heads, heads / kv_heads, seq_len, std::min(window, seq_len),
-                               std::min(sinks, seq_len), nw);
+                               std::min(sinks, seq_len), causal, nw);
     return ((batch * heads * seq_len + 3) / 4 * 4 + batch * kv_heads * p.slabs * 2 * nw * 32 * head_dim) * 4;
 }
 
@@ -729,7 +765,7 @@ ASME_API int asme_window_attention_bwd(const void* q, const void* k, const void*
                    "asme_window_attention_bwd: bad size");
     ASME_CHECK_ARG(scale > 0.f && scale < INFINITY, "asme_window_attention_bwd: scale > 0");
     ASME_CHECK_ARG(ws_bytes >= asme_window_attention_bwd_workspace(batch, heads, kv_heads, seq_len, head_dim, window,
-                                                                   sinks, dtype) &&
+                                                                   sinks, causal, dtype) &&
                        ((uintptr_t)workspace & 15) == 0,
                    "asme_window_attention_bwd: workspace too small or not 16-byte aligned");
     Args a = make_args(batch, heads, kv_heads, seq_len, head_dim, window, sinks, causal, scale, valid);
@@ -743,22 +779,26 @@ ASME_API int asme_window_attention_bwd(const void* q, const void* k, const void*
     a.state = (float2*)const_cast<float*>(state);
     a.delta = (float*)workspace;
     a.part = a.delta + (batch * heads * seq_len + 3) / 4 * 4;
-    const int dp = padded_dim(head_dim), nw = waves(seq_len, dtype, dp), rows = nw * 32;
+    const int dp = padded_dim(head_dim), nq = waves(seq_len, dtype, dp), nw = waves_kv(seq_len, dtype, dp), rows = nw * 32;
+    a.blocks = (int)((seq_len + nq * 32 - 1) / (nq * 32));
+    const int64_t q_items = batch * heads * a.blocks;
+    Args aq = a;
     a.blocks = (int)((seq_len + rows - 1) / rows);
-    const Pieces p = pieces_of(batch, kv_heads, a.group, seq_len, a.window, a.sinks, nw);
+    const Pieces p = pieces_of(batch, kv_heads, a.group, seq_len, a.window, a.sinks, causal, nw);
     a.far_blocks = p.far_blocks, a.far_pieces = p.far_pieces, a.near_pieces = p.near_pieces;
     hipStream_t s = (hipStream_t)stream;
-    const int64_t q_items = batch * heads * a.blocks;
     const int64_t k_items = batch * kv_heads * ((int64_t)a.far_blocks * a.far_pieces +
                                                 (int64_t)(a.blocks - a.far_blocks) * a.near_pieces);
     ASME_CHECK_ARG(q_items + 8 < (1ll << 31) && k_items + 8 < (1ll << 31), "asme_window_attention_bwd: bad size");
+    aq.items = (uint32_t)q_items, aq.per_xcd = (uint32_t)((q_items + 7) / 8);
+    with_pass(dtype, dp, nq, [&](auto t, auto d, auto w) {
+        hipLaunchKernelGGL((dq_kernel<decltype(t), decltype(d)::value, decltype(w)::value>),
+                           dim3((unsigned)(8 * aq.per_xcd)), dim3(nq * 64), 0, s, aq);
+    });
+    a.items = (uint32_t)k_items, a.per_xcd = (uint32_t)((k_items + 7) / 8);
     with_pass(dtype, dp, nw, [&](auto t, auto d, auto w) {
-        using T = decltype(t);
-        constexpr int DP = decltype(d)::value, NW = decltype(w)::value;
-        a.items = q_items, a.per_xcd = (q_items + 7) / 8;
-        hipLaunchKernelGGL((dq_kernel<T, DP, NW>), dim3((unsigned)(8 * a.per_xcd)), dim3(nw * 64), 0, s, a);
-        a.items = k_items, a.per_xcd = (k_items + 7) / 8;
-        hipLaunchKernelGGL((dkv_kernel<T, DP, NW>), dim3((unsigned)(8 * a.per_xcd)), dim3(nw * 64), 0, s, a);
+        hipLaunchKernelGGL((dkv_kernel<decltype(t), decltype(d)::value, decltype(w)::value>),
+                           dim3((unsigned)(8 * a.per_xcd)), dim3(nw * 64), 0, s, a);
     });
     const int64_t far_slabs = (int64_t)a.far_blocks * (a.far_pieces > 1 ? a.far_pieces : 0);
     auto add = [&](int first, int blocks, int pieces, int64_t slab0) {

@@ -1669,8 +1669,8 @@ def _window_backward(q, k, v, valid, out, state, dout, grads, window, sinks, cau
     B, L, H, D = q.shape
     dout = _strided_heads(dout)
     with torch.cuda.device(q.device):
-        ws, nb = _ws_bytes("asme_window_attention_bwd_workspace", B, H, k.shape[2], L, D, window, sinks, _dtype_code(q),
-                           device=q.device)
+        ws, nb = _ws_bytes("asme_window_attention_bwd_workspace", B, H, k.shape[2], L, D, window, sinks, int(causal),
+                         _dtype_code(q),                           device=q.device)
         call("asme_window_attention_bwd", ptr(q), ptr(k), ptr(v), ptr(out), ptr(dout), *(ptr(g) for g in grads),
              _strides(q, k, v, out, dout, *grads), ptr(valid), B, H, k.shape[2], L, D, window, sinks, int(causal),
              scale, _dtype_code(q), ptr(state), ptr(ws), nb, stream())
@@ -1831,7 +1831,8 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
 def _strided_heads(t: torch.Tensor) -> torch.Tensor:
     """(B, L, heads, head_dim) with adjacent head values and every row on a 16-byte boundary, copied only if it is not"""
     per = 16 // t.element_size()
-    ok = t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(s % per == 0 and s >= 0 for s in t.stride()[:3])
+    ok = (t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(s % per == 0 and s >= 0 for s in t.stride()[:3])
+          and t.stride(1) < 2 ** 23)
     return t if ok else t.contiguous().clone() if t.is_contiguous() else t.contiguous()
 
 
