@@ -83,13 +83,13 @@ struct Args {
     const uint8_t* valid;  // (batch, seq_len) or null
     float2* state;         // (batch, heads, seq_len): maximum of the scaled scores in base 2, 1 / sum
     float* delta;          // (batch, heads, seq_len): D
-    float* part;           // partial dK, dV: (key head, split block, piece, 2, rows, dim)
+    float *part, *far_part;  // partial dK, dV: (key head, block, piece, 2, rows, dim), (key head, 32 sinks, piece, 2, 2, 32, dim)
     int seq_len, dim, heads, kv_heads, group, window, sinks, causal;
     int blocks;            // stationary blocks of a sequence
     uint32_t items, per_xcd;  // workgroups of the pass, those of an XCD
-    // dK, dV: the first `far_blocks` key blocks hold sinks, which every later query sees: cut into far_pieces pieces;
-    // the others into near_pieces
-    int far_blocks, far_pieces, near_pieces;
+    // dK, dV: rows of a key block and its pieces; groups of 32 sinks that queries outside their block's tiles see (0: none
+    // do), and the pieces of a group
+    int near_rows, near_pieces, far_groups, far_pieces;
     float scale;
 };
 
@@ -192,23 +192,28 @@ struct Pass {
     }
     // X[streamed row of the 32-row half `sub`][stationary row] of tensor `op`.  The reads of kStep k steps are issued
     // together, so that a product waits for the first of them and not each for its own
-    static constexpr int kStep = NP == 1 ? KS : 2;
+    static constexpr int kStep = NP == 1 ? (KS < 4 ? KS : 4) : 2;
     static __device__ __forceinline__ floatx16 score(const char* lds, int op, int sub, const F (&st)[KS]) {
+        return score_of(lds, op, sub, [&](int ks) { return st[ks]; });
+    }
+    template <class Stationary>
+    static __device__ __forceinline__ floatx16 score_of(const char* lds, int op, int sub, Stationary&& st) {
         const int lane = threadIdx.x & 63, r32 = lane & 31, h = lane >> 5;
         floatx16 x;
 #pragma unroll
         for (int i = 0; i < 16; ++i) x[i] = 0.f;
 #pragma unroll
         for (int k0 = 0; k0 < KS; k0 += kStep) {
-            F A[kStep];
+            F A[kStep], B[kStep];
 #pragma unroll
-            for (int ks = 0; ks < kStep; ++ks)
+            for (int ks = 0; ks < kStep; ++ks) {
 #pragma unroll
                 for (int p = 0; p < NP; ++p)
                     A[ks].p[p] = *reinterpret_cast<const bf16x8*>(lds + place(op, p, 32 * sub + r32, 2 * (k0 + ks) + h));
-            __builtin_amdgcn_sched_barrier(0);
+                B[ks] = st(k0 + ks);
+            }
 #pragma unroll
-            for (int ks = 0; ks < kStep; ++ks) x = product(A[ks], st[k0 + ks], x);
+            for (int ks = 0; ks < kStep; ++ks) x = product(A[ks], B[ks], x);
         }
         return x;
     }
@@ -244,7 +249,6 @@ struct Pass {
         for (int s2 = 0; s2 < 2; ++s2) {
             F A[NFT];
             read_transposed(lds, op, sub, s2, A);
-            __builtin_amdgcn_sched_barrier(0);
             const F P = weights_of(x, s2);
 #pragma unroll
             for (int ft = 0; ft < NFT; ++ft) y[ft] = product(A[ft], P, y[ft]);
@@ -268,6 +272,21 @@ struct Pass {
                                (__bf16)(y[ft][4 * i + 2] * f), (__bf16)(y[ft][4 * i + 3] * f)};
                 }
             }
+    }
+    // y += f * a row of fp32 values laid out like that
+    static __device__ __forceinline__ void add_row(const float* row, floatx16 (&y)[NFT], float f, int h, int dim) {
+        floatx4 x[NFT][4];
+#pragma unroll
+        for (int ft = 0; ft < NFT; ++ft)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int c = 32 * ft + 8 * i + 4 * h;
+                x[ft][i] = *reinterpret_cast<const floatx4*>(row + (DP > 32 || c < dim ? c : 0));
+            }
+#pragma unroll
+        for (int ft = 0; ft < NFT; ++ft)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) y[ft][e] = fmaf(f, x[ft][e >> 2][e & 3], y[ft][e]);
     }
     static __device__ __forceinline__ void clear(floatx16 (&y)[NFT]) {
 #pragma unroll
@@ -501,44 +520,62 @@ __global__ __launch_bounds__(NW * 64) void dq_kernel(Args a) {
 }
 
 // ------------------------------------------------------------------------------------------------ dK, dV
-// Item: (sequence, key head, key block, piece); its steps are the query tiles of the block's range for each query head of
-// the group, of which a piece takes a contiguous share.  One piece: dK and dV at once, else partial rows.
-template <class T, int DP, int NW>
+// The query tiles that the near pass of the key block from k0 on streams: those that a key of the block is in the window
+// of.  What a sink is seen by beyond them is the far pass's.
+struct QueryTiles {
+    int lo, hi;
+    __host__ __device__ QueryTiles(const Args& a, int k0, int rows) {
+        const int64_t k1 = k0 + rows < a.seq_len ? k0 + rows : a.seq_len, end = k1 - 1 + a.window;
+        const int first = a.causal ? k0 : k0 - a.window + 1;
+        lo = first > 0 ? first / kTS : 0;
+        hi = (int)(((end < a.seq_len ? end : a.seq_len) + kTS - 1) / kTS);
+    }
+};
+
+// Near item: (sequence, key head, key block of NW x 32, piece); its steps are the block's query tiles for each query head
+// of the group, of which a piece takes a contiguous share.  One piece: dK and dV at once, the far pass's rows added; else
+// partial rows.  V's fragments (VL) wait in LDS, in the order they are read: with them in registers the pass needs over
+// 256 and runs at one wave per SIMD, where the matrix and vector units take turns.
+// Far item: (sequence, key head, 32 sinks, piece) over the query tiles outside the near pass's of the sinks' block; both
+// waves hold the same sinks and each takes its half of every tile, into partial rows of its own.
+template <class T, int DP, int NW, bool VL, bool FAR>
 __global__ __launch_bounds__(NW * 64) void dkv_kernel(Args a) {
     using P = Pass<T, DP, NW>;
+    static_assert(!FAR || NW == 2, "a half of the tile for each wave");
     __shared__ __attribute__((aligned(16))) char lds[P::kBytes];
+    __shared__ __attribute__((aligned(16))) char vlds[VL ? NW * P::KS * P::NP * 1024 : 16];
     __shared__ __attribute__((aligned(16))) float meta[3][kTS];  // maximum, 1 / sum, D of the tile's queries
     uint32_t item;
     if (!item_of(a, item)) return;
     const int lane = threadIdx.x & 63, h = lane >> 5, r32 = lane & 31;
-    const int near = a.blocks - a.far_blocks, per_head = a.far_blocks * a.far_pieces + near * a.near_pieces;
-    const uint32_t bk = item / (uint32_t)per_head;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int pieces = FAR ? a.far_pieces : a.near_pieces;
+    const uint32_t unit = item / (uint32_t)pieces, per_head = FAR ? a.far_groups : a.blocks, bk = unit / per_head;
+    const int piece = (int)(item - unit * pieces), block = (int)(unit - bk * per_head);
     const int kh = (int)(bk % (uint32_t)a.kv_heads);
     const int64_t b = bk / (uint32_t)a.kv_heads;
-    int within = (int)(item - bk * per_head), block, piece, pieces;
-    if (within < a.far_blocks * a.far_pieces) {
-        pieces = a.far_pieces, block = within / pieces, piece = within % pieces;
-    } else {
-        within -= a.far_blocks * a.far_pieces;
-        pieces = a.near_pieces, block = a.far_blocks + within / pieces, piece = within % pieces;
-    }
-    const int k0 = block * NW * 32, k1 = min(a.seq_len, k0 + NW * 32);
-    const int w0 = k0 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 32, kj = w0 + r32;
-    const bool live = kj < a.seq_len && (!a.valid || a.valid[b * a.seq_len + kj]);
+    const int w0 = FAR ? block * 32 : (block * NW + wave) * 32, kj = w0 + r32;
+    const bool live = kj < a.seq_len && (!FAR || kj < a.sinks) && (!a.valid || a.valid[b * a.seq_len + kj]);
     const bool any = __ballot(live) != 0;
     const uint32_t ok = (uint32_t)__ballot(live);  // (both halves of the lanes hold the same keys)
     typename P::F K[P::KS], V[P::KS];
     P::stationary(K, live ? a.k.at<T>(b, kh) + kj * a.k.st : nullptr, h, a.dim);
     P::stationary(V, live ? a.v.at<T>(b, kh) + kj * a.v.st : nullptr, h, a.dim);
+    char* mine = vlds + wave * P::KS * P::NP * 1024 + lane * 16;
+    if constexpr (VL) {
+#pragma unroll
+        for (int ks = 0; ks < P::KS; ++ks)
+#pragma unroll
+            for (int p = 0; p < P::NP; ++p) *reinterpret_cast<bf16x8*>(mine + (ks * P::NP + p) * 1024) = V[ks].p[p];
+    }
     floatx16 yk[P::NFT], yv[P::NFT];
     P::clear(yk);
     P::clear(yv);
     const float c = a.scale * kLog2e;
-    // the queries that see a key of the block
-    const bool all = k0 < a.sinks;
-    const int lo = (a.causal ? k0 : all ? 0 : max(0, k0 - a.window + 1)) / kTS * kTS;
-    const int hi = all ? a.seq_len : (int)min((int64_t)a.seq_len, (int64_t)k1 - 1 + a.window);
-    const int tiles = (hi - lo + kTS - 1) / kTS, steps = tiles * a.group;
+    const QueryTiles near(a, FAR ? block * 32 / a.near_rows * a.near_rows : block * NW * 32, FAR ? a.near_rows : NW * 32);
+    // the near tiles, or those beside them: [0, lo) without causal, and [hi, all)
+    const int before = FAR && !a.causal ? near.lo : 0, jump = FAR ? near.hi : near.lo;
+    const int tiles = FAR ? before + (a.seq_len + kTS - 1) / kTS - near.hi : near.hi - near.lo, steps = tiles * a.group;
     int i = (int)((int64_t)steps * piece / pieces), t0 = 0;
     const int last = (int)((int64_t)steps * (piece + 1) / pieces);
     int valid = 0;
@@ -547,9 +584,9 @@ __global__ __launch_bounds__(NW * 64) void dkv_kernel(Args a) {
     float delta = 0.f;
     auto issue = [&]() {
         if (i >= last) return;
-        t0 = lo + i % tiles * kTS;
+        const int tile = i % tiles, head = kh * a.group + i / tiles;
+        t0 = (tile < before ? tile : tile - before + jump) * kTS;
         valid = P::valid_row(a, b, t0);
-        const int head = kh * a.group + i / tiles;
         P::fetch(next, a.q.at<T>(b, head), a.q.st, a.dout.at<T>(b, head), a.dout.st, t0, a.seq_len, a.dim);
         if (threadIdx.x < kTS) {  // (of a query that is none: (infinity, 0) and 0)
             const int64_t at = (b * a.heads + head) * a.seq_len + t0 + threadIdx.x;
@@ -570,7 +607,8 @@ __global__ __launch_bounds__(NW * 64) void dkv_kernel(Args a) {
         issue();
         if (!any) continue;
 #pragma unroll
-        for (int sub = 0; sub < 2; ++sub) {
+        for (int half = 0; half < (FAR ? 1 : 2); ++half) {
+            const int sub = FAR ? wave : half;
             const int i0 = q0 + 32 * sub, seen = (uint32_t)(queries >> (32 * sub)) ? block_seen(a, i0, w0) : 0;
             if (!seen) continue;
             floatx16 x = P::score(lds, 0, sub, K);
@@ -586,52 +624,76 @@ __global__ __launch_bounds__(NW * 64) void dkv_kernel(Args a) {
                 x[e] = __builtin_amdgcn_exp2f(fmaf(x[e], c, -m[r])) * m[kTS + r];
             }
             P::gather(lds, 1, sub, x, yv);
-            floatx16 dp = P::score(lds, 1, sub, V);
+            floatx16 dp = P::score_of(lds, 1, sub, [&](int ks) {
+                if constexpr (!VL) return V[ks];
+                typename P::F f;
+#pragma unroll
+                for (int p = 0; p < P::NP; ++p)
+                    f.p[p] = *reinterpret_cast<const bf16x8*>(mine + (ks * P::NP + p) * 1024);
+                return f;
+            });
 #pragma unroll
             for (int e = 0; e < 16; ++e) dp[e] = x[e] * (dp[e] - m[2 * kTS + 8 * (e >> 2) + (e & 3)]);
             P::gather(lds, 0, sub, dp, yk);
         }
     }
-    if (pieces > 1) {  // fp32 rows of this piece, zeros where there is nothing
-        const int64_t far = (int64_t)a.far_blocks * (a.far_pieces > 1 ? a.far_pieces : 0);
-        const int64_t split = far + (int64_t)near * (a.near_pieces > 1 ? a.near_pieces : 0);
-        const int64_t slab = (int64_t)bk * split + (block < a.far_blocks ? (int64_t)block * a.far_pieces
-                                                                : far + (int64_t)(block - a.far_blocks) * a.near_pieces) +
-                             piece;
-        float* p = a.part + (slab * 2 * NW * 32 + (kj - k0)) * a.dim;
-        using PF = Pass<float, DP, NW>;
+    using PF = Pass<float, DP, NW>;
+    if constexpr (FAR) {  // slab (key head, sinks, piece, wave): dK and dV of 32 rows
+        float* p = a.far_part + ((((int64_t)unit * pieces + piece) * 2 + wave) * 64 + r32) * a.dim;
+        PF::write_row(p, yk, a.scale, h, a.dim);
+        PF::write_row(p + 32 * a.dim, yv, 1.f, h, a.dim);
+        return;
+    }
+    if (pieces > 1) {  // slab (key head, block, piece): dK and dV of the block's rows, zeros where there is nothing
+        float* p = a.part + ((int64_t)item * 2 * NW * 32 + wave * 32 + r32) * a.dim;
         PF::write_row(p, yk, a.scale, h, a.dim);
         PF::write_row(p + (int64_t)NW * 32 * a.dim, yv, 1.f, h, a.dim);
         return;
     }
     if (kj >= a.seq_len) return;
+    if (w0 < 32 * a.far_groups) {  // the far pass's sums, added up in its first slab (0 for rows that are no sinks)
+        const float* p = a.far_part + ((int64_t)(bk * a.far_groups + w0 / 32) * a.far_pieces * 128 + r32) * a.dim;
+        P::add_row(p, yk, 1.f / a.scale, h, a.dim);
+        P::add_row(p + 32 * a.dim, yv, 1.f, h, a.dim);
+    }
     if (!live) P::clear(yk), P::clear(yv);
     P::write_row(a.dk.at<T>(b, kh) + kj * a.dk.st, yk, a.scale, h, a.dim);
     P::write_row(a.dv.at<T>(b, kh) + kj * a.dv.st, yv, 1.f, h, a.dim);
 }
 
-// dK, dV of the blocks in pieces: their partial rows added in order, 4 columns a thread
-template <class T>
-__global__ __launch_bounds__(256) void add_pieces_kernel(Args a, int block_rows, int first, int blocks, int pieces,
-                                                         int64_t slab0, int64_t slabs, int64_t total) {
+// the far pass's slabs of 32 sinks (2 x 32 rows each) added up in the first, in order, 4 columns a thread
+__global__ __launch_bounds__(256) void add_far_kernel(float* part, int slabs, int dim, int64_t total) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= total) return;
-    const int quads = a.dim / 4, c = (int)(i % quads) * 4, row = (int)(i / quads % block_rows);
-    const int64_t u = i / quads / block_rows;
-    const int which = (int)(u % 2), block = (int)(u / 2 % blocks);
-    const int64_t bk = u / 2 / blocks, b = bk / a.kv_heads;
-    const int kh = (int)(bk % a.kv_heads), kj = (first + block) * block_rows + row;
-    if (kj >= a.seq_len) return;
-    const bool live = !a.valid || a.valid[b * a.seq_len + kj];
+    const int64_t slab = 64 * dim, quads = slab / 4;
+    float* p = part + i / quads * slabs * slab + i % quads * 4;
+    floatx4 s = *reinterpret_cast<const floatx4*>(p);
+#pragma unroll 8
+    for (int u = 1; u < slabs; ++u) s += *reinterpret_cast<const floatx4*>(p + u * slab);
+    *reinterpret_cast<floatx4*>(p) = s;
+}
+
+// dK, dV of blocks in pieces: the near pass's partial rows and the far pass's added in order, 4 columns a thread
+template <class T>
+__global__ __launch_bounds__(256) void add_pieces_kernel(Args a, int64_t total) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= total) return;
+    const int quads = a.dim / 4, c = (int)(i % quads) * 4, kj = (int)(i / quads % a.seq_len);
+    const int64_t u = i / quads / a.seq_len, bk = u / 2, b = bk / a.kv_heads;
+    const int which = (int)(u % 2), kh = (int)(bk % a.kv_heads), block = kj / a.near_rows, row = kj % a.near_rows;
     float s[4] = {0.f, 0.f, 0.f, 0.f};
-    if (live)
-        for (int p = 0; p < pieces; ++p) {
-            float x[4];
-            Elem<float>::load(a.part + (((bk * slabs + slab0 + (int64_t)block * pieces + p) * 2 + which) * block_rows +
-                                        row) * a.dim + c, x);
+    auto add = [&](const float* p) {
+        float x[4];
+        Elem<float>::load(p, x);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[e] += x[e];
-        }
+        for (int e = 0; e < 4; ++e) s[e] += x[e];
+    };
+    if (!a.valid || a.valid[b * a.seq_len + kj]) {
+        for (int p = 0; p < a.near_pieces; ++p)
+            add(a.part + ((((bk * a.blocks + block) * a.near_pieces + p) * 2 + which) * a.near_rows + row) * a.dim + c);
+        if (kj < 32 * a.far_groups)
+            add(a.far_part + ((bk * a.far_groups + kj / 32) * a.far_pieces * 128 + which * 32 + kj % 32) * a.dim + c);
+    }
     const Tensor& t = which ? a.dv : a.dk;
     T* o = t.at<T>(b, kh) + kj * t.st + c;
 #pragma unroll
@@ -649,28 +711,31 @@ int waves(int64_t seq_len, int dtype, int dp) {
 }
 int waves_kv(int64_t seq_len, int dtype, int dp) {
     if (seq_len <= 64) return 2;
-    return dp == 64 && dtype == kBF16 ? 8 : 4;
+    return dp != 64 ? 4 : 8;
 }
 
-struct Pieces {
-    int far_blocks, far_pieces, near_pieces;
-    int64_t slabs;  // partial slabs per key head
-};
-// key blocks are cut so that none takes much longer than the others: a block with sinks is seen by every later query
-Pieces pieces_of(int64_t batch, int64_t kv_heads, int64_t group, int64_t seq_len, int64_t window, int64_t sinks,
-                 int causal, int nw) {
-    const int64_t rows = nw * 32, blocks = (seq_len + rows - 1) / rows;
-    Pieces p;
-    p.far_blocks = (int)std::min(blocks, (sinks + rows - 1) / rows);
-    const int64_t reach = std::min(seq_len, rows + window * (causal ? 1 : 2));
-    const int64_t near_steps = (reach + kTS - 1) / kTS * group, far_steps = (seq_len + kTS - 1) / kTS * group;
-    const int64_t have = batch * kv_heads * blocks;
-    p.near_pieces = (int)std::max<int64_t>(1, std::min<int64_t>((512 + have - 1) / have, near_steps / 6));
-    p.far_pieces = (int)std::max<int64_t>(1, far_steps / std::max<int64_t>(6, near_steps / p.near_pieces));
-    p.near_pieces = std::min(p.near_pieces, 64), p.far_pieces = std::min(p.far_pieces, 64);
-    p.slabs = (int64_t)p.far_blocks * (p.far_pieces > 1 ? p.far_pieces : 0) +
-              (blocks - p.far_blocks) * (p.near_pieces > 1 ? p.near_pieces : 0);
-    return p;
+// pieces of the dK, dV passes: as many as it takes to give every CU a workgroup, each at least 6 tiles long (near) or 4
+void plan_kv(Args& a, int64_t batch, int nw) {
+    a.near_rows = nw * 32;
+    a.blocks = (a.seq_len + a.near_rows - 1) / a.near_rows;
+    const int64_t have = batch * a.kv_heads, all = (a.seq_len + kTS - 1) / kTS;
+    const int64_t reach = std::min<int64_t>(a.seq_len, a.near_rows + (int64_t)a.window * (a.causal ? 1 : 2));
+    a.near_pieces = (int)std::max<int64_t>(
+        1, std::min<int64_t>({256 / (have * a.blocks), (reach + kTS - 1) / kTS * a.group / 6, 64}));
+    int64_t most = 0;  // tiles beside the near pass's, of the block that has the most
+    for (int k0 = 0; k0 < a.sinks; k0 += a.near_rows) {
+        const QueryTiles t(a, k0, a.near_rows);
+        most = std::max<int64_t>(most, all - t.hi + (a.causal ? 0 : t.lo));
+    }
+    a.far_groups = most > 0 ? (a.sinks + 31) / 32 : 0;
+    a.far_pieces = a.far_groups ? (int)std::max<int64_t>(
+        1, std::min<int64_t>({512 / (have * a.far_groups), most * a.group / 4, 64})) : 1;
+}
+int64_t slab_floats(const Args& a, int64_t batch) {
+    return a.near_pieces > 1 ? batch * a.kv_heads * a.blocks * a.near_pieces * 2 * a.near_rows * a.dim : 0;
+}
+int64_t far_floats(const Args& a, int64_t batch) {
+    return batch * a.kv_heads * a.far_groups * a.far_pieces * 128 * a.dim;
 }
 
 bool sizes_ok(int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq_len, int64_t dim, int64_t window,
@@ -702,7 +767,7 @@ template <class F>
 void with_pass(int dtype, int dp, int nw, F&& f) {
     with_dtype(dtype, [&](auto t) {
         auto dim = [&](auto d) {
-            constexpr int most = decltype(d)::value == 32 ? 4 : 8;
+            constexpr int most = decltype(d)::value == 32 || (sizeof(t) == 4 && decltype(d)::value == 128) ? 4 : 8;
             if (nw == 2) f(t, d, std::integral_constant<int, 2>{});
             else if (nw == 4) f(t, d, std::integral_constant<int, 4>{});
             else f(t, d, std::integral_constant<int, most>{});
@@ -747,10 +812,9 @@ ASME_API int64_t asme_window_attention_bwd_workspace(int64_t batch, int64_t head
                                                      int64_t head_dim, int64_t window, int64_t sinks, int causal,
                                                      int dtype) {
     if (!dtype_ok(dtype) || !sizes_ok(batch, heads, kv_heads, seq_len, head_dim, window, sinks)) return 0;
-    const int nw = waves_kv(seq_len, dtype, padded_dim(head_dim));
-    const Pieces p = pieces_of(batch, kv_heads, heads / kv_heads, seq_len, std::min(window, seq_len),
-                               std::min(sinks, seq_len), causal, nw);
-    return ((batch * heads * seq_len + 3) / 4 * 4 + batch * kv_heads * p.slabs * 2 * nw * 32 * head_dim) * 4;
+    Args a = make_args(batch, heads, kv_heads, seq_len, head_dim, window, sinks, causal, 1.f, nullptr);
+    plan_kv(a, batch, waves_kv(seq_len, dtype, padded_dim(head_dim)));
+    return ((batch * heads * seq_len + 3) / 4 * 4 + slab_floats(a, batch) + far_floats(a, batch)) * 4;
 }
 
 ASME_API int asme_window_attention_bwd(const void* q, const void* k, const void* v, const void* out, const void* dout,
@@ -779,37 +843,47 @@ ASME_API int asme_window_attention_bwd(const void* q, const void* k, const void*
     a.state = (float2*)const_cast<float*>(state);
     a.delta = (float*)workspace;
     a.part = a.delta + (batch * heads * seq_len + 3) / 4 * 4;
-    const int dp = padded_dim(head_dim), nq = waves(seq_len, dtype, dp), nw = waves_kv(seq_len, dtype, dp), rows = nw * 32;
-    a.blocks = (int)((seq_len + nq * 32 - 1) / (nq * 32));
-    const int64_t q_items = batch * heads * a.blocks;
-    Args aq = a;
-    a.blocks = (int)((seq_len + rows - 1) / rows);
-    const Pieces p = pieces_of(batch, kv_heads, a.group, seq_len, a.window, a.sinks, causal, nw);
-    a.far_blocks = p.far_blocks, a.far_pieces = p.far_pieces, a.near_pieces = p.near_pieces;
+    const int dp = padded_dim(head_dim), nq = waves(seq_len, dtype, dp), nw = waves_kv(seq_len, dtype, dp);
     hipStream_t s = (hipStream_t)stream;
-    const int64_t k_items = batch * kv_heads * ((int64_t)a.far_blocks * a.far_pieces +
-                                                (int64_t)(a.blocks - a.far_blocks) * a.near_pieces);
-    ASME_CHECK_ARG(q_items + 8 < (1ll << 31) && k_items + 8 < (1ll << 31), "asme_window_attention_bwd: bad size");
-    aq.items = (uint32_t)q_items, aq.per_xcd = (uint32_t)((q_items + 7) / 8);
+    // the whole grid of `items` workgroups of a pass
+    auto grid = [](Args& x, int64_t items) {
+        x.items = (uint32_t)items, x.per_xcd = (uint32_t)((items + 7) / 8);
+        return dim3(8 * x.per_xcd);
+    };
+    const int64_t key_heads = batch * kv_heads;
+    Args aq = a;
+    aq.blocks = (int)((seq_len + nq * 32 - 1) / (nq * 32));
+    plan_kv(a, batch, nw);
+    a.far_part = a.part + slab_floats(a, batch);
+    const int64_t q_items = batch * heads * aq.blocks, k_items = key_heads * a.blocks * a.near_pieces;
+    ASME_CHECK_ARG(q_items + 8 < (1ll << 31) && k_items + 8 < (1ll << 31) &&
+                       key_heads * std::max(1, a.far_groups) * a.far_pieces + 8 < (1ll << 31),
+                   "asme_window_attention_bwd: bad size");
+    const dim3 q_grid = grid(aq, q_items);
     with_pass(dtype, dp, nq, [&](auto t, auto d, auto w) {
-        hipLaunchKernelGGL((dq_kernel<decltype(t), decltype(d)::value, decltype(w)::value>),
-                           dim3((unsigned)(8 * aq.per_xcd)), dim3(nq * 64), 0, s, aq);
+        hipLaunchKernelGGL((dq_kernel<decltype(t), decltype(d)::value, decltype(w)::value>), q_grid, dim3(nq * 64), 0, s,
+                           aq);
     });
-    a.items = (uint32_t)k_items, a.per_xcd = (uint32_t)((k_items + 7) / 8);
+    if (a.far_groups) {
+        const dim3 g = grid(a, key_heads * a.far_groups * a.far_pieces);
+        with_pass(dtype, dp, 2, [&](auto t, auto d, auto) {
+            hipLaunchKernelGGL((dkv_kernel<decltype(t), decltype(d)::value, 2, false, true>), g, dim3(128), 0, s, a);
+        });
+        const int64_t total = key_heads * a.far_groups * 16 * head_dim;
+        hipLaunchKernelGGL(add_far_kernel, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, s, a.far_part,
+                           2 * a.far_pieces, (int)head_dim, total);
+    }
+    const dim3 g = grid(a, k_items);
     with_pass(dtype, dp, nw, [&](auto t, auto d, auto w) {
-        hipLaunchKernelGGL((dkv_kernel<decltype(t), decltype(d)::value, decltype(w)::value>),
-                           dim3((unsigned)(8 * a.per_xcd)), dim3(nw * 64), 0, s, a);
+        constexpr int DP = decltype(d)::value, NW = decltype(w)::value;
+        hipLaunchKernelGGL((dkv_kernel<decltype(t), DP, NW, NW == 8, false>), g, dim3(nw * 64), 0, s, a);
     });
-    const int64_t far_slabs = (int64_t)a.far_blocks * (a.far_pieces > 1 ? a.far_pieces : 0);
-    auto add = [&](int first, int blocks, int pieces, int64_t slab0) {
-        if (blocks <= 0 || pieces <= 1) return;
-        const int64_t total = batch * kv_heads * blocks * 2 * rows * (head_dim / 4);
+    if (a.near_pieces > 1) {
+        const int64_t total = key_heads * 2 * seq_len * (head_dim / 4);
         with_dtype(dtype, [&](auto t) {
             hipLaunchKernelGGL(add_pieces_kernel<decltype(t)>, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, s, a,
-                               rows, first, blocks, pieces, slab0, p.slabs, total);
+                               total);
         });
-    };
-    add(0, a.far_blocks, a.far_pieces, 0);
-    add(a.far_blocks, a.blocks - a.far_blocks, a.near_pieces, far_slabs);
+    }
     ASME_LAUNCH_CHECK("asme_window_attention_bwd");
 }
