@@ -83,11 +83,11 @@ struct Args {
     const uint8_t* valid;  // (batch, seq_len) or null
     float2* state;         // (batch, heads, seq_len): maximum of the scaled scores in base 2, 1 / sum
     float* delta;          // (batch, heads, seq_len): D
-    float *part, *far_part;  // partial dK, dV: (key head, block, piece, 2, rows, dim), (key head, 32 sinks, piece, 2, 2, 32, dim)
+    float *part, *far_part;  // partial dK, dV: (key head, block, piece, 2, rows, dim), (key head, sinks, piece, 2, 64, dim)
     int seq_len, dim, heads, kv_heads, group, window, sinks, causal;
     int blocks;            // stationary blocks of a sequence
     uint32_t items, per_xcd;  // workgroups of the pass, those of an XCD
-    // dK, dV: rows of a key block and its pieces; groups of 32 sinks that queries outside their block's tiles see (0: none
+    // dK, dV: rows of a key block and its pieces; groups of 64 sinks that queries outside their block's tiles see (0: none
     // do), and the pieces of a group
     int near_rows, near_pieces, far_groups, far_pieces;
     float scale;
@@ -194,26 +194,20 @@ struct Pass {
     // together, so that a product waits for the first of them and not each for its own
     static constexpr int kStep = NP == 1 ? (KS < 4 ? KS : 4) : 2;
     static __device__ __forceinline__ floatx16 score(const char* lds, int op, int sub, const F (&st)[KS]) {
-        return score_of(lds, op, sub, [&](int ks) { return st[ks]; });
-    }
-    template <class Stationary>
-    static __device__ __forceinline__ floatx16 score_of(const char* lds, int op, int sub, Stationary&& st) {
         const int lane = threadIdx.x & 63, r32 = lane & 31, h = lane >> 5;
         floatx16 x;
 #pragma unroll
         for (int i = 0; i < 16; ++i) x[i] = 0.f;
 #pragma unroll
         for (int k0 = 0; k0 < KS; k0 += kStep) {
-            F A[kStep], B[kStep];
+            F A[kStep];
 #pragma unroll
-            for (int ks = 0; ks < kStep; ++ks) {
+            for (int ks = 0; ks < kStep; ++ks)
 #pragma unroll
                 for (int p = 0; p < NP; ++p)
                     A[ks].p[p] = *reinterpret_cast<const bf16x8*>(lds + place(op, p, 32 * sub + r32, 2 * (k0 + ks) + h));
-                B[ks] = st(k0 + ks);
-            }
 #pragma unroll
-            for (int ks = 0; ks < kStep; ++ks) x = product(A[ks], B[ks], x);
+            for (int ks = 0; ks < kStep; ++ks) x = product(A[ks], st[k0 + ks], x);
         }
         return x;
     }
@@ -243,16 +237,19 @@ struct Pass {
         for (int j = 0; j < 8; ++j) v[j] = x[8 * s2 + j];
         return frag_of(v, (F*)nullptr);
     }
-    static __device__ __forceinline__ void gather(const char* lds, int op, int sub, const floatx16& x,
-                                                  floatx16 (&y)[NFT]) {
+    static __device__ __forceinline__ void gather(const char* lds, int op, int sub, const F (&w)[2], floatx16 (&y)[NFT]) {
 #pragma unroll
         for (int s2 = 0; s2 < 2; ++s2) {
             F A[NFT];
             read_transposed(lds, op, sub, s2, A);
-            const F P = weights_of(x, s2);
 #pragma unroll
-            for (int ft = 0; ft < NFT; ++ft) y[ft] = product(A[ft], P, y[ft]);
+            for (int ft = 0; ft < NFT; ++ft) y[ft] = product(A[ft], w[s2], y[ft]);
         }
+    }
+    static __device__ __forceinline__ void gather(const char* lds, int op, int sub, const floatx16& x,
+                                                  floatx16 (&y)[NFT]) {
+        const F w[2] = {weights_of(x, 0), weights_of(x, 1)};
+        gather(lds, op, sub, w, y);
     }
     // row `row` (features 32 ft + 8 i + 4 h .. + 3 of this lane's stationary row) = y * f
     static __device__ __forceinline__ void write_row(T* row, const floatx16 (&y)[NFT], float f, int h, int dim) {
@@ -532,47 +529,47 @@ struct QueryTiles {
     }
 };
 
-// Near item: (sequence, key head, key block of NW x 32, piece); its steps are the block's query tiles for each query head
+// Two waves hold the same 32 keys.  Each forms P and dS of its half of the tile's queries and passes on what the other
+// sums: the first all of dV, the second all of dK.  With both sums in one wave the pass needs over 256 registers at 64 or
+// 128 columns and runs at one wave per SIMD, where the matrix and vector units take turns (395 us for the L = 8192 bf16
+// case in place of KVUS).
+constexpr int kFarWaves = 4, kFarRows = 16 * kFarWaves;  // sinks of a workgroup of the far pass
+// where the far pass's sums of dK (0) or dV (1) of key kj begin
+__device__ __forceinline__ int64_t far_row(const Args& a, int64_t bk, int kj, int which) {
+    return ((bk * a.far_groups + kj / kFarRows) * a.far_pieces * 2 * kFarRows + which * kFarRows + kj % kFarRows) * a.dim;
+}
+
+// Near item: (sequence, key head, block of NW x 16 keys, piece); its steps are the block's query tiles for each query head
 // of the group, of which a piece takes a contiguous share.  One piece: dK and dV at once, the far pass's rows added; else
-// partial rows.  V's fragments (VL) wait in LDS, in the order they are read: with them in registers the pass needs over
-// 256 and runs at one wave per SIMD, where the matrix and vector units take turns.
-// Far item: (sequence, key head, 32 sinks, piece) over the query tiles outside the near pass's of the sinks' block; both
-// waves hold the same sinks and each takes its half of every tile, into partial rows of its own.
-template <class T, int DP, int NW, bool VL, bool FAR>
+// partial rows.
+// Far item: (sequence, key head, NW x 16 sinks, piece) over the query tiles outside the near pass's of the sinks' block,
+// into partial rows.
+template <class T, int DP, int NW, bool FAR>
 __global__ __launch_bounds__(NW * 64) void dkv_kernel(Args a) {
     using P = Pass<T, DP, NW>;
-    static_assert(!FAR || NW == 2, "a half of the tile for each wave");
     __shared__ __attribute__((aligned(16))) char lds[P::kBytes];
-    __shared__ __attribute__((aligned(16))) char vlds[VL ? NW * P::KS * P::NP * 1024 : 16];
+    __shared__ __attribute__((aligned(16))) char exchange[NW * 2 * P::NP * 1024];  // fragments in lane order
     __shared__ __attribute__((aligned(16))) float meta[3][kTS];  // maximum, 1 / sum, D of the tile's queries
     uint32_t item;
     if (!item_of(a, item)) return;
     const int lane = threadIdx.x & 63, h = lane >> 5, r32 = lane & 31;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), role = wave & 1;
     const int pieces = FAR ? a.far_pieces : a.near_pieces;
     const uint32_t unit = item / (uint32_t)pieces, per_head = FAR ? a.far_groups : a.blocks, bk = unit / per_head;
     const int piece = (int)(item - unit * pieces), block = (int)(unit - bk * per_head);
     const int kh = (int)(bk % (uint32_t)a.kv_heads);
     const int64_t b = bk / (uint32_t)a.kv_heads;
-    const int w0 = FAR ? block * 32 : (block * NW + wave) * 32, kj = w0 + r32;
+    const int w0 = block * NW * 16 + (wave >> 1) * 32, kj = w0 + r32;
     const bool live = kj < a.seq_len && (!FAR || kj < a.sinks) && (!a.valid || a.valid[b * a.seq_len + kj]);
     const bool any = __ballot(live) != 0;
     const uint32_t ok = (uint32_t)__ballot(live);  // (both halves of the lanes hold the same keys)
     typename P::F K[P::KS], V[P::KS];
     P::stationary(K, live ? a.k.at<T>(b, kh) + kj * a.k.st : nullptr, h, a.dim);
     P::stationary(V, live ? a.v.at<T>(b, kh) + kj * a.v.st : nullptr, h, a.dim);
-    char* mine = vlds + wave * P::KS * P::NP * 1024 + lane * 16;
-    if constexpr (VL) {
-#pragma unroll
-        for (int ks = 0; ks < P::KS; ++ks)
-#pragma unroll
-            for (int p = 0; p < P::NP; ++p) *reinterpret_cast<bf16x8*>(mine + (ks * P::NP + p) * 1024) = V[ks].p[p];
-    }
-    floatx16 yk[P::NFT], yv[P::NFT];
-    P::clear(yk);
-    P::clear(yv);
+    floatx16 y[P::NFT];
+    P::clear(y);
     const float c = a.scale * kLog2e;
-    const QueryTiles near(a, FAR ? block * 32 / a.near_rows * a.near_rows : block * NW * 32, FAR ? a.near_rows : NW * 32);
+    const QueryTiles near(a, block * NW * 16 / a.near_rows * a.near_rows, a.near_rows);
     // the near tiles, or those beside them: [0, lo) without causal, and [hi, all)
     const int before = FAR && !a.causal ? near.lo : 0, jump = FAR ? near.hi : near.lo;
     const int tiles = FAR ? before + (a.seq_len + kTS - 1) / kTS - near.hi : near.hi - near.lo, steps = tiles * a.group;
@@ -594,6 +591,8 @@ __global__ __launch_bounds__(NW * 64) void dkv_kernel(Args a) {
             if (t0 + (int)threadIdx.x < a.seq_len) st = a.state[at], delta = a.delta[at];
         }
     };
+    char* mine = exchange + wave * 2 * P::NP * 1024 + lane * 16;
+    const char* other = exchange + (wave ^ 1) * 2 * P::NP * 1024 + lane * 16;
     if (__syncthreads_or(any)) issue();
     else i = last;
     while (i < last) {
@@ -605,67 +604,66 @@ __global__ __launch_bounds__(NW * 64) void dkv_kernel(Args a) {
         __syncthreads();
         ++i;
         issue();
-        if (!any) continue;
-#pragma unroll
-        for (int half = 0; half < (FAR ? 1 : 2); ++half) {
-            const int sub = FAR ? wave : half;
-            const int i0 = q0 + 32 * sub, seen = (uint32_t)(queries >> (32 * sub)) ? block_seen(a, i0, w0) : 0;
-            if (!seen) continue;
-            floatx16 x = P::score(lds, 0, sub, K);
+        auto seen_of = [&](int sub) {
+            return any && (uint32_t)(queries >> (32 * sub)) ? block_seen(a, q0 + 32 * sub, w0) : 0;
+        };
+        const int seen = seen_of(role), theirs = seen_of(role ^ 1);
+        if (seen) {
+            floatx16 x = P::score(lds, 0, role, K);
+            floatx16 dp = P::score(lds, 1, role, V);
             if (seen == 1 || ok != 0xFFFFFFFFu) {
-                const uint32_t bits = live ? queries_seen(a, i0, kj) >> (4 * h) : 0u;
+                const uint32_t bits = live ? queries_seen(a, q0 + 32 * role, kj) >> (4 * h) : 0u;
 #pragma unroll
                 for (int e = 0; e < 16; ++e) x[e] = row_bit(bits, e) ? x[e] : -INFINITY;
             }
-            const float* m = &meta[0][32 * sub + 4 * h];
+            const float* m = &meta[0][32 * role + 4 * h];
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
                 const int r = 8 * (e >> 2) + (e & 3);
                 x[e] = __builtin_amdgcn_exp2f(fmaf(x[e], c, -m[r])) * m[kTS + r];
+                dp[e] = x[e] * (dp[e] - m[2 * kTS + r]);
             }
-            P::gather(lds, 1, sub, x, yv);
-            floatx16 dp = P::score_of(lds, 1, sub, [&](int ks) {
-                if constexpr (!VL) return V[ks];
-                typename P::F f;
+            const floatx16 give = role ? x : dp, keep = role ? dp : x;
+#pragma unroll
+            for (int s2 = 0; s2 < 2; ++s2) {
+                const typename P::F f = P::weights_of(give, s2);
+#pragma unroll
+                for (int p = 0; p < P::NP; ++p) *reinterpret_cast<bf16x8*>(mine + (s2 * P::NP + p) * 1024) = f.p[p];
+            }
+            P::gather(lds, role ^ 1, role, keep, y);
+        }
+        __syncthreads();
+        if (theirs) {
+            typename P::F w[2];
+#pragma unroll
+            for (int s2 = 0; s2 < 2; ++s2)
 #pragma unroll
                 for (int p = 0; p < P::NP; ++p)
-                    f.p[p] = *reinterpret_cast<const bf16x8*>(mine + (ks * P::NP + p) * 1024);
-                return f;
-            });
-#pragma unroll
-            for (int e = 0; e < 16; ++e) dp[e] = x[e] * (dp[e] - m[2 * kTS + 8 * (e >> 2) + (e & 3)]);
-            P::gather(lds, 0, sub, dp, yk);
+                    w[s2].p[p] = *reinterpret_cast<const bf16x8*>(other + (s2 * P::NP + p) * 1024);
+            P::gather(lds, role ^ 1, role ^ 1, w, y);
         }
     }
     using PF = Pass<float, DP, NW>;
-    if constexpr (FAR) {  // slab (key head, sinks, piece, wave): dK and dV of 32 rows
-        float* p = a.far_part + ((((int64_t)unit * pieces + piece) * 2 + wave) * 64 + r32) * a.dim;
-        PF::write_row(p, yk, a.scale, h, a.dim);
-        PF::write_row(p + 32 * a.dim, yv, 1.f, h, a.dim);
-        return;
-    }
-    if (pieces > 1) {  // slab (key head, block, piece): dK and dV of the block's rows, zeros where there is nothing
-        float* p = a.part + ((int64_t)item * 2 * NW * 32 + wave * 32 + r32) * a.dim;
-        PF::write_row(p, yk, a.scale, h, a.dim);
-        PF::write_row(p + (int64_t)NW * 32 * a.dim, yv, 1.f, h, a.dim);
+    const float scale = role ? a.scale : 1.f;
+    if (FAR || pieces > 1) {  // slab (key head, block, piece): dK and dV of the block's rows, zeros where there is nothing
+        PF::write_row((FAR ? a.far_part : a.part) +
+                          (((int64_t)item * 2 + (role ^ 1)) * NW * 16 + (wave >> 1) * 32 + r32) * a.dim,
+                      y, scale, h, a.dim);
         return;
     }
     if (kj >= a.seq_len) return;
-    if (w0 < 32 * a.far_groups) {  // the far pass's sums, added up in its first slab (0 for rows that are no sinks)
-        const float* p = a.far_part + ((int64_t)(bk * a.far_groups + w0 / 32) * a.far_pieces * 128 + r32) * a.dim;
-        P::add_row(p, yk, 1.f / a.scale, h, a.dim);
-        P::add_row(p + 32 * a.dim, yv, 1.f, h, a.dim);
-    }
-    if (!live) P::clear(yk), P::clear(yv);
-    P::write_row(a.dk.at<T>(b, kh) + kj * a.dk.st, yk, a.scale, h, a.dim);
-    P::write_row(a.dv.at<T>(b, kh) + kj * a.dv.st, yv, 1.f, h, a.dim);
+    if (w0 < kFarRows * a.far_groups)  // the far pass's sums, added up in its first slab (0 for rows that are no sinks)
+        P::add_row(a.far_part + far_row(a, bk, kj, role ^ 1), y, 1.f / scale, h, a.dim);
+    if (!live) P::clear(y);
+    const Tensor& t = role ? a.dk : a.dv;
+    P::write_row(t.at<T>(b, kh) + kj * t.st, y, scale, h, a.dim);
 }
 
-// the far pass's slabs of 32 sinks (2 x 32 rows each) added up in the first, in order, 4 columns a thread
+// the far pass's slabs of a group of sinks added up in the first, in order, 4 columns a thread
 __global__ __launch_bounds__(256) void add_far_kernel(float* part, int slabs, int dim, int64_t total) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= total) return;
-    const int64_t slab = 64 * dim, quads = slab / 4;
+    const int64_t slab = 2 * kFarRows * dim, quads = slab / 4;
     float* p = part + i / quads * slabs * slab + i % quads * 4;
     floatx4 s = *reinterpret_cast<const floatx4*>(p);
 #pragma unroll 8
@@ -691,8 +689,8 @@ __global__ __launch_bounds__(256) void add_pieces_kernel(Args a, int64_t total) 
     if (!a.valid || a.valid[b * a.seq_len + kj]) {
         for (int p = 0; p < a.near_pieces; ++p)
             add(a.part + ((((bk * a.blocks + block) * a.near_pieces + p) * 2 + which) * a.near_rows + row) * a.dim + c);
-        if (kj < 32 * a.far_groups)
-            add(a.far_part + ((bk * a.far_groups + kj / 32) * a.far_pieces * 128 + which * 32 + kj % 32) * a.dim + c);
+        if (kj < kFarRows * a.far_groups)
+            add(a.far_part + far_row(a, bk, kj, which) + c);
     }
     const Tensor& t = which ? a.dv : a.dk;
     T* o = t.at<T>(b, kh) + kj * t.st + c;
@@ -709,14 +707,13 @@ int waves(int64_t seq_len, int dtype, int dp) {
     if (seq_len <= 64) return 2;
     return dp == 32 || (dtype == kF32 && dp == 128) ? 4 : 8;
 }
-int waves_kv(int64_t seq_len, int dtype, int dp) {
-    if (seq_len <= 64) return 2;
-    return dp != 64 ? 4 : 8;
+int waves_kv(int64_t seq_len, int dtype, int dp) {  // (two to 32 rows)
+    return seq_len <= 64 || dp == 32 || (dtype == kF32 && dp == 128) ? 4 : 8;
 }
 
 // pieces of the dK, dV passes: as many as it takes to give every CU a workgroup, each at least 6 tiles long (near) or 4
 void plan_kv(Args& a, int64_t batch, int nw) {
-    a.near_rows = nw * 32;
+    a.near_rows = nw * 16;
     a.blocks = (a.seq_len + a.near_rows - 1) / a.near_rows;
     const int64_t have = batch * a.kv_heads, all = (a.seq_len + kTS - 1) / kTS;
     const int64_t reach = std::min<int64_t>(a.seq_len, a.near_rows + (int64_t)a.window * (a.causal ? 1 : 2));
@@ -727,7 +724,7 @@ void plan_kv(Args& a, int64_t batch, int nw) {
         const QueryTiles t(a, k0, a.near_rows);
         most = std::max<int64_t>(most, all - t.hi + (a.causal ? 0 : t.lo));
     }
-    a.far_groups = most > 0 ? (a.sinks + 31) / 32 : 0;
+    a.far_groups = most > 0 ? (a.sinks + kFarRows - 1) / kFarRows : 0;
     a.far_pieces = a.far_groups ? (int)std::max<int64_t>(
         1, std::min<int64_t>({512 / (have * a.far_groups), most * a.group / 4, 64})) : 1;
 }
@@ -735,7 +732,7 @@ int64_t slab_floats(const Args& a, int64_t batch) {
     return a.near_pieces > 1 ? batch * a.kv_heads * a.blocks * a.near_pieces * 2 * a.near_rows * a.dim : 0;
 }
 int64_t far_floats(const Args& a, int64_t batch) {
-    return batch * a.kv_heads * a.far_groups * a.far_pieces * 128 * a.dim;
+    return batch * a.kv_heads * a.far_groups * a.far_pieces * 2 * kFarRows * a.dim;
 }
 
 bool sizes_ok(int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq_len, int64_t dim, int64_t window,
@@ -767,6 +764,7 @@ template <class F>
 void with_pass(int dtype, int dp, int nw, F&& f) {
     with_dtype(dtype, [&](auto t) {
         auto dim = [&](auto d) {
+            // (the workgroup sizes that waves() and waves_kv() give)
             constexpr int most = decltype(d)::value == 32 || (sizeof(t) == 4 && decltype(d)::value == 128) ? 4 : 8;
             if (nw == 2) f(t, d, std::integral_constant<int, 2>{});
             else if (nw == 4) f(t, d, std::integral_constant<int, 4>{});
@@ -866,17 +864,18 @@ ASME_API int asme_window_attention_bwd(const void* q, const void* k, const void*
     });
     if (a.far_groups) {
         const dim3 g = grid(a, key_heads * a.far_groups * a.far_pieces);
-        with_pass(dtype, dp, 2, [&](auto t, auto d, auto) {
-            hipLaunchKernelGGL((dkv_kernel<decltype(t), decltype(d)::value, 2, false, true>), g, dim3(128), 0, s, a);
+        with_pass(dtype, dp, kFarWaves, [&](auto t, auto d, auto) {
+            hipLaunchKernelGGL((dkv_kernel<decltype(t), decltype(d)::value, kFarWaves, true>), g, dim3(kFarWaves * 64), 0,
+                               s, a);
         });
-        const int64_t total = key_heads * a.far_groups * 16 * head_dim;
+        const int64_t total = key_heads * a.far_groups * 2 * kFarRows * (head_dim / 4);
         hipLaunchKernelGGL(add_far_kernel, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, s, a.far_part,
-                           2 * a.far_pieces, (int)head_dim, total);
+                           a.far_pieces, (int)head_dim, total);
     }
     const dim3 g = grid(a, k_items);
     with_pass(dtype, dp, nw, [&](auto t, auto d, auto w) {
-        constexpr int DP = decltype(d)::value, NW = decltype(w)::value;
-        hipLaunchKernelGGL((dkv_kernel<decltype(t), DP, NW, NW == 8, false>), g, dim3(nw * 64), 0, s, a);
+        constexpr int NW = decltype(w)::value == 2 ? 4 : decltype(w)::value;
+        hipLaunchKernelGGL((dkv_kernel<decltype(t), decltype(d)::value, NW, false>), g, dim3(nw * 64), 0, s, a);
     });
     if (a.near_pieces > 1) {
         const int64_t total = key_heads * 2 * seq_len * (head_dim / 4);
