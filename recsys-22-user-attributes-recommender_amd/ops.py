@@ -72,6 +72,16 @@ def _alike(like: torch.Tensor, dtype: Optional[torch.dtype] = None, **tensors):
             raise TypeError(f"{name} is {t.dtype}, expected {dtype}")
 
 
+def _call_on(t: torch.Tensor, name: str, *args):
+    """call(name, *args, stream) on t's device, whichever is current, and its current stream"""
+    dev = t.get_device()
+    if dev == torch._C._cuda_getDevice():
+        call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        with torch.cuda.device(dev):
+            call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
+
+
 def _ws_bytes(name: str, *sizes, device) -> Tuple[Optional[torch.Tensor], int]:
     """a workspace of the size a *_workspace query names"""
     n = int(getattr(_lib.load(), name)(*sizes))
@@ -1478,39 +1488,43 @@ class _GatedResidualNormFn(torch.autograd.Function):
     def forward(ctx, res, y, gate, post_w, post_b, pre_w, pre_b, rows_per_gate: int, residual_scale: float, eps: float,
                 rms: bool):
         ctx.set_materialize_grads(False)
-        n, D = res.shape
+        ctx.types = tuple(None if w is None else w.dtype for w in (post_w, post_b, pre_w, pre_b))
+        res, y, gate = (None if t is None else _aligned(t) for t in (res, y, gate))
+        post_w, post_b, pre_w, pre_b = (None if w is None else w.to(torch.float32).contiguous()
+                                        for w in (post_w, post_b, pre_w, pre_b))
+        D = res.shape[-1]
+        n = res.numel() // D
         s = torch.empty_like(res)
         z = torch.empty_like(res) if pre_w is not None else None
         stats = torch.empty(n, 4, device=res.device, dtype=torch.float32)
-        with torch.cuda.device(res.device):
-            call("asme_gated_residual_norm_fwd", ptr(res), ptr(y), ptr(gate), rows_per_gate, ptr(post_w), ptr(post_b),
-                 ptr(pre_w), ptr(pre_b), n, D, residual_scale, eps, int(rms), _dtype_code(res), ptr(s), ptr(z),
-                 ptr(stats), stream())
+        _call_on(res, "asme_gated_residual_norm_fwd", ptr(res), ptr(y), ptr(gate), rows_per_gate, ptr(post_w),
+                 ptr(post_b), ptr(pre_w), ptr(pre_b), n, D, residual_scale, eps, int(rms), _dtype_code(res), ptr(s),
+                 ptr(z), ptr(stats))
         ctx.save_for_backward(res, y, gate, post_w, post_b, pre_w, stats)
-        ctx.meta = (rows_per_gate, residual_scale, rms, pre_b is not None)
+        ctx.meta = (rows_per_gate, residual_scale, rms)
         return s, z
 
     @staticmethod
     @once_differentiable
     def backward(ctx, ds, dz):
-        res, y, gate, post_w, post_b, pre_w, stats = ctx.saved_tensors
-        rows_per_gate, residual_scale, rms, has_pre_b = ctx.meta
-        n, D = res.shape
-        need = ctx.needs_input_grad
-        ds, dz = (None if g is None else _aligned(g) for g in (ds, dz))
         if ds is None and dz is None:
             return (None,) * 11
+        res, y, gate, post_w, post_b, pre_w, stats = ctx.saved_tensors
+        rows_per_gate, residual_scale, rms = ctx.meta
+        D = res.shape[-1]
+        n = res.numel() // D
+        need = ctx.needs_input_grad
+        ds, dz = (None if g is None else _aligned(g) for g in (ds, dz))
         dres = torch.empty_like(res) if need[0] else None
         dy = torch.empty_like(res) if need[1] else None
         dgate = torch.empty_like(gate) if need[2] else None
         dw = torch.empty(4, D, device=res.device, dtype=torch.float32) if any(need[3:7]) else None
-        with torch.cuda.device(res.device):
-            shared = n if gate is None or rows_per_gate == 1 else rows_per_gate
-            ws, nb = _ws_bytes("asme_gated_residual_norm_bwd_workspace", n, D, shared, device=res.device)
-            call("asme_gated_residual_norm_bwd", ptr(res), ptr(y), ptr(gate), rows_per_gate, ptr(post_w), ptr(post_b),
-                 ptr(pre_w), n, D, residual_scale, int(rms), _dtype_code(res), ptr(stats), ptr(ds), ptr(dz), ptr(dres),
-                 ptr(dy), ptr(dgate), ptr(dw), ptr(ws), nb, stream())
-        w = [dw[i] if need[3 + i] else None for i in range(4)] if dw is not None else [None] * 4
+        shared = n if gate is None or rows_per_gate == 1 else rows_per_gate
+        ws, nb = _ws_bytes("asme_gated_residual_norm_bwd_workspace", n, D, shared, device=res.device)
+        _call_on(res, "asme_gated_residual_norm_bwd", ptr(res), ptr(y), ptr(gate), rows_per_gate, ptr(post_w),
+                 ptr(post_b), ptr(pre_w), n, D, residual_scale, int(rms), _dtype_code(res), ptr(stats), ptr(ds), ptr(dz),
+                 ptr(dres), ptr(dy), ptr(dgate), ptr(dw), ptr(ws), nb)
+        w = [dw[i].to(ctx.types[i]) if need[3 + i] else None for i in range(4)]
         return (dres, dy, dgate, w[0], w[1], w[2], w[3], None, None, None, None)
 
 
@@ -1553,11 +1567,7 @@ def gated_residual_norm(res: torch.Tensor, y: torch.Tensor, post_w: torch.Tensor
     if n == 0:
         zero = res + y * post_w.to(y.dtype)
         return zero, (zero if pre_w is not None else None)
-    s, z = _GatedResidualNormFn.apply(
-        _aligned(res).view(n, D), _aligned(y).view(n, D), None if gate is None else _aligned(gate).view(-1, D),
-        *(None if w is None else w.float().contiguous() for w in weights.values()), per, float(residual_scale),
-        float(eps), bool(rms))
-    return s.view(res.shape), (None if z is None else z.view(res.shape))
+    return _GatedResidualNormFn.apply(res, y, gate, *weights.values(), per, float(residual_scale), float(eps), bool(rms))
 
 
 class _GeluDropoutFn(torch.autograd.Function):
@@ -1659,21 +1669,19 @@ def _window_forward(q, k, v, valid, window, sinks, causal, scale, with_state):
     B, L, H, D = q.shape
     out = torch.empty(B, L, H, D, device=q.device, dtype=q.dtype)
     state = torch.empty(B, H, L, 2, device=q.device, dtype=torch.float32) if with_state else None
-    with torch.cuda.device(q.device):
-        call("asme_window_attention_fwd", ptr(q), ptr(k), ptr(v), ptr(out), _strides(q, k, v, out), ptr(valid), B, H,
-             k.shape[2], L, D, window, sinks, int(causal), scale, _dtype_code(q), ptr(state), stream())
+    _call_on(q, "asme_window_attention_fwd", ptr(q), ptr(k), ptr(v), ptr(out), _strides(q, k, v, out), ptr(valid), B, H,
+             k.shape[2], L, D, window, sinks, int(causal), scale, _dtype_code(q), ptr(state))
     return out, state
 
 
 def _window_backward(q, k, v, valid, out, state, dout, grads, window, sinks, causal, scale):
     B, L, H, D = q.shape
     dout = _strided_heads(dout)
-    with torch.cuda.device(q.device):
-        ws, nb = _ws_bytes("asme_window_attention_bwd_workspace", B, H, k.shape[2], L, D, window, sinks, int(causal),
-                         _dtype_code(q),                           device=q.device)
-        call("asme_window_attention_bwd", ptr(q), ptr(k), ptr(v), ptr(out), ptr(dout), *(ptr(g) for g in grads),
-             _strides(q, k, v, out, dout, *grads), ptr(valid), B, H, k.shape[2], L, D, window, sinks, int(causal),
-             scale, _dtype_code(q), ptr(state), ptr(ws), nb, stream())
+    ws, nb = _ws_bytes("asme_window_attention_bwd_workspace", B, H, k.shape[2], L, D, window, sinks, int(causal),
+                       _dtype_code(q), device=q.device)
+    _call_on(q, "asme_window_attention_bwd", ptr(q), ptr(k), ptr(v), ptr(out), ptr(dout), *(ptr(g) for g in grads),
+             _strides(q, k, v, out, dout, *grads), ptr(valid), B, H, k.shape[2], L, D, window, sinks, int(causal), scale,
+             _dtype_code(q), ptr(state), ptr(ws), nb)
 
 
 class _WindowAttentionFn(torch.autograd.Function):
@@ -1785,9 +1793,8 @@ def window_cache_fill(cache_k: torch.Tensor, cache_v: torch.Tensor, k: torch.Ten
     if B == 0 or k.shape[1] == 0:
         return
     k, v = _strided_heads(k.detach()), _strided_heads(v.detach())
-    with torch.cuda.device(cache_k.device):
-        call("asme_window_cache_fill", ptr(k), ptr(v), *k.stride()[:3], *v.stride()[:3], ptr(_i64(lengths)), B,
-             k.shape[1], KV, D, slots, sinks, _dtype_code(cache_k), ptr(cache_k), ptr(cache_v), stream())
+    _call_on(k, "asme_window_cache_fill", ptr(k), ptr(v), *k.stride()[:3], *v.stride()[:3], ptr(_i64(lengths)), B,
+             k.shape[1], KV, D, slots, sinks, _dtype_code(cache_k), ptr(cache_k), ptr(cache_v))
 
 
 def window_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache_k: torch.Tensor,
@@ -1814,11 +1821,9 @@ def window_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cac
     out = torch.empty_like(q)
     if B == 0:
         return out
-    with torch.cuda.device(q.device):
-        ws, nb = _ws_bytes("asme_window_step_workspace", B, q.shape[1], KV, D, slots, device=q.device)
-        call("asme_window_step", ptr(q), ptr(k), ptr(v), ptr(cache_k), ptr(cache_v), ptr(_i64(lengths)), B, q.shape[1],
-             KV, D, slots, sinks, D ** -0.5 if scale is None else scale, _dtype_code(q), ptr(ws), nb, ptr(out),
-             stream())
+    ws, nb = _ws_bytes("asme_window_step_workspace", B, q.shape[1], KV, D, slots, device=q.device)
+    _call_on(q, "asme_window_step", ptr(q), ptr(k), ptr(v), ptr(cache_k), ptr(cache_v), ptr(_i64(lengths)), B, q.shape[1],
+             KV, D, slots, sinks, D ** -0.5 if scale is None else scale, _dtype_code(q), ptr(ws), nb, ptr(out))
     return out
 
 
@@ -1983,29 +1988,32 @@ class _DistillFn(torch.autograd.Function):
     """tau^2 KL(teacher's list || softmax over the catalogue), mean over the rows with a list (csrc/distill.hip)."""
 
     @staticmethod
-    def forward(ctx, x, ids, teacher, temperature: float):
-        n, V = x.shape
-        top = ids.shape[1]
-        state = torch.empty(n, 2, device=x.device, dtype=torch.float32)
-        prob = torch.empty(n, top, device=x.device, dtype=torch.float32)
-        out = torch.empty(2, device=x.device, dtype=torch.float32)
-        with torch.cuda.device(x.device):
-            ws, nb = _ws_bytes("asme_distill_xent_workspace", n, V, device=x.device)
-            call("asme_distill_xent_fwd", ptr(x), x.stride(0), n, V, ptr(ids), ptr(teacher), top, temperature,
-                 _dtype_code(x), ptr(state), ptr(prob), ptr(ws), nb, ptr(out), stream())
+    def forward(ctx, logits, ids, teacher, temperature: float):
+        V, top = logits.shape[-1], ids.shape[-1]
+        x = logits.reshape(-1, V)
+        if x.stride(1) != 1 or x.stride(0) < V:
+            x = x.contiguous()
+        ids, teacher = _i64(ids), teacher.to(torch.float32).contiguous()
+        n, dev = x.shape[0], x.device
+        state = torch.empty(n, 2, device=dev, dtype=torch.float32)
+        prob = torch.empty(n, top, device=dev, dtype=torch.float32)
+        out = torch.empty(2, device=dev, dtype=torch.float32)
+        ws, nb = _ws_bytes("asme_distill_xent_workspace", n, V, device=dev)
+        _call_on(x, "asme_distill_xent_fwd", ptr(x), x.stride(0), n, V, ptr(ids), ptr(teacher), top, temperature,
+                 _dtype_code(x), ptr(state), ptr(prob), ptr(ws), nb, ptr(out))
         ctx.save_for_backward(x, ids, state, prob, out)
-        ctx.temperature = temperature
+        ctx.meta = (temperature, logits.shape)
         return out[0]
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dloss):
         x, ids, state, prob, out = ctx.saved_tensors
+        temperature, shape = ctx.meta
         n, V = x.shape
-        g = torch.empty(n, V, device=x.device, dtype=x.dtype)
-        with torch.cuda.device(x.device):
-            call("asme_distill_xent_bwd", ptr(x), x.stride(0), n, V, ptr(ids), ids.shape[1], ctx.temperature,
-                 _dtype_code(x), ptr(state), ptr(prob), ptr(out), ptr(_f32(dloss.reshape(1))), ptr(g), V, stream())
+        g = torch.empty(shape, device=x.device, dtype=x.dtype)
+        _call_on(x, "asme_distill_xent_bwd", ptr(x), x.stride(0), n, V, ptr(ids), ids.shape[-1], temperature,
+                 _dtype_code(x), ptr(state), ptr(prob), ptr(out), ptr(_f32(dloss)), ptr(g), V)
         return g, None, None, None
 
 
@@ -2031,13 +2039,9 @@ def distill_cross_entropy(logits: torch.Tensor, teacher_ids: torch.Tensor, teach
         raise ValueError("distill_cross_entropy gives the teacher no gradient: detach teacher_logits")
     _dtype_code(logits)
     _alike(logits, teacher_ids=teacher_ids, teacher_logits=teacher_logits)
-    x = logits.reshape(-1, V)
-    if x.shape[0] == 0:
-        return x.float().sum() * math.nan  # the mean over no rows
-    if x.stride(1) != 1 or x.stride(0) < V:
-        x = x.contiguous()
-    return _DistillFn.apply(x, _i64(teacher_ids).reshape(-1, top), teacher_logits.float().reshape(-1, top).contiguous(),
-                            float(temperature))
+    if logits.numel() == 0:
+        return logits.float().sum() * math.nan  # the mean over no rows
+    return _DistillFn.apply(logits, teacher_ids, teacher_logits, float(temperature))
 
 
 def linear_xent_ok(hidden: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None) -> bool:
