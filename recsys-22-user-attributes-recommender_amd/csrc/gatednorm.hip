@@ -10,9 +10,9 @@
 // gate: none, or one row of `dim` values for every rows_per_gate consecutive rows (all rows: a gate per channel; one
 // sequence's rows: a gate per sequence; 1: a gate per element).
 // Memory bound: forward reads res, y and writes s, z; backward reads res, y, ds, dz and writes dres, dy (s is formed
-// again from res and y, in fp32, instead of being read back rounded).  Every row is held in registers, at most 8 values a
-// thread, by as many threads as that takes (16 .. 1024, so a row's sums are shuffles within a wave up to 512 values and
-// one LDS exchange between waves beyond).  Weights stay in registers over a workgroup's rows.  Column sums: registers
+// again from res and y, in fp32, instead of being read back rounded).  A row is held in registers, one 16-byte vector a
+// thread (16 .. 1024 threads: a row's sums are lane moves within a wave, and one LDS exchange beyond it), and the next row
+// is on its way during its sums.  Weights stay in registers over a workgroup's rows.  Column sums: registers
 // over a workgroup's rows, then partial rows summed in a fixed order -- no atomics.
 #include "elem.h"
 
@@ -21,36 +21,54 @@ using namespace asme;
 namespace {
 
 constexpr int kMaxDim = 8192;
-constexpr int kPer = 8;  // values per thread
 
-// values i = 0..7 of thread t of a row: VEC: whole 16-byte vectors, else single elements kPer apart in threads
-template <class T, int TPR, bool VEC>
+template <int CTRL>
+__device__ __forceinline__ float dpp_add(float x) {
+    return x + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xF, 0xF, true));
+}
+// sum over aligned groups of N >= 16 lanes, in every lane (quad permutes, then mirrors of 8 and 16 lanes whose quads agree)
+template <int N>
+__device__ __forceinline__ float lanes_sum(float x) {
+    x = dpp_add<0x140>(dpp_add<0x141>(dpp_add<0x4E>(dpp_add<0xB1>(x))));
+    if constexpr (N >= 32) x += __shfl_xor(x, 16, 64);
+    if constexpr (N >= 64) x += __shfl_xor(x, 32, 64);
+    return x;
+}
+
+// A row over TPR threads of N values each: VEC: whole 16-byte vectors, else single elements TPR apart
+template <class T, int TPR, int N, bool VEC>
 struct Row {
-    static constexpr int TPRv = TPR;
-    static constexpr int kBlock = TPR > 256 ? TPR : 256;
-    static constexpr int kSlots = TPR >= 64 ? (TPR > 64 ? 1 : kBlock / 64) : kBlock / TPR;  // rows at a time
+    static constexpr int kPer = N, TPRv = TPR;
     static constexpr int kThreads = TPR > 64 ? TPR : 256;
-    static constexpr int E = VEC ? Elem<T>::V : 1;
-    static __device__ __forceinline__ int col(int t, int i) { return ((i / E) * TPR + t) * E + i % E; }
-    static __device__ __forceinline__ void load(const T* p, int t, int D, float (&x)[kPer]) {
-        if constexpr (VEC) {
+    static constexpr int kSlots = kThreads / TPR;  // rows at a time
+    static constexpr int E = VEC ? Elem<T>::V : 1, kVecs = N / E;
+    // a row's values as they are stored
+    struct Raw {
+        typedef T Vec __attribute__((ext_vector_type(VEC ? E : 1)));
+        std::conditional_t<VEC, Vec, T> v[kVecs];
+        __device__ __forceinline__ void load(const T* p, int t, int D) {
 #pragma unroll
-            for (int c = 0; c < kPer / E; ++c) {
-                float v[E];
+            for (int c = 0; c < kVecs; ++c) {
                 const int j = (c * TPR + t) * E;
-                if (j < D) Elem<T>::load(p + j, v);
-#pragma unroll
-                for (int e = 0; e < E; ++e) x[c * E + e] = j < D ? v[e] : 0.f;
+                // (behind the row: its first value, not used)
+                v[c] = *reinterpret_cast<const std::conditional_t<VEC, Vec, T>*>(p + (j < D ? j : 0));
             }
-        } else {
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) x[i] = i * TPR + t < D ? Elem<T>::get(p + i * TPR + t) : 0.f;
         }
-    }
-    static __device__ __forceinline__ void store(T* p, int t, int D, const float (&x)[kPer]) {
+        __device__ __forceinline__ void get(int t, int D, float (&x)[N]) const {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                float f;
+                if constexpr (VEC) f = (float)v[i / E][i % E];
+                else f = (float)v[i];
+                x[i] = col(t, i) < D ? f : 0.f;
+            }
+        }
+    };
+    static __device__ __forceinline__ int col(int t, int i) { return ((i / E) * TPR + t) * E + i % E; }
+    static __device__ __forceinline__ void store(T* p, int t, int D, const float (&x)[N]) {
         if constexpr (VEC) {
 #pragma unroll
-            for (int c = 0; c < kPer / E; ++c) {
+            for (int c = 0; c < kVecs; ++c) {
                 float v[E];
                 const int j = (c * TPR + t) * E;
 #pragma unroll
@@ -59,35 +77,32 @@ struct Row {
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < kPer; ++i)
+            for (int i = 0; i < N; ++i)
                 if (i * TPR + t < D) Elem<T>::put(p + i * TPR + t, x[i]);
         }
     }
-    static __device__ __forceinline__ void load_f32(const float* p, int t, int D, float def, float (&x)[kPer]) {
+    static __device__ __forceinline__ void load_f32(const float* p, int t, int D, float def, float (&x)[N]) {
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) {
+        for (int i = 0; i < N; ++i) {
             const int j = col(t, i);
             x[i] = p && j < D ? p[j] : (j < D ? def : 0.f);
         }
     }
-    // N sums over the row's threads, in every one of them.  Rows of more than one wave: through `red` (2 x N x 16 floats,
+    // K sums over the row's threads, in every one of them.  Rows of more than one wave: through `red` (2 x K x 16 floats,
     // alternating halves, so one barrier a call is enough); `flip` counts the calls.
-    template <int N>
-    static __device__ __forceinline__ void sum(float (&v)[N], float* red, int& flip) {
-        constexpr int W = TPR < 64 ? TPR : 64;
+    template <int K>
+    static __device__ __forceinline__ void sum(float (&v)[K], float* red, int& flip) {
 #pragma unroll
-        for (int k = 0; k < N; ++k)
-#pragma unroll
-            for (int o = W / 2; o >= 1; o >>= 1) v[k] += __shfl_xor(v[k], o, 64);
+        for (int k = 0; k < K; ++k) v[k] = lanes_sum<(TPR < 64 ? TPR : 64)>(v[k]);
         if constexpr (TPR > 64) {
             float* r = red + (flip & 1) * 32;
             ++flip;
             if ((threadIdx.x & 63) == 0)
 #pragma unroll
-                for (int k = 0; k < N; ++k) r[k * 16 + (threadIdx.x >> 6)] = v[k];
+                for (int k = 0; k < K; ++k) r[k * 16 + (threadIdx.x >> 6)] = v[k];
             __syncthreads();
 #pragma unroll
-            for (int k = 0; k < N; ++k) {
+            for (int k = 0; k < K; ++k) {
                 v[k] = 0.f;
 #pragma unroll
                 for (int w = 0; w < TPR / 64; ++w) v[k] += r[k * 16 + w];
@@ -114,7 +129,7 @@ struct Args {
 };
 
 // mean and 1 / deviation of the row's values (two passes over registers)
-template <class R>
+template <class R, int kPer = R::kPer>
 __device__ __forceinline__ void moments(const float (&x)[kPer], int t, int D, float eps, int rms, float* red, int& flip,
                                         float& mean, float& r) {
     mean = 0.f;
@@ -137,6 +152,7 @@ __device__ __forceinline__ void moments(const float (&x)[kPer], int t, int D, fl
 
 template <class T, class R>
 __global__ __launch_bounds__(R::kThreads) void fwd_kernel(Args a) {
+    constexpr int kPer = R::kPer;
     __shared__ float red[64];
     int flip = 0;
     const int t = threadIdx.x % R::TPRv, slot = R::kSlots > 1 ? threadIdx.x / R::TPRv : 0, D = a.D;
@@ -145,25 +161,35 @@ __global__ __launch_bounds__(R::kThreads) void fwd_kernel(Args a) {
     R::load_f32(a.post_b, t, D, 0.f, pb);
     R::load_f32(a.pre_w, t, D, 1.f, qw);
     R::load_f32(a.pre_b, t, D, 0.f, qb);
-    // (every thread of a workgroup makes the same number of turns: the row sums may hold a barrier)
-    for (int64_t base = (int64_t)blockIdx.x * R::kSlots; base < a.n; base += (int64_t)gridDim.x * R::kSlots) {
+    typename R::Raw raw_y, raw_s, raw_g;
+    const int64_t step = (int64_t)gridDim.x * R::kSlots;
+    auto fetch = [&](int64_t base) {  // the row that this thread's slot has from `base` on
         const int64_t row = min(base + slot, a.n - 1);
-        const bool live = base + slot < a.n;
-        float x[kPer], s[kPer], m, r;
-        R::load((const T*)a.y + row * D, t, D, x);
-        R::load((const T*)a.res + row * D, t, D, s);
-        float g[kPer];
-        if (a.gate) R::load((const T*)a.gate + row / a.rows_per_gate * D, t, D, g);
+        raw_y.load((const T*)a.y + row * D, t, D);
+        raw_s.load((const T*)a.res + row * D, t, D);
+        if (a.gate) raw_g.load((const T*)a.gate + row / a.rows_per_gate * D, t, D);
+    };
+    // (every thread of a workgroup makes the same number of turns: the row sums may hold a barrier)
+    int64_t base = (int64_t)blockIdx.x * R::kSlots;
+    if (base < a.n) fetch(base);
+    for (; base < a.n; base += step) {
+        const int64_t row = base + slot;
+        const bool live = row < a.n;
+        float x[kPer], s[kPer], g[kPer], m, r;
+        raw_y.get(t, D, x);
+        raw_s.get(t, D, s);
+        if (a.gate) raw_g.get(t, D, g);
+        if (base + step < a.n) fetch(base + step);  // the next row is on its way during this one's sums
         moments<R>(x, t, D, a.eps, a.rms, red, flip, m, r);
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
             const float b = fmaf((x[i] - m) * r, pw[i], pb[i]);
             s[i] = a.gate ? fmaf(g[i], b, a.scale * s[i]) : fmaf(a.scale, s[i], b);
+            if (R::col(t, i) >= D) s[i] = 0.f;
         }
         if (live) R::store((T*)a.s + row * D, t, D, s);
         float m2 = 0.f, r2 = 0.f;
         if (a.pre_w) {
-            // columns behind the row hold b's 0, not a number of the row
             moments<R>(s, t, D, a.eps, a.rms, red, flip, m2, r2);
 #pragma unroll
             for (int i = 0; i < kPer; ++i) s[i] = fmaf((s[i] - m2) * r2, qw[i], qb[i]);
@@ -174,7 +200,7 @@ __global__ __launch_bounds__(R::kThreads) void fwd_kernel(Args a) {
 }
 
 // the workgroup's column sums of one accumulator over its row slots -> out[0..D)
-template <class R, class Put>
+template <class R, class Put, int kPer = R::kPer>
 __device__ __forceinline__ void column_sums(const float (&acc)[kPer], int t, int slot, int D, float* buf, Put&& put) {
     if constexpr (R::kSlots == 1) {
 #pragma unroll
@@ -201,8 +227,9 @@ __device__ __forceinline__ void column_sums(const float (&acc)[kPer], int t, int
 // blockIdx.x, + gridDim.x, ...: a shared gate's sums are closed at the end of each item, the weights' at the end of all.
 template <class T, class R, int GATE>
 __global__ __launch_bounds__(R::kThreads) void bwd_kernel(Args a) {
+    constexpr int kPer = R::kPer;
     __shared__ float red[64];
-    __shared__ float buf[R::kSlots > 1 ? R::kSlots * R::TPRv * kPer : 1];
+    __shared__ float buf[R::kSlots > 1 ? R::kThreads * kPer : 1];
     int flip = 0;
     const int t = threadIdx.x % R::TPRv, slot = R::kSlots > 1 ? threadIdx.x / R::TPRv : 0, D = a.D;
     const float inv_d = 1.f / (float)D, centre = a.rms ? 0.f : 1.f;
@@ -213,29 +240,41 @@ __global__ __launch_bounds__(R::kThreads) void bwd_kernel(Args a) {
     float acc[4][kPer], gacc[kPer];
 #pragma unroll
     for (int i = 0; i < kPer; ++i) acc[0][i] = acc[1][i] = acc[2][i] = acc[3][i] = gacc[i] = 0.f;
+    typename R::Raw raw_y, raw_s, raw_d, raw_z, raw_g;
+    float4 next_st;
+    // this thread's slot of the rows from `base` on (the last one again behind `end`)
+    auto fetch = [&](int64_t base, int64_t end, int64_t group) {
+        const int64_t row = min(base + slot, end - 1);
+        next_st = *reinterpret_cast<const float4*>(a.stats + row * 4);
+        raw_y.load((const T*)a.y + row * D, t, D);
+        raw_s.load((const T*)a.res + row * D, t, D);
+        if (a.ds) raw_d.load((const T*)a.ds + row * D, t, D);
+        if (a.dz) raw_z.load((const T*)a.dz + row * D, t, D);
+        if (GATE) raw_g.load((const T*)a.gate + (GATE == 1 ? row : group) * D, t, D);
+    };
     for (int64_t item = blockIdx.x; item < a.items; item += gridDim.x) {
         const int64_t group = item / a.subs, first = (item % a.subs) * a.sub_rows;
         const int64_t begin = group * a.rows_per_gate + first;
         const int64_t end = group * a.rows_per_gate + min(a.rows_per_gate, first + a.sub_rows);
+        fetch(begin, end, group);
         for (int64_t base = begin; base < end; base += R::kSlots) {
             const bool live = base + slot < end;
             const int64_t row = live ? base + slot : end - 1;
-            const float4 st = *reinterpret_cast<const float4*>(a.stats + row * 4);
+            const float4 st = next_st;
             float y[kPer], s[kPer], d[kPer], g[kPer], dz[kPer];
-            R::load((const T*)a.y + row * D, t, D, y);
-            R::load((const T*)a.res + row * D, t, D, s);
-            if (a.ds) R::load((const T*)a.ds + row * D, t, D, d);
-            if (a.dz) R::load((const T*)a.dz + row * D, t, D, dz);
-            if (GATE == 1) R::load((const T*)a.gate + row * D, t, D, g);
-            if (GATE == 2) R::load((const T*)a.gate + group * D, t, D, g);
-            float br[kPer];
+            raw_y.get(t, D, y);
+            raw_s.get(t, D, s);
+            if (a.ds) raw_d.get(t, D, d);
+            if (a.dz) raw_z.get(t, D, dz);
+            if (GATE) raw_g.get(t, D, g);
+            if (base + R::kSlots < end) fetch(base + R::kSlots, end, group);  // on its way during this row's sums
 #pragma unroll
             for (int i = 0; i < kPer; ++i) {
                 if (!live || !a.ds) d[i] = 0.f;
                 const bool in = R::col(t, i) < D;
                 y[i] = in ? (y[i] - st.x) * st.y : 0.f;
-                br[i] = fmaf(y[i], pw[i], pb[i]);
-                s[i] = GATE ? fmaf(g[i], br[i], a.scale * s[i]) : fmaf(a.scale, s[i], br[i]);
+                const float br = fmaf(y[i], pw[i], pb[i]);
+                s[i] = GATE ? fmaf(g[i], br, a.scale * s[i]) : fmaf(a.scale, s[i], br);
                 s[i] = in ? (s[i] - st.z) * st.w : 0.f;
             }
             if (a.dz) {
@@ -261,17 +300,17 @@ __global__ __launch_bounds__(R::kThreads) void bwd_kernel(Args a) {
                 for (int i = 0; i < kPer; ++i) o[i] = a.scale * d[i];
                 R::store((T*)a.dres + row * D, t, D, o);
             }
-            if (GATE == 1 && a.dgate) {
+            if (GATE == 1 && a.dgate && live) {
                 float o[kPer];
 #pragma unroll
-                for (int i = 0; i < kPer; ++i) o[i] = d[i] * br[i];
-                if (live) R::store((T*)a.dgate + row * D, t, D, o);
+                for (int i = 0; i < kPer; ++i) o[i] = d[i] * fmaf(y[i], pw[i], pb[i]);
+                R::store((T*)a.dgate + row * D, t, D, o);
             }
             float v[2] = {0.f, 0.f};
 #pragma unroll
             for (int i = 0; i < kPer; ++i) {
                 if (R::col(t, i) >= D) d[i] = 0.f;
-                if (GATE == 2) gacc[i] = fmaf(d[i], br[i], gacc[i]);
+                if (GATE == 2) gacc[i] = fmaf(d[i], fmaf(y[i], pw[i], pb[i]), gacc[i]);
                 const float db = GATE ? d[i] * g[i] : d[i];
                 acc[0][i] = fmaf(db, y[i], acc[0][i]);
                 acc[1][i] += db;
@@ -305,22 +344,31 @@ __global__ __launch_bounds__(R::kThreads) void bwd_kernel(Args a) {
                            [&](int j, float v) { a.part[((int64_t)blockIdx.x * 4 + k) * D + j] = v; });
 }
 
-// out[g][j] = sum over m < rows of part[g * rows + m][j], j < width: 64 columns x 16 row lanes a workgroup, then the
-// lanes' sums in order
+// out[g][j] = sum over m < rows of part[g * rows + m][j], j < width: 16 columns x 64 row lanes a workgroup, then the
+// lanes' sums in order (64 columns x 16 lanes took 13 us for 1024 rows of 512: one load after another)
+constexpr int kCols = 16;
 template <class T>
 __global__ __launch_bounds__(1024) void column_reduce_kernel(const float* __restrict__ part, int64_t rows, int64_t width,
                                                              int64_t col_groups, T* __restrict__ out) {
-    __shared__ float buf[16][64];
-    const int64_t g = blockIdx.x / col_groups, j = blockIdx.x % col_groups * 64 + (threadIdx.x & 63);
-    const int lane = threadIdx.x >> 6;
+    __shared__ float buf[64][kCols + 1];
+    const int64_t g = blockIdx.x / col_groups, j = blockIdx.x % col_groups * kCols + threadIdx.x % kCols;
+    const int lane = threadIdx.x / kCols;
     float v = 0.f;
-    if (j < width)
-        for (int64_t m = lane; m < rows; m += 16) v += part[(g * rows + m) * width + j];
-    buf[lane][threadIdx.x & 63] = v;
+    if (j < width) {
+        const float* p = part + g * rows * width + j;
+#pragma unroll 8
+        for (int64_t m = lane; m < rows; m += 64) v += p[m * width];
+    }
+    buf[lane][threadIdx.x % kCols] = v;
     __syncthreads();
-    if (lane == 0 && j < width) {
-        for (int k = 1; k < 16; ++k) v += buf[k][threadIdx.x];
-        Elem<T>::put(out + g * width + j, v);
+    if (threadIdx.x < 4 * kCols) {  // a quarter of the lanes each, then the quarters
+        const int c = threadIdx.x % kCols, q = threadIdx.x / kCols;
+        v = 0.f;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) v += buf[16 * q + k][c];
+        v += __shfl_xor(v, 16, 64);
+        v += __shfl_xor(v, 32, 64);
+        if (q == 0 && j < width) Elem<T>::put(out + g * width + j, v);
     }
 }
 
@@ -330,37 +378,44 @@ bool aligned(std::initializer_list<const void*> ps) {
     return true;
 }
 
-// f(Row<...>{}) for a checked dim: the fewest threads a row that hold it at 8 values each
+// f(Row<...>{}) for a checked dim: the fewest threads a row (at least 16) that hold it at one 16-byte vector each -- 8
+// single elements where rows are not whole vectors or not aligned, two fp32 vectors beyond 4096
 template <class T, class F>
 void with_row(int64_t D, bool vec, F&& f) {
     auto pick = [&](auto v) {
         constexpr bool VEC = decltype(v)::value;
-        if (D <= 16 * kPer) f(Row<T, 16, VEC>{});
-        else if (D <= 32 * kPer) f(Row<T, 32, VEC>{});
-        else if (D <= 64 * kPer) f(Row<T, 64, VEC>{});
-        else if (D <= 128 * kPer) f(Row<T, 128, VEC>{});
-        else if (D <= 256 * kPer) f(Row<T, 256, VEC>{});
-        else if (D <= 512 * kPer) f(Row<T, 512, VEC>{});
-        else f(Row<T, 1024, VEC>{});
+        constexpr int N = VEC ? Elem<T>::V : 8;
+        if (D <= 16 * N) f(Row<T, 16, N, VEC>{});
+        else if (D <= 32 * N) f(Row<T, 32, N, VEC>{});
+        else if (D <= 64 * N) f(Row<T, 64, N, VEC>{});
+        else if (D <= 128 * N) f(Row<T, 128, N, VEC>{});
+        else if (D <= 256 * N) f(Row<T, 256, N, VEC>{});
+        else if (D <= 512 * N) f(Row<T, 512, N, VEC>{});
+        else if (N == 8 || D > 1024 * N) f(Row<T, 1024, 8, VEC>{});
+        else f(Row<T, 1024, N, VEC>{});
     };
     if (vec) pick(std::true_type{});
     else pick(std::false_type{});
 }
 
-// rows at a time and workgroups that fill the chip for a row layout
-int64_t slots_of(int64_t D) { return D <= 128 ? 16 : D <= 256 ? 8 : D <= 512 ? 4 : 1; }
-int64_t threads_of(int64_t D) {
-    return D <= 512 ? 256 : D <= 1024 ? 128 : D <= 2048 ? 256 : D <= 4096 ? 512 : 1024;
+// workgroups of a layout that fill the chip: 16 waves on each of 256 CUs, at most 1024 (their partial rows are written)
+constexpr int64_t fill_of(int64_t threads) { return std::min<int64_t>(1024, 256 * 1024 / threads); }
+template <class R>
+constexpr int64_t fill() {
+    return fill_of(R::kThreads);
 }
-int64_t resident(int64_t D) { return 256 * 1024 / threads_of(D); }  // 16 waves per CU
+// the most of them that any layout of a dim takes: rows at 8 values a thread
+int64_t most_groups(int64_t D) {
+    return fill_of(D <= 512 ? 256 : D <= 1024 ? 128 : D <= 2048 ? 256 : D <= 4096 ? 512 : 1024);
+}
 
 struct Plan {
     int64_t subs, sub_rows, items, grid;
 };
 // pieces of the backward: the rows of a shared gate (else all rows) cut so that there are enough items to fill the chip,
 // each a whole number of turns; the grid (and with it the partial rows) is at most what runs at once
-Plan plan(int64_t n, int64_t rows_per_gate, int64_t D) {
-    const int64_t groups = n / rows_per_gate, slots = slots_of(D), fill = resident(D);
+Plan plan(int64_t n, int64_t rows_per_gate, int64_t slots, int64_t fill) {
+    const int64_t groups = n / rows_per_gate;
     Plan p;
     const int64_t turns = (rows_per_gate + slots - 1) / slots;
     int64_t subs = std::min(turns, std::max<int64_t>(1, fill / groups));
@@ -396,18 +451,19 @@ ASME_API int asme_gated_residual_norm_fwd(const void* res, const void* y, const 
         with_row<T>(dim, dim % Elem<T>::V == 0 && aligned({res, y, gate, s_out, z_out}), [&](auto r) {
             using R = decltype(r);
             const int64_t turns = (n + R::kSlots - 1) / R::kSlots;
-            hipLaunchKernelGGL((fwd_kernel<T, R>), dim3((unsigned)std::min(turns, 2 * resident(dim))),
+            hipLaunchKernelGGL((fwd_kernel<T, R>), dim3((unsigned)std::min(turns, 2 * fill<R>())),
                                dim3(R::kThreads), 0, (hipStream_t)stream, a);
         });
     });
     ASME_LAUNCH_CHECK("asme_gated_residual_norm_fwd");
 }
 
-// bytes; 0 for sizes that the calls refuse
+// bytes, whatever the layout that the call takes; 0 for sizes that the calls refuse
 ASME_API int64_t asme_gated_residual_norm_bwd_workspace(int64_t n, int64_t dim, int64_t rows_per_gate) {
     if (!sizes_ok(n, dim, rows_per_gate)) return 0;
-    const Plan p = plan(n, rows_per_gate, dim);
-    return (p.grid * 4 + (p.subs > 1 ? p.items : 0)) * dim * 4;
+    // partial rows of the weights, and (only where a gate's rows are cut into pieces: then no more pieces than workgroups)
+    // of the gate
+    return std::min(n, most_groups(dim)) * 5 * dim * 4;
 }
 
 // rows_per_gate: as in the forward; n (all rows) without a gate or with a gate row for every row (gate_rows = 1)
@@ -425,20 +481,21 @@ ASME_API int asme_gated_residual_norm_bwd(const void* res, const void* y, const 
     const int64_t rows = shared ? rows_per_gate : n;
     ASME_CHECK_ARG(ws_bytes >= asme_gated_residual_norm_bwd_workspace(n, dim, rows),
                    "asme_gated_residual_norm_bwd: workspace too small");
-    const Plan p = plan(n, rows, dim);
     Args a{};
     a.res = res, a.y = y, a.gate = gate, a.post_w = post_w, a.post_b = post_b, a.pre_w = pre_w;
     a.n = n, a.rows_per_gate = rows, a.D = (int)dim, a.scale = residual_scale, a.rms = rms;
     a.stats = const_cast<float*>(stats), a.ds = ds, a.dz = dz, a.dres = dres, a.dy = dy, a.dgate = dgate;
     a.part = dw ? (float*)workspace : nullptr;
-    a.gate_part = (float*)workspace + p.grid * 4 * dim;
-    a.subs = p.subs, a.sub_rows = p.sub_rows, a.items = p.items;
     hipStream_t st = (hipStream_t)stream;
-    const unsigned cg = (unsigned)((dim + 63) / 64), cg4 = (unsigned)((4 * dim + 63) / 64);
+    const unsigned cg = (unsigned)((dim + kCols - 1) / kCols), cg4 = (unsigned)((4 * dim + kCols - 1) / kCols);
+    Plan p{};
     with_dtype(dtype, [&](auto e) {
         using T = decltype(e);
         with_row<T>(dim, dim % Elem<T>::V == 0 && aligned({res, y, gate, ds, dz, dres, dy, dgate}), [&](auto r) {
             using R = decltype(r);
+            p = plan(n, rows, R::kSlots, fill<R>());
+            a.gate_part = (float*)workspace + p.grid * 4 * dim;
+            a.subs = p.subs, a.sub_rows = p.sub_rows, a.items = p.items;
             const dim3 grid((unsigned)p.grid), block(R::kThreads);
             if (!gate) hipLaunchKernelGGL((bwd_kernel<T, R, 0>), grid, block, 0, st, a);
             else if (!shared) hipLaunchKernelGGL((bwd_kernel<T, R, 1>), grid, block, 0, st, a);
