@@ -498,11 +498,12 @@ int asme_gated_residual_norm_bwd(const void* res, const void* y, const void* gat
  * query head h reads key head h / (heads / kv_heads).  strides: HOST array of (batch, token, head) element strides of
  * q, k, v, out; a head's values are adjacent, every row on a 16-byte boundary.  valid (batch, seq_len) bytes, nullable:
  * a position that is not valid is neither query nor key -- it is not read, its rows of the outputs are 0.
- * head_dim 16, 32, 64 or 128.  state (batch, heads, seq_len, 2) for the backward, nullable. */
+ * head_dim 16, 32, 64 or 128.  For the backward, nullable: state (batch, heads, seq_len, 2), and of bf16 tensors out_low,
+ * laid out like out: what rounding took from it (the backward's row sums dout . out are formed from both). */
 int asme_window_attention_fwd(const void* q, const void* k, const void* v, void* out, const int64_t* strides,
                               const uint8_t* valid, int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq_len,
                               int64_t head_dim, int64_t window, int64_t sinks, int causal, float scale, int dtype,
-                              float* state, void* stream);
+                              void* out_low, float* state, void* stream);
 int64_t asme_window_attention_bwd_workspace(int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq_len,
                                             int64_t head_dim, int64_t window, int64_t sinks, int causal,
                                             int dtype);
@@ -510,8 +511,8 @@ int64_t asme_window_attention_bwd_workspace(int64_t batch, int64_t heads, int64_
 int asme_window_attention_bwd(const void* q, const void* k, const void* v, const void* out, const void* dout, void* dq,
                               void* dk, void* dv, const int64_t* strides, const uint8_t* valid, int64_t batch,
                               int64_t heads, int64_t kv_heads, int64_t seq_len, int64_t head_dim, int64_t window,
-                              int64_t sinks, int causal, float scale, int dtype, const float* state, void* workspace,
-                              int64_t ws_bytes, void* stream);
+                              int64_t sinks, int causal, float scale, int dtype, const void* out_low,
+                              const float* state, void* workspace, int64_t ws_bytes, void* stream);
 
 /* Serving window attention (csrc/windowcache.hip).  Cache of a sequence: cache_k, cache_v (batch, kv_heads, slots,
  * head_dim), slots = sinks + window; position p in slot p while p < sinks, then in sinks + (p - sinks) mod window.

@@ -129,10 +129,10 @@ SIGNATURES = {
     "asme_gated_residual_norm_fwd": [p, p, p, i64, p, p, p, p, i64, i64, f32, f32, i32, i32, p, p, p, p],
     "asme_gated_residual_norm_bwd_workspace": [i64, i64, i64],
     "asme_gated_residual_norm_bwd": [p, p, p, i64, p, p, p, i64, i64, f32, i32, i32, p, p, p, p, p, p, p, p, i64, p],
-    "asme_window_attention_fwd": [p, p, p, p, p, p, i64, i64, i64, i64, i64, i64, i64, i32, f32, i32, p, p],
+    "asme_window_attention_fwd": [p, p, p, p, p, p, i64, i64, i64, i64, i64, i64, i64, i32, f32, i32, p, p, p],
     "asme_window_attention_bwd_workspace": [i64, i64, i64, i64, i64, i64, i64, i32, i32],
     "asme_window_attention_bwd": [p, p, p, p, p, p, p, p, p, p, i64, i64, i64, i64, i64, i64, i64, i32, f32, i32, p, p,
-                                  i64, p],
+                                  p, i64, p],
     "asme_window_step_workspace": [i64, i64, i64, i64, i64],
     "asme_window_step": [p, p, p, p, p, p, i64, i64, i64, i64, i64, i64, f32, i32, p, i64, p, p],
     "asme_window_cache_fill": [p, p, i64, i64, i64, i64, i64, i64, p, i64, i64, i64, i64, i64, i64, i32, p, p, p],

@@ -24,8 +24,9 @@
 // (7 products for the 5 of a single pass), so no sum depends on the order of atomics.
 //
 // fp32 tensors are split exactly into three bf16 planes on the way into LDS and the products kept to fp32 level by six
-// MFMAs (common.h, bf16x6); bf16 tensors take one, P and dS rounded to bf16 for their second product (at most 2^-8 of
-// each term, the size of the output's own rounding, averaged over the row).  Scores, softmax statistics and all sums are fp32.
+// MFMAs (common.h, bf16x6); bf16 tensors take one, P rounded to bf16 for its second product (at most 2^-8 of each
+// term, the size of the output's own rounding, averaged over the row).  dS, whose terms cancel (a row of it sums to 0),
+// goes in as two bf16 terms: rounded to one, dQ was off by 1.5 times its own rounding, now by KDQ.  Scores, softmax statistics and all sums are fp32.
 #include "elem.h"
 
 using namespace asme;
@@ -62,6 +63,19 @@ __device__ __forceinline__ floatx16 product(const Frag<3>& a, const Frag<3>& b, 
     c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[1], b.p[0], c, 0, 0, 0);
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[0], b.p[0], c, 0, 0, 0);
 }
+__device__ __forceinline__ floatx16 product(const Frag<1>& a, const Frag<2>& b, floatx16 c) {
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[0], b.p[1], c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[0], b.p[0], c, 0, 0, 0);
+}
+__device__ __forceinline__ Frag<2> frag_of(const float (&x)[8], Frag<2>*) {  // to 2^-16
+    Frag<2> f;
+    f.p[0] = Elem<__bf16>::pack(x);
+    float r[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = x[i] - (float)f.p[0][i];
+    f.p[1] = Elem<__bf16>::pack(r);
+    return f;
+}
 __device__ __forceinline__ Frag<1> frag_of(const float (&x)[8], Frag<1>*) { return {Elem<__bf16>::pack(x)}; }
 __device__ __forceinline__ Frag<3> frag_of(const float (&x)[8], Frag<3>*) {
     const Bf3 s = split_bf3(make_float4(x[0], x[1], x[2], x[3]), make_float4(x[4], x[5], x[6], x[7]));
@@ -81,6 +95,7 @@ struct Tensor {
 struct Args {
     Tensor q, k, v, out, dout, dq, dk, dv;
     const uint8_t* valid;  // (batch, seq_len) or null
+    void* out_low;         // bf16 only, null or laid out like out: what rounding took from it
     float2* state;         // (batch, heads, seq_len): maximum of the scaled scores in base 2, 1 / sum
     float* delta;          // (batch, heads, seq_len): D
     float *part, *far_part;  // partial dK, dV: (key head, block, piece, 2, rows, dim), (key head, sinks, piece, 2, 64, dim)
@@ -133,6 +148,7 @@ struct Pass {
     static constexpr int kImages = DP == 128 ? 2 : 1;
     static constexpr int kBytes = NP * kImages * kImage;
     using F = Frag<NP>;
+    using S = Frag<NP == 1 ? 2 : NP>;  // dS as a factor
 
     static __device__ __forceinline__ int place(int op, int plane, int row, int ch) {
         if constexpr (DP == 128) return (plane * 2 + op) * kImage + swz(row, ch);
@@ -231,13 +247,15 @@ struct Pass {
             }
         }
     }
-    static __device__ __forceinline__ F weights_of(const floatx16& x, int s2) {
+    template <class W>
+    static __device__ __forceinline__ W weights_of(const floatx16& x, int s2) {
         float v[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = x[8 * s2 + j];
-        return frag_of(v, (F*)nullptr);
+        return frag_of(v, (W*)nullptr);
     }
-    static __device__ __forceinline__ void gather(const char* lds, int op, int sub, const F (&w)[2], floatx16 (&y)[NFT]) {
+    template <class W>
+    static __device__ __forceinline__ void gather(const char* lds, int op, int sub, const W (&w)[2], floatx16 (&y)[NFT]) {
 #pragma unroll
         for (int s2 = 0; s2 < 2; ++s2) {
             F A[NFT];
@@ -246,9 +264,31 @@ struct Pass {
             for (int ft = 0; ft < NFT; ++ft) y[ft] = product(A[ft], w[s2], y[ft]);
         }
     }
-    static __device__ __forceinline__ void gather(const char* lds, int op, int sub, const floatx16& x,
-                                                  floatx16 (&y)[NFT]) {
-        const F w[2] = {weights_of(x, 0), weights_of(x, 1)};
+    template <class W>
+    static __device__ __forceinline__ void gather_as(const char* lds, int op, int sub, const floatx16& x,
+                                                     floatx16 (&y)[NFT]) {
+        const W w[2] = {weights_of<W>(x, 0), weights_of<W>(x, 1)};
+        gather(lds, op, sub, w, y);
+    }
+    // fragments in lane order: a wave's plane p of k step s2 is 1 KiB at `at` + (s2 planes + p) KiB
+    static __device__ __forceinline__ void pass_on(char* at, const floatx16& x) {
+        constexpr int planes = sizeof(S) / 16;
+#pragma unroll
+        for (int s2 = 0; s2 < 2; ++s2) {
+            const S f = weights_of<S>(x, s2);
+#pragma unroll
+            for (int p = 0; p < planes; ++p) *reinterpret_cast<bf16x8*>(at + (s2 * planes + p) * 1024) = f.p[p];
+        }
+    }
+    static __device__ __forceinline__ void gather_passed(const char* at, const char* lds, int op, int sub,
+                                                         floatx16 (&y)[NFT]) {
+        constexpr int planes = sizeof(S) / 16;
+        S w[2];
+#pragma unroll
+        for (int s2 = 0; s2 < 2; ++s2)
+#pragma unroll
+            for (int p = 0; p < planes; ++p)
+                w[s2].p[p] = *reinterpret_cast<const bf16x8*>(at + (s2 * planes + p) * 1024);
         gather(lds, op, sub, w, y);
     }
     // row `row` (features 32 ft + 8 i + 4 h .. + 3 of this lane's stationary row) = y * f
@@ -268,6 +308,24 @@ struct Pass {
                         bf16x4{(__bf16)(y[ft][4 * i] * f), (__bf16)(y[ft][4 * i + 1] * f),
                                (__bf16)(y[ft][4 * i + 2] * f), (__bf16)(y[ft][4 * i + 3] * f)};
                 }
+            }
+    }
+    // low = what rounding takes from y * f where write_row() stores it
+    static __device__ __forceinline__ void write_low(__bf16* row, const floatx16 (&y)[NFT], float f, int h, int dim) {
+#pragma unroll
+        for (int ft = 0; ft < NFT; ++ft)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int c = 32 * ft + 8 * i + 4 * h;
+                if (c >= dim) continue;
+                typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+                bf16x4 v;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float x = y[ft][4 * i + e] * f;
+                    v[e] = (__bf16)(x - (float)(__bf16)x);
+                }
+                *reinterpret_cast<bf16x4*>(row + c) = v;
             }
     }
     // y += f * a row of fp32 values laid out like that
@@ -414,7 +472,7 @@ __global__ __launch_bounds__(NW * 64) void forward_kernel(Args a) {
                 x[e] = __builtin_amdgcn_exp2f(fmaf(x[e], c, -base));
                 sum += x[e];
             }
-            P::gather(lds, 1, sub, x, y);
+            P::template gather_as<typename P::F>(lds, 1, sub, x, y);
         }
     }
     sum += __shfl_xor(sum, 32, 64);
@@ -422,6 +480,8 @@ __global__ __launch_bounds__(NW * 64) void forward_kernel(Args a) {
     const float inv = live ? 1.f / sum : 0.f;
     if (!live) P::clear(y);
     P::write_row(a.out.at<T>(b, head) + qi * a.out.st, y, inv, h, a.dim);
+    if constexpr (sizeof(T) == 2)
+        if (a.out_low) P::write_low((T*)a.out_low + b * a.out.sb + head * a.out.sh + qi * a.out.st, y, inv, h, a.dim);
     // a position that is no query: P = 2^-inf = 0 in the backward
     if (a.state && h == 0) a.state[(b * a.heads + head) * a.seq_len + qi] = make_float2(live ? top : INFINITY, inv);
 }
@@ -444,11 +504,13 @@ __global__ __launch_bounds__(NW * 64) void dq_kernel(Args a) {
     typename P::F Q[P::KS], O[P::KS];
     P::stationary(Q, live ? a.q.at<T>(b, head) + qi * a.q.st : nullptr, h, a.dim);
     P::stationary(O, live ? a.dout.at<T>(b, head) + qi * a.dout.st : nullptr, h, a.dim);
-    // D of the row: each half of the lanes holds half of its columns
+    // D of the row: each half of the lanes holds half of its columns.  O with what its rounding took: D is the same number
+    // for every key of the row, so that its error would not average out of dQ and dK as the rounding of dS does
     float delta = 0.f;
     if (live) {
         const T* o = a.out.at<T>(b, head) + qi * a.out.st;
         const T* d = a.dout.at<T>(b, head) + qi * a.dout.st;
+        const T* low = a.out_low ? (const T*)a.out_low + (o - (const T*)a.out.p) : nullptr;
 #pragma unroll
         for (int ks = 0; ks < P::KS; ++ks) {
             if (16 * ks >= a.dim) continue;
@@ -460,6 +522,11 @@ __global__ __launch_bounds__(NW * 64) void dq_kernel(Args a) {
                 Elem<T>::load(d + 16 * ks + 8 * h + e, z);
 #pragma unroll
                 for (int k = 0; k < E; ++k) delta = fmaf(x[k], z[k], delta);
+                if (low) {
+                    Elem<T>::load(low + 16 * ks + 8 * h + e, x);
+#pragma unroll
+                    for (int k = 0; k < E; ++k) delta = fmaf(x[k], z[k], delta);
+                }
             }
         }
     }
@@ -508,7 +575,7 @@ __global__ __launch_bounds__(NW * 64) void dq_kernel(Args a) {
 #pragma unroll
             for (int e = 0; e < 16; ++e)
                 x[e] = __builtin_amdgcn_exp2f(fmaf(x[e], c, -st.x)) * st.y * (dp[e] - delta);
-            P::gather(lds, 0, sub, x, y);
+            P::template gather_as<typename P::S>(lds, 0, sub, x, y);
         }
     }
     if (qi >= a.seq_len) return;
@@ -547,8 +614,9 @@ __device__ __forceinline__ int64_t far_row(const Args& a, int64_t bk, int kj, in
 template <class T, int DP, int NW, bool FAR>
 __global__ __launch_bounds__(NW * 64) void dkv_kernel(Args a) {
     using P = Pass<T, DP, NW>;
+    constexpr int kPassed = 2 * 64 * sizeof(typename P::S);
     __shared__ __attribute__((aligned(16))) char lds[P::kBytes];
-    __shared__ __attribute__((aligned(16))) char exchange[NW * 2 * P::NP * 1024];  // fragments in lane order
+    __shared__ __attribute__((aligned(16))) char exchange[NW * kPassed];  // P or dS of a wave's half
     __shared__ __attribute__((aligned(16))) float meta[3][kTS];  // maximum, 1 / sum, D of the tile's queries
     uint32_t item;
     if (!item_of(a, item)) return;
@@ -591,8 +659,8 @@ __global__ __launch_bounds__(NW * 64) void dkv_kernel(Args a) {
             if (t0 + (int)threadIdx.x < a.seq_len) st = a.state[at], delta = a.delta[at];
         }
     };
-    char* mine = exchange + wave * 2 * P::NP * 1024 + lane * 16;
-    const char* other = exchange + (wave ^ 1) * 2 * P::NP * 1024 + lane * 16;
+    char* mine = exchange + wave * kPassed + lane * 16;
+    const char* other = exchange + (wave ^ 1) * kPassed + lane * 16;
     if (__syncthreads_or(any)) issue();
     else i = last;
     while (i < last) {
@@ -623,25 +691,12 @@ __global__ __launch_bounds__(NW * 64) void dkv_kernel(Args a) {
                 x[e] = __builtin_amdgcn_exp2f(fmaf(x[e], c, -m[r])) * m[kTS + r];
                 dp[e] = x[e] * (dp[e] - m[2 * kTS + r]);
             }
-            const floatx16 give = role ? x : dp, keep = role ? dp : x;
-#pragma unroll
-            for (int s2 = 0; s2 < 2; ++s2) {
-                const typename P::F f = P::weights_of(give, s2);
-#pragma unroll
-                for (int p = 0; p < P::NP; ++p) *reinterpret_cast<bf16x8*>(mine + (s2 * P::NP + p) * 1024) = f.p[p];
-            }
-            P::gather(lds, role ^ 1, role, keep, y);
+            // (P as finely as dS: one path for both waves -- a branch for each had the pass spill)
+            P::pass_on(mine, role ? x : dp);
+            P::template gather_as<typename P::S>(lds, role ^ 1, role, role ? dp : x, y);
         }
         __syncthreads();
-        if (theirs) {
-            typename P::F w[2];
-#pragma unroll
-            for (int s2 = 0; s2 < 2; ++s2)
-#pragma unroll
-                for (int p = 0; p < P::NP; ++p)
-                    w[s2].p[p] = *reinterpret_cast<const bf16x8*>(other + (s2 * P::NP + p) * 1024);
-            P::gather(lds, role ^ 1, role ^ 1, w, y);
-        }
+        if (theirs) P::gather_passed(other, lds, role ^ 1, role ^ 1, y);
     }
     using PF = Pass<float, DP, NW>;
     const float scale = role ? a.scale : 1.f;
@@ -781,7 +836,7 @@ void with_pass(int dtype, int dp, int nw, F&& f) {
 ASME_API int asme_window_attention_fwd(const void* q, const void* k, const void* v, void* out, const int64_t* strides,
                                        const uint8_t* valid, int64_t batch, int64_t heads, int64_t kv_heads,
                                        int64_t seq_len, int64_t head_dim, int64_t window, int64_t sinks, int causal,
-                                       float scale, int dtype, float* state, void* stream) {
+                                       float scale, int dtype, void* out_low, float* state, void* stream) {
     ASME_CHECK_ARG(q && k && v && out && strides, "asme_window_attention_fwd: null pointer");
     ASME_CHECK_ARG(dtype_ok(dtype), "asme_window_attention_fwd: dtype is 0 (fp32) or 1 (bf16)");
     ASME_CHECK_ARG(sizes_ok(batch, heads, kv_heads, seq_len, head_dim, window, sinks),
@@ -792,7 +847,9 @@ ASME_API int asme_window_attention_fwd(const void* q, const void* k, const void*
     const int64_t per = 16 / dtype_size(dtype);
     ASME_CHECK_ARG(strides_ok(a.q, per) && strides_ok(a.k, per) && strides_ok(a.v, per) && strides_ok(a.out, per),
                    "asme_window_attention_fwd: 16-byte alignment");
-    a.state = (float2*)state;
+    ASME_CHECK_ARG(!out_low || (dtype == kBF16 && ((uintptr_t)out_low & 15) == 0),
+                   "asme_window_attention_fwd: out_low is of bf16, 16-byte aligned");
+    a.state = (float2*)state, a.out_low = out_low;
     const int dp = padded_dim(head_dim), nw = waves(seq_len, dtype, dp);
     a.blocks = (int)((seq_len + nw * 32 - 1) / (nw * 32));
     const int64_t items = batch * heads * a.blocks;
@@ -819,7 +876,8 @@ ASME_API int asme_window_attention_bwd(const void* q, const void* k, const void*
                                        void* dq, void* dk, void* dv, const int64_t* strides, const uint8_t* valid,
                                        int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq_len,
                                        int64_t head_dim, int64_t window, int64_t sinks, int causal, float scale,
-                                       int dtype, const float* state, void* workspace, int64_t ws_bytes, void* stream) {
+                                       int dtype, const void* out_low, const float* state, void* workspace,
+                                       int64_t ws_bytes, void* stream) {
     ASME_CHECK_ARG(q && k && v && out && dout && dq && dk && dv && strides && state && workspace,
                    "asme_window_attention_bwd: null pointer");
     ASME_CHECK_ARG(dtype_ok(dtype), "asme_window_attention_bwd: dtype is 0 (fp32) or 1 (bf16)");
@@ -838,7 +896,9 @@ ASME_API int asme_window_attention_bwd(const void* q, const void* k, const void*
         *ts[i] = tensor(ps[i], strides + 3 * i);
         ASME_CHECK_ARG(strides_ok(*ts[i], per), "asme_window_attention_bwd: 16-byte alignment");
     }
-    a.state = (float2*)const_cast<float*>(state);
+    ASME_CHECK_ARG(!out_low || (dtype == kBF16 && ((uintptr_t)out_low & 15) == 0),
+                   "asme_window_attention_bwd: out_low is of bf16, 16-byte aligned");
+    a.state = (float2*)const_cast<float*>(state), a.out_low = const_cast<void*>(out_low);
     a.delta = (float*)workspace;
     a.part = a.delta + (batch * heads * seq_len + 3) / 4 * 4;
     const int dp = padded_dim(head_dim), nq = waves(seq_len, dtype, dp), nw = waves_kv(seq_len, dtype, dp);

@@ -1666,22 +1666,24 @@ def _strides(*ts):
 
 
 def _window_forward(q, k, v, valid, window, sinks, causal, scale, with_state):
+    """(out, what the backward takes beside it: the rows' softmax state and, of bf16, what rounding took from out)"""
     B, L, H, D = q.shape
     out = torch.empty(B, L, H, D, device=q.device, dtype=q.dtype)
     state = torch.empty(B, H, L, 2, device=q.device, dtype=torch.float32) if with_state else None
+    low = torch.empty_like(out) if with_state and out.dtype == torch.bfloat16 else None
     _call_on(q, "asme_window_attention_fwd", ptr(q), ptr(k), ptr(v), ptr(out), _strides(q, k, v, out), ptr(valid), B, H,
-             k.shape[2], L, D, window, sinks, int(causal), scale, _dtype_code(q), ptr(state))
-    return out, state
+             k.shape[2], L, D, window, sinks, int(causal), scale, _dtype_code(q), ptr(low), ptr(state))
+    return out, low, state
 
 
-def _window_backward(q, k, v, valid, out, state, dout, grads, window, sinks, causal, scale):
+def _window_backward(q, k, v, valid, out, low, state, dout, grads, window, sinks, causal, scale):
     B, L, H, D = q.shape
     dout = _strided_heads(dout)
     ws, nb = _ws_bytes("asme_window_attention_bwd_workspace", B, H, k.shape[2], L, D, window, sinks, int(causal),
                        _dtype_code(q), device=q.device)
     _call_on(q, "asme_window_attention_bwd", ptr(q), ptr(k), ptr(v), ptr(out), ptr(dout), *(ptr(g) for g in grads),
              _strides(q, k, v, out, dout, *grads), ptr(valid), B, H, k.shape[2], L, D, window, sinks, int(causal), scale,
-             _dtype_code(q), ptr(state), ptr(ws), nb)
+             _dtype_code(q), ptr(low), ptr(state), ptr(ws), nb)
 
 
 class _WindowAttentionFn(torch.autograd.Function):
@@ -1689,17 +1691,17 @@ class _WindowAttentionFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, valid, *how):
-        out, state = _window_forward(q, k, v, valid, *how, any(ctx.needs_input_grad[:3]))
-        ctx.save_for_backward(q, k, v, valid, out, state)
+        out, *kept = _window_forward(q, k, v, valid, *how, any(ctx.needs_input_grad[:3]))
+        ctx.save_for_backward(q, k, v, valid, out, *kept)
         ctx.how = how
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        q, k, v, valid, out, state = ctx.saved_tensors
+        q, k, v, valid, out, *kept = ctx.saved_tensors
         grads = [torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in (q, k, v)]
-        _window_backward(q, k, v, valid, out, state, dout, grads, *ctx.how)
+        _window_backward(q, k, v, valid, out, *kept, dout, grads, *ctx.how)
         return (*grads, *([None] * (1 + len(ctx.how))))
 
 
@@ -1709,17 +1711,17 @@ class _WindowAttentionQKVFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, qkv, valid, heads: int, *how):
         kv = (qkv.shape[2] - heads) // 2
-        out, state = _window_forward(*qkv.split((heads, kv, kv), 2), valid, *how, ctx.needs_input_grad[0])
-        ctx.save_for_backward(qkv, valid, out, state)
+        out, *kept = _window_forward(*qkv.split((heads, kv, kv), 2), valid, *how, ctx.needs_input_grad[0])
+        ctx.save_for_backward(qkv, valid, out, *kept)
         ctx.how, ctx.parts = how, (heads, kv, kv)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        qkv, valid, out, state = ctx.saved_tensors
+        qkv, valid, out, *kept = ctx.saved_tensors
         grad = torch.empty(qkv.shape, device=qkv.device, dtype=qkv.dtype)
-        _window_backward(*qkv.split(ctx.parts, 2), valid, out, state, dout, grad.split(ctx.parts, 2), *ctx.how)
+        _window_backward(*qkv.split(ctx.parts, 2), valid, out, *kept, dout, grad.split(ctx.parts, 2), *ctx.how)
         return (grad, None, None, *([None] * len(ctx.how)))
 
 
