@@ -24,9 +24,9 @@
 // (7 products for the 5 of a single pass), so no sum depends on the order of atomics.
 //
 // fp32 tensors are split exactly into three bf16 planes on the way into LDS and the products kept to fp32 level by six
-// MFMAs (common.h, bf16x6); bf16 tensors take one, P rounded to bf16 for its second product (at most 2^-8 of each
-// term, the size of the output's own rounding, averaged over the row).  dS, whose terms cancel (a row of it sums to 0),
-// goes in as two bf16 terms: rounded to one, dQ was off by 1.5 times its own rounding, now by KDQ.  Scores, softmax statistics and all sums are fp32.
+// MFMAs (common.h, bf16x6); bf16 tensors take one, P and dS rounded to bf16 for their second product (at most 2^-8 of
+// each term, the size of the output's own rounding, averaged over the row) -- but for dQ, where the terms cancel (a row of
+// dS sums to 0) and dS goes in as two bf16 terms: rounded to one, dQ was off by 1.5 times its own rounding.  Scores, softmax statistics and all sums are fp32.
 #include "elem.h"
 
 using namespace asme;
@@ -148,7 +148,7 @@ struct Pass {
     static constexpr int kImages = DP == 128 ? 2 : 1;
     static constexpr int kBytes = NP * kImages * kImage;
     using F = Frag<NP>;
-    using S = Frag<NP == 1 ? 2 : NP>;  // dS as a factor
+    using S = Frag<NP == 1 ? 2 : NP>;  // dS as a factor of dQ
 
     static __device__ __forceinline__ int place(int op, int plane, int row, int ch) {
         if constexpr (DP == 128) return (plane * 2 + op) * kImage + swz(row, ch);
@@ -270,25 +270,22 @@ struct Pass {
         const W w[2] = {weights_of<W>(x, 0), weights_of<W>(x, 1)};
         gather(lds, op, sub, w, y);
     }
-    // fragments in lane order: a wave's plane p of k step s2 is 1 KiB at `at` + (s2 planes + p) KiB
+    // fragments in lane order: a wave's plane p of k step s2 is 1 KiB at `at` + (s2 NP + p) KiB
     static __device__ __forceinline__ void pass_on(char* at, const floatx16& x) {
-        constexpr int planes = sizeof(S) / 16;
 #pragma unroll
         for (int s2 = 0; s2 < 2; ++s2) {
-            const S f = weights_of<S>(x, s2);
+            const F f = weights_of<F>(x, s2);
 #pragma unroll
-            for (int p = 0; p < planes; ++p) *reinterpret_cast<bf16x8*>(at + (s2 * planes + p) * 1024) = f.p[p];
+            for (int p = 0; p < NP; ++p) *reinterpret_cast<bf16x8*>(at + (s2 * NP + p) * 1024) = f.p[p];
         }
     }
     static __device__ __forceinline__ void gather_passed(const char* at, const char* lds, int op, int sub,
                                                          floatx16 (&y)[NFT]) {
-        constexpr int planes = sizeof(S) / 16;
-        S w[2];
+        F w[2];
 #pragma unroll
         for (int s2 = 0; s2 < 2; ++s2)
 #pragma unroll
-            for (int p = 0; p < planes; ++p)
-                w[s2].p[p] = *reinterpret_cast<const bf16x8*>(at + (s2 * planes + p) * 1024);
+            for (int p = 0; p < NP; ++p) w[s2].p[p] = *reinterpret_cast<const bf16x8*>(at + (s2 * NP + p) * 1024);
         gather(lds, op, sub, w, y);
     }
     // row `row` (features 32 ft + 8 i + 4 h .. + 3 of this lane's stationary row) = y * f
@@ -614,7 +611,7 @@ __device__ __forceinline__ int64_t far_row(const Args& a, int64_t bk, int kj, in
 template <class T, int DP, int NW, bool FAR>
 __global__ __launch_bounds__(NW * 64) void dkv_kernel(Args a) {
     using P = Pass<T, DP, NW>;
-    constexpr int kPassed = 2 * 64 * sizeof(typename P::S);
+    constexpr int kPassed = 2 * 64 * sizeof(typename P::F);
     __shared__ __attribute__((aligned(16))) char lds[P::kBytes];
     __shared__ __attribute__((aligned(16))) char exchange[NW * kPassed];  // P or dS of a wave's half
     __shared__ __attribute__((aligned(16))) float meta[3][kTS];  // maximum, 1 / sum, D of the tile's queries
@@ -691,9 +688,9 @@ __global__ __launch_bounds__(NW * 64) void dkv_kernel(Args a) {
                 x[e] = __builtin_amdgcn_exp2f(fmaf(x[e], c, -m[r])) * m[kTS + r];
                 dp[e] = x[e] * (dp[e] - m[2 * kTS + r]);
             }
-            // (P as finely as dS: one path for both waves -- a branch for each had the pass spill)
+            // (one path for both waves: a branch for each had the pass spill)
             P::pass_on(mine, role ? x : dp);
-            P::template gather_as<typename P::S>(lds, role ^ 1, role, role ? dp : x, y);
+            P::template gather_as<typename P::F>(lds, role ^ 1, role, role ? dp : x, y);
         }
         __syncthreads();
         if (theirs) P::gather_passed(other, lds, role ^ 1, role ^ 1, y);
