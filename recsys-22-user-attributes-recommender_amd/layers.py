@@ -224,9 +224,18 @@ class Attention(nn.Module):
 
 
 class MultiHeadedAttention(nn.Module):
-    def __init__(self, heads: int, d_model: int, dropout: float = 0.1):
+    """window: positions that a query sees (None: all), beside the first `sinks` (ops.window_attention); then without
+    attention dropout"""
+
+    def __init__(self, heads: int, d_model: int, dropout: float = 0.1, window: Optional[int] = None, sinks: int = 0):
         super().__init__()
         assert d_model % heads == 0
+        if window is not None and dropout > 0.0:
+            raise ValueError("attention_window has no attention dropout: set transformer_attention_dropout=0")
+        if (window is not None and window < 1) or sinks < 0 or (window is None and sinks):
+            raise ValueError(f"attention_window {window}, attention_sinks {sinks}: expected a window of at least one "
+                             "position, and sinks only beside one")
+        self.window, self.sinks = window, sinks
         self.d_k = d_model // heads
         self.heads = heads
         self.linear_layers = nn.ModuleList([nn.Linear(d_model, d_model) for _ in range(3)])
@@ -250,6 +259,32 @@ class MultiHeadedAttention(nn.Module):
         return ops.linear_row_parts(x, ws, bs)
 
 
+    def attend(self, qkv, key_valid, causal: bool, p_drop: float):
+        """the heads' outputs side by side (transformer_layers.py:138-155), over the window where there is one"""
+        if self.window is None:
+            return ops.attention(qkv, key_valid, self.heads, causal, p_drop)
+        return ops.window_attention_qkv(qkv, self.heads, self.window, sinks=self.sinks, causal=causal, valid=key_valid)
+
+
+class GatedNorm(nn.Module):
+    """What a gated block puts behind a sublayer: a norm of its output and a gate for each channel
+    (ops.gated_residual_norm with the next sublayer's own norm)."""
+
+    def __init__(self, size: int):
+        super().__init__()
+        self.norm = LayerNorm(size)
+        self.gate = nn.Parameter(torch.ones(size))
+
+    def residual(self, res, y, nxt: Optional[nn.LayerNorm]):
+        """(res + gate * norm(y), nxt of it or None)"""
+        if nxt is not None and (has_forward_hooks(nxt) or nxt.eps != self.norm.eps):
+            s, _ = ops.gated_residual_norm(res, y, self.norm.weight, self.norm.bias, gate=self.gate, eps=self.norm.eps)
+            return s, nxt(s)
+        w, b = (None, None) if nxt is None else (nxt.weight, nxt.bias)
+        return ops.gated_residual_norm(res, y, self.norm.weight, self.norm.bias, w, b, gate=self.gate,
+                                       eps=self.norm.eps)
+
+
 class PositionwiseFeedForward(nn.Module):
     def __init__(self, d_model: int, d_ff: int, dropout: float = 0.1):
         super().__init__()
@@ -261,29 +296,82 @@ class PositionwiseFeedForward(nn.Module):
 
 class TransformerBlock(nn.Module):
     def __init__(self, hidden: int, attn_heads: int, feed_forward_hidden: int, dropout: float,
-                 attention_dropout: float = None):
+                 attention_dropout: float = None, attention_window: Optional[int] = None, attention_sinks: int = 0,
+                 gated_norms: bool = False):
         super().__init__()
         if attention_dropout is None:
             attention_dropout = dropout
-        self.attention = MultiHeadedAttention(heads=attn_heads, d_model=hidden, dropout=attention_dropout)
+        self.attention = MultiHeadedAttention(heads=attn_heads, d_model=hidden, dropout=attention_dropout,
+                                              window=attention_window, sinks=attention_sinks)
         self.feed_forward = PositionwiseFeedForward(d_model=hidden, d_ff=feed_forward_hidden, dropout=dropout)
         self.input_sublayer = SublayerConnection(size=hidden, dropout=dropout)
         self.output_sublayer = SublayerConnection(size=hidden, dropout=dropout)
         self.dropout = nn.Dropout(p=dropout)
+        if gated_norms:
+            self.input_gate, self.output_gate = GatedNorm(hidden), GatedNorm(hidden)
+
+
+class WindowCaches:
+    """The ring caches of every block's keys and values while sequences are served (ops.window_attention_step), and the
+    tokens that each sequence has so far.  `most` is the longest sequence's count as the host knows it."""
+
+    def __init__(self, blocks, batch: int, device, dtype=torch.float32):
+        att = [b.attention for b in blocks]
+        if not att or any(a.window is None for a in att):
+            raise ValueError("only blocks with an attention_window are served from ring caches")
+        self.sinks = att[0].sinks
+        self.layers = [tuple(torch.zeros(batch, a.heads, a.sinks + a.window, a.d_k, device=device, dtype=dtype)
+                             for _ in range(2)) for a in att]
+        self.lengths = torch.zeros(batch, dtype=torch.int64, device=device)
+        self.most = 0
 
 
 class TransformerLayer(nn.Module):
+    """attention_window / attention_sinks: sliding-window attention in every block; gated_norms: every sublayer's output
+    normed and gated before it joins the residual (GatedNorm), dropout on it before that."""
+
     def __init__(self, hidden_size: int, num_heads: int, num_layers: int, dim_feedforward: int, dropout: float,
-                 attention_dropout: float = None):
+                 attention_dropout: float = None, attention_window: Optional[int] = None, attention_sinks: int = 0,
+                 gated_norms: bool = False):
         super().__init__()
+        self.gated_norms = gated_norms
         self.transformer_blocks = nn.ModuleList(
-            [TransformerBlock(hidden_size, num_heads, dim_feedforward, dropout, attention_dropout=attention_dropout)
+            [TransformerBlock(hidden_size, num_heads, dim_feedforward, dropout, attention_dropout=attention_dropout,
+                              attention_window=attention_window, attention_sinks=attention_sinks,
+                              gated_norms=gated_norms)
              for _ in range(num_layers)])
 
     def forward(self, x: torch.Tensor, key_valid: Optional[torch.Tensor], causal: bool) -> torch.Tensor:
         """N pre-LN blocks (transformer_layers.py:100-106, 120-130, 251-258) on the fused kernels:
            h1 = x + drop(O(attn(LN_in(x))));  x' = drop(h1 + drop(W2 drop(GELU(W1 LN_out(h1)))))
         No final LayerNorm after the last block."""
+        return self._run(x, lambda i, att, qkv: att.attend(qkv, key_valid, causal, _p(att.dropout, self.training)))
+
+    def prefill(self, x: torch.Tensor, key_valid: torch.Tensor, caches: WindowCaches) -> torch.Tensor:
+        """forward (causal) over prompts whose valid positions come first, their keys and values laid into `caches`"""
+        def attend(i, att, qkv):
+            B, L, _ = qkv.shape
+            _, k, v = qkv.view(B, L, 3, att.heads, att.d_k).unbind(2)
+            ops.window_cache_fill(*caches.layers[i], k, v, caches.lengths, sinks=att.sinks)
+            return att.attend(qkv, key_valid, True, 0.0)
+
+        caches.lengths.copy_(key_valid.sum(1))
+        caches.most = x.shape[1]
+        return self._run(x, attend)
+
+    def step(self, x: torch.Tensor, caches: WindowCaches) -> torch.Tensor:
+        """one more token of every sequence, (B, d) -> (B, d): what forward gives its position"""
+        def attend(i, att, qkv):
+            q, k, v = qkv.view(qkv.shape[0], 3, att.heads, att.d_k).unbind(1)
+            return ops.window_attention_step(q, k, v, *caches.layers[i], caches.lengths, sinks=att.sinks).view(x.shape)
+
+        out = self._run(x, attend)
+        caches.lengths.add_(1)
+        caches.most += 1
+        return out
+
+    def _run(self, x: torch.Tensor, attend) -> torch.Tensor:
+        """the blocks around attend(block number, attention module, qkv)"""
         blocks = self.transformer_blocks
         if len(blocks) == 0:
             return x
@@ -299,11 +387,18 @@ class TransformerLayer(nn.Module):
         for i, blk in enumerate(blocks):
             att, ff = blk.attention, blk.feed_forward
             qkv = att.qkv(ln)
-            o = ops.attention(qkv, key_valid, att.heads, causal, _p(att.dropout, tr))
+            o = attend(i, att, qkv)
+            nxt = blocks[i + 1].input_sublayer.norm if i + 1 < len(blocks) else None
+            if self.gated_norms:
+                a = ops.linear(o, att.output_linear.weight, att.output_linear.bias)
+                h1, ln2 = blk.input_gate.residual(x, ops.dropout(a, _p(blk.input_sublayer.dropout, tr)),
+                                                  blk.output_sublayer.norm)
+                f2 = ops.ffn(ln2, ff.w_1.weight, ff.w_1.bias, ff.w_2.weight, ff.w_2.bias, _p(ff.dropout, tr))
+                x, ln = blk.output_gate.residual(h1, ops.dropout(f2, _p(blk.output_sublayer.dropout, tr)), nxt)
+                continue
             h1, ln2 = self._projection_residual_norm(o, att.output_linear, x, blk.output_sublayer.norm,
                                                      _p(blk.input_sublayer.dropout, tr))
             f2 = ops.ffn(ln2, ff.w_1.weight, ff.w_1.bias, ff.w_2.weight, ff.w_2.bias, _p(ff.dropout, tr))
-            nxt = blocks[i + 1].input_sublayer.norm if i + 1 < len(blocks) else None
             x, ln = _residual_norm(h1, f2, nxt, _p(blk.output_sublayer.dropout, tr), _p(blk.dropout, tr))
         return x
 

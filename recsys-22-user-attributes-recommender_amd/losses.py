@@ -3,6 +3,8 @@
   SASRecBinaryCrossEntropyLoss       core/losses/sasrec/sas_rec_losses.py:35-75
   SASRecFullSequenceCrossEntropyLoss core/losses/sasrec/sas_rec_losses.py:9-32
   SingleTargetCrossEntropyLoss       core/losses/losses.py:65-115
+
+and, beyond the reference, TopKDistillationLoss: a student's logits against a teacher's best items.
 """
 from __future__ import annotations
 
@@ -20,6 +22,22 @@ class SASRecBinaryCrossEntropyLoss(nn.Module):
     def forward(self, pos_input: torch.Tensor, neg_input: torch.Tensor, mask: torch.Tensor) -> torch.Tensor:
         # torchmetrics reduce(scalar, 'elementwise_mean') is the identity on the scalar mean
         return ops.sasrec_bce(pos_input, neg_input, mask)
+
+
+class TopKDistillationLoss(nn.Module):
+    """temperature^2 KL(teacher || student) over the teacher's own lists of best items (ops.distill_cross_entropy), mean
+    over the rows with a list.  A training module whose `distillation` it is mixes it into the cross-entropy: weight *
+    this + (1 - weight) * cross-entropy, on the lists that a batch carries (modules.TEACHER_IDS_ENTRY_NAME /
+    TEACHER_LOGITS_ENTRY_NAME)."""
+
+    def __init__(self, temperature: float = 1.0, weight: float = 0.5):
+        super().__init__()
+        if not 0.0 <= weight <= 1.0:
+            raise ValueError(f"weight {weight}: expected 0 to 1")
+        self.temperature, self.weight = temperature, weight
+
+    def forward(self, teacher_ids: torch.Tensor, teacher_logits: torch.Tensor, logits: torch.Tensor) -> torch.Tensor:
+        return ops.distill_cross_entropy(logits, teacher_ids, teacher_logits, self.temperature)
 
 
 class SASRecFullSequenceCrossEntropyLoss(nn.Module):

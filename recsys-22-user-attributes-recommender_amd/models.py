@@ -1,5 +1,9 @@
 """SASRec / BERT4Rec / KeBERT4Rec / NARM with the reference constructors and forward contract.
 
+Beyond the reference, the transformer models take attention_window / attention_sinks (attention over a sliding window
+and the first positions -- UBERT4Rec's user token is the first), gated_norms (layers.GatedNorm), and a SASRec with a
+window serves growing sequences one item at a time (SASRecModel.prefill / decode).
+
 Constructor parameter names and defaults equal the reference's, because ASME's GenericModelFactory
 builds models by introspecting `__init__` (core/init/factories/modules/modules.py:116-127):
   SASRecModel      core/models/sasrec/sasrec_model.py:29-116
@@ -79,12 +83,15 @@ class TransformerEncoderModel(SequenceRecommenderModel):
     def __init__(self, transformer_hidden_size: int, num_transformer_heads: int, num_transformer_layers: int,
                  transformer_dropout: float, embedding_layer, sequence_representation_modifier_layer,
                  projection_layer, bidirectional: bool = False, transformer_intermediate_size: int = None,
-                 transformer_attention_dropout: float = None):
+                 transformer_attention_dropout: float = None, attention_window: Optional[int] = None,
+                 attention_sinks: int = 0, gated_norms: bool = False):
         if transformer_intermediate_size is None:
             transformer_intermediate_size = 4 * transformer_hidden_size
         transformer_layer = Ly.TransformerLayer(transformer_hidden_size, num_transformer_heads,
                                                 num_transformer_layers, transformer_intermediate_size,
-                                                transformer_dropout, attention_dropout=transformer_attention_dropout)
+                                                transformer_dropout, attention_dropout=transformer_attention_dropout,
+                                                attention_window=attention_window, attention_sinks=attention_sinks,
+                                                gated_norms=gated_norms)
         rep = Ly.TransformerSequenceRepresentationComponent(transformer_layer, bidirectional=bidirectional)
         super().__init__(embedding_layer, rep, sequence_representation_modifier_layer, projection_layer)
         self.apply(self._init_weights)
@@ -179,7 +186,8 @@ class SASRecModel(TransformerEncoderModel):
                  postfusion_attributes: Dict[str, Dict[str, Any]] = None,
                  additional_attributes_tokenizer: Dict[str, Any] = None, postfusion_merge_function: str = "add",
                  embedding_pooling_type: str = None, transformer_intermediate_size: int = None,
-                 transformer_attention_dropout: float = None, mode: str = "neg_sampling"):
+                 transformer_attention_dropout: float = None, mode: str = "neg_sampling",
+                 attention_window: Optional[int] = None, attention_sinks: int = 0, gated_norms: bool = False):
         self.additional_metadata_keys = list(prefusion_attributes or {}) + list(postfusion_attributes or {})
         emb = Ly.TransformerEmbedding(item_voc_size=item_vocab_size, max_seq_len=max_seq_length,
                                       embedding_size=transformer_hidden_size, dropout=transformer_dropout,
@@ -205,7 +213,8 @@ class SASRecModel(TransformerEncoderModel):
                          bidirectional=False, embedding_layer=element_rep,
                          sequence_representation_modifier_layer=modifier, projection_layer=projection,
                          transformer_intermediate_size=transformer_intermediate_size,
-                         transformer_attention_dropout=transformer_attention_dropout)
+                         transformer_attention_dropout=transformer_attention_dropout,
+                         attention_window=attention_window, attention_sinks=attention_sinks, gated_norms=gated_norms)
         self.apply(self._init_weights)  # the reference initialises twice
 
     def required_metadata_keys(self):
@@ -225,6 +234,46 @@ class SASRecModel(TransformerEncoderModel):
             return last, lin.weight, lin.bias
         return None
 
+    # Serving a growing sequence (attention_window models without attributes): prefill() reads the history once,
+    # decode() takes one more item per user.  Both return the representation (B, d) of each user's last item, which
+    # catalog_query() pairs with the item table; memory per user is sinks + window positions a block, for any history.
+    @torch.no_grad()
+    def prefill(self, sequence):
+        """(representations, layers.WindowCaches) of right-padded histories"""
+        layer = self._servable()
+        mask = sequence.padding_mask if sequence.padding_mask is not None else torch.ones_like(sequence.sequence,
+                                                                                               dtype=torch.bool)
+        emb = self._sequence_embedding_layer(sequence)
+        B, L, _ = emb.shape
+        caches = Ly.WindowCaches(layer.transformer_blocks, B, emb.device)
+        rep = layer.prefill(emb, Ly.key_valid_mask(mask, emb.shape), caches)
+        rows = torch.arange(B, device=rep.device) * L + (caches.lengths - 1).clamp(min=0)
+        return ops.gather_rows(rows, rep.view(B * L, -1)), caches
+
+    @torch.no_grad()
+    def decode(self, items: torch.Tensor, caches) -> torch.Tensor:
+        """the representation (B, d) of one more item (B,) per user; `caches` go on to it"""
+        layer = self._servable()
+        if items.shape != caches.lengths.shape:
+            raise ValueError(f"items {tuple(items.shape)}: expected one for each of {caches.lengths.shape[0]} users")
+        emb, ln2 = self._sequence_embedding_layer.item_embedding_layer, self._sequence_embedding_layer.norm_embedding
+        pos, ln1, eps1 = emb.fused_args()
+        if pos is not None and caches.most >= pos.shape[0]:
+            raise IndexError(f"position {caches.most} exceeds max_seq_len {pos.shape[0]}")
+        B = items.shape[0]
+        spec = ops.EmbeddingSpec(seq_len=B, ln1_eps=eps1, ln2_eps=ln2.eps)  # (row b of the B position rows for token b)
+        x = ops.embedding(items.view(1, B), emb.get_item_embedding_weight(),
+                          None if pos is None else ops.gather_rows(caches.lengths, pos), ln1, None,
+                          (ln2.weight, ln2.bias), spec)
+        return layer.step(x.view(B, -1), caches)
+
+    def _servable(self):
+        if self.training:
+            raise RuntimeError("prefill / decode serve a model in eval mode")
+        if self.additional_metadata_keys:
+            raise NotImplementedError("prefill / decode take no attributes")
+        return self._sequence_representation_layer.transformer_layer
+
     def item_table(self):
         return self._sequence_embedding_layer.item_embedding_layer.get_item_embedding_weight()
 
@@ -237,7 +286,8 @@ class BERT4RecModel(TransformerEncoderModel):
                  item_vocab_size: int, max_seq_length: int, transformer_dropout: float,
                  project_layer_type: str = "transpose_embedding", embedding_pooling_type: str = None,
                  initializer_range: float = 0.02, transformer_intermediate_size: int = None,
-                 transformer_attention_dropout: float = None):
+                 transformer_attention_dropout: float = None, attention_window: Optional[int] = None,
+                 attention_sinks: int = 0, gated_norms: bool = False):
         modifier = Ly.FFNSequenceRepresentationModifierComponent(transformer_hidden_size)
         # The reference passes embedding_pooling_type POSITIONALLY into TransformerEmbedding's 5th
         # parameter, `positional_embedding` (bert4rec_model.py:40-41 vs transformer_layers.py:21-28): with
@@ -251,7 +301,8 @@ class BERT4RecModel(TransformerEncoderModel):
                          bidirectional=True, embedding_layer=emb,
                          projection_layer=projection, sequence_representation_modifier_layer=modifier,
                          transformer_intermediate_size=transformer_intermediate_size,
-                         transformer_attention_dropout=transformer_attention_dropout)
+                         transformer_attention_dropout=transformer_attention_dropout,
+                         attention_window=attention_window, attention_sinks=attention_sinks, gated_norms=gated_norms)
         self.apply(functools.partial(normal_initialize_weights, initializer_range=initializer_range))
 
     def item_table(self):
@@ -269,7 +320,8 @@ class KeBERT4RecModel(TransformerEncoderModel):
                  additional_attributes_tokenizer: Dict[str, Any] = None, postfusion_merge_function: str = "add",
                  positional_embedding: bool = True, embedding_pooling_type: str = None,
                  initializer_range: float = 0.02, transformer_intermediate_size: Optional[int] = None,
-                 transformer_attention_dropout: Optional[float] = None):
+                 transformer_attention_dropout: Optional[float] = None, attention_window: Optional[int] = None,
+                 attention_sinks: int = 0, gated_norms: bool = False):
         self.additional_metadata_keys = list(prefusion_attributes or {}) + list(postfusion_attributes or {})
         emb = Ly.TransformerEmbedding(item_vocab_size, max_seq_length, transformer_hidden_size, 0.0,
                                       positional_embedding=positional_embedding,
@@ -290,7 +342,8 @@ class KeBERT4RecModel(TransformerEncoderModel):
                          embedding_layer=element_rep, sequence_representation_modifier_layer=modifier,
                          projection_layer=projection, bidirectional=True,
                          transformer_intermediate_size=transformer_intermediate_size,
-                         transformer_attention_dropout=transformer_attention_dropout)
+                         transformer_attention_dropout=transformer_attention_dropout,
+                         attention_window=attention_window, attention_sinks=attention_sinks, gated_norms=gated_norms)
         self.apply(functools.partial(normal_initialize_weights, initializer_range=initializer_range))
 
     def required_metadata_keys(self):
@@ -390,7 +443,8 @@ class UserTransformerSequenceRepresentationComponent(nn.Module):
     def __init__(self, transformer_hidden_size: int, num_transformer_heads: int, num_transformer_layers: int,
                  transformer_dropout: float, user_attributes: Optional[Dict[str, Dict[str, Any]]], bidirectional: bool,
                  transformer_attention_dropout: Optional[float] = None,
-                 transformer_intermediate_size: Optional[int] = None, replace_first_item: bool = False):
+                 transformer_intermediate_size: Optional[int] = None, replace_first_item: bool = False,
+                 attention_window: Optional[int] = None, attention_sinks: int = 0, gated_norms: bool = False):
         super().__init__()
         self.user_attributes = user_attributes
         self.bidirectional = bidirectional
@@ -400,7 +454,9 @@ class UserTransformerSequenceRepresentationComponent(nn.Module):
         self.transformer_encoder = Ly.TransformerLayer(transformer_hidden_size, num_transformer_heads,
                                                        num_transformer_layers, transformer_intermediate_size,
                                                        transformer_dropout,
-                                                       attention_dropout=transformer_attention_dropout)
+                                                       attention_dropout=transformer_attention_dropout,
+                                                       attention_window=attention_window,
+                                                       attention_sinks=attention_sinks, gated_norms=gated_norms)
 
     def forward(self, embedded: torch.Tensor, padding_mask: Optional[torch.Tensor]) -> torch.Tensor:
         if padding_mask is not None and self.user_attributes and not self.replace_first_item:
@@ -420,7 +476,8 @@ class UBERT4RecModel(TransformerEncoderModel):
                  user_attributes: Dict[str, Dict[str, Any]], positional_embedding: bool, segment_embedding: bool,
                  embedding_pooling_type: str = None, initializer_range: float = 0.02,
                  transformer_intermediate_size: Optional[int] = None,
-                 transformer_attention_dropout: Optional[float] = None):
+                 transformer_attention_dropout: Optional[float] = None, attention_window: Optional[int] = None,
+                 attention_sinks: int = 0, gated_norms: bool = False):
         self.additional_userdata_keys = []
         self.additional_metadata_keys = []
         if user_attributes is not None:
@@ -447,7 +504,8 @@ class UBERT4RecModel(TransformerEncoderModel):
         self._sequence_representation_layer = UserTransformerSequenceRepresentationComponent(
             transformer_hidden_size, num_transformer_heads, num_transformer_layers, transformer_dropout,
             user_attributes, bidirectional=False, transformer_attention_dropout=transformer_attention_dropout,
-            transformer_intermediate_size=transformer_intermediate_size)
+            transformer_intermediate_size=transformer_intermediate_size, attention_window=attention_window,
+            attention_sinks=attention_sinks, gated_norms=gated_norms)
         self.apply(functools.partial(normal_initialize_weights, initializer_range=initializer_range))
 
     def required_metadata_keys(self):

@@ -35,6 +35,9 @@ ITEM_SEQ_ENTRY_NAME = "item"
 TARGET_ENTRY_NAME = "item.target"
 POSITIVE_SAMPLES_ENTRY_NAME = "positive_samples"
 NEGATIVE_SAMPLES_ENTRY_NAME = "negative_samples"
+# a teacher's best items for every position of the batch, (B, L, k) ids and logits (losses.TopKDistillationLoss)
+TEACHER_IDS_ENTRY_NAME = "teacher.ids"
+TEACHER_LOGITS_ENTRY_NAME = "teacher.logits"
 LOG_KEY_TRAINING_LOSS = "train_loss"
 LOG_KEY_VALIDATION_LOSS = "val_loss"
 LOG_KEY_TEST_LOSS = "test_loss"
@@ -306,6 +309,22 @@ def _rows_cross_entropy(model, sequence, rows, targets, pad: int, inverse=None) 
     return ops.cross_entropy(model.forward_rows(sequence, rows, inverse), targets, pad)
 
 
+def _rows_distillation(model, sequence, batch, rows, targets, pad: int, loss, inverse=None) -> torch.Tensor:
+    """_rows_cross_entropy mixed with `loss` (losses.TopKDistillationLoss) over the same rows' teacher lists, both on
+    logits that are formed once"""
+    if TEACHER_IDS_ENTRY_NAME not in batch or TEACHER_LOGITS_ENTRY_NAME not in batch:
+        raise Exception(f"The batch does not contain {TEACHER_IDS_ENTRY_NAME} and {TEACHER_LOGITS_ENTRY_NAME}. "
+                        f"Found the following batch entries: {', '.join(batch.keys())}")
+    for k in (TEACHER_IDS_ENTRY_NAME, TEACHER_LOGITS_ENTRY_NAME):
+        if batch[k].shape[:-1] != batch[TARGET_ENTRY_NAME].shape:
+            raise ValueError(f"{k} {tuple(batch[k].shape)}: expected a list for each of the targets "
+                             f"{tuple(batch[TARGET_ENTRY_NAME].shape)}")
+    lists = [batch[k].reshape(-1, batch[k].shape[-1]).index_select(0, rows)
+             for k in (TEACHER_IDS_ENTRY_NAME, TEACHER_LOGITS_ENTRY_NAME)]
+    logits = model.forward_rows(sequence, rows, inverse)
+    return loss.weight * loss(*lists, logits) + (1.0 - loss.weight) * ops.cross_entropy(logits, targets, pad)
+
+
 def _single_target_cross_entropy(model, sequence, targets, pad: int) -> torch.Tensor:
     """SingleTargetCrossEntropyLoss(context . W^T) for a bilinear head (NARM, losses.py:77-115 + narm/layers.py:
     93-120): the fused logits + cross-entropy kernels where the width fits them, else logits on the Linear kernel
@@ -328,6 +347,8 @@ class NextItemPredictionTrainingModule(_TableGradMixin, _Base):
         self.item_tokenizer = item_tokenizer
         self.metrics = metrics
         self.loss_function = _instantiate_loss(loss_function, item_tokenizer)
+        # set to a losses.TopKDistillationLoss: per-step targets are trained on it and the cross-entropy together
+        self.distillation = None
         self._init_table_grad(table_grad)
 
     def forward(self, batch, batch_idx: Optional[int] = None) -> torch.Tensor:
@@ -342,8 +363,12 @@ class NextItemPredictionTrainingModule(_TableGradMixin, _Base):
         if ce_loss and target.dim() == 2 and hasattr(self.model, "forward_rows"):
             # per-step targets: only the non-pad positions contribute to the CE
             rows = torch.nonzero(target.reshape(-1) != pad).squeeze(1)
-            loss = _rows_cross_entropy(self.model, build_model_input(self.model, self.item_tokenizer, batch), rows,
-                                       target.reshape(-1).index_select(0, rows), pad)
+            sequence, row_targets = (build_model_input(self.model, self.item_tokenizer, batch),
+                                     target.reshape(-1).index_select(0, rows))
+            loss = (_rows_cross_entropy(self.model, sequence, rows, row_targets, pad) if self.distillation is None else
+                    _rows_distillation(self.model, sequence, batch, rows, row_targets, pad, self.distillation))
+        elif self.distillation is not None:
+            raise NotImplementedError("distillation needs a target and a teacher's list for every position")
         elif ce_loss and target.dim() == 1 and hasattr(self.model, "context_and_head"):
             loss = _single_target_cross_entropy(self.model, build_model_input(self.model, self.item_tokenizer, batch),
                                                 target, pad)
@@ -396,6 +421,8 @@ class MaskedTrainingModule(_TableGradMixin, _Base):
         self.learning_rate, self.beta_1, self.beta_2 = learning_rate, beta_1, beta_2
         self.weight_decay = weight_decay  # accepted but unused by the optimizer, as in the reference (Q7)
         self.num_warmup_steps = num_warmup_steps
+        # set to a losses.TopKDistillationLoss: the masked positions are trained on it and the cross-entropy together
+        self.distillation = None
         self.item_tokenizer = item_tokenizer
         self.metrics = metrics
         # fused_eval: rank each masked position's target with asme_catalog_rank from its hidden state and the head
@@ -426,8 +453,9 @@ class MaskedTrainingModule(_TableGradMixin, _Base):
         else:
             rows = torch.nonzero(target.reshape(-1) != pad).squeeze(1)  # (reads the row count on the host)
             row_targets, inverse = target.reshape(-1).index_select(0, rows), None
-        loss = _rows_cross_entropy(self.model, build_model_input(self.model, self.item_tokenizer, batch), rows,
-                                   row_targets, pad, inverse)
+        sequence = build_model_input(self.model, self.item_tokenizer, batch)
+        loss = (_rows_cross_entropy(self.model, sequence, rows, row_targets, pad, inverse) if self.distillation is None
+                else _rows_distillation(self.model, sequence, batch, rows, row_targets, pad, self.distillation, inverse))
         self.log(LOG_KEY_TRAINING_LOSS, loss, prog_bar=False)
         return {"loss": loss}
 
@@ -553,6 +581,10 @@ class UBERTMaskedTrainingModule(MaskedTrainingModule):
         if target.dim() > 2:
             raise NotImplementedError("basket (multi-target) masked training is outside the MI355X hot path")
         batch[TARGET_ENTRY_NAME] = self._with_user_column(target, self.item_tokenizer.pad_token_id)
+        if self.distillation is not None and self.user_key_len:  # (the user token has no list)
+            for k, absent in ((TEACHER_IDS_ENTRY_NAME, -1), (TEACHER_LOGITS_ENTRY_NAME, 0.0)):
+                if k in batch:
+                    batch[k] = F.pad(batch[k], (0, 0, 1, 0), value=absent)
         return super().training_step(batch, batch_idx)
 
     def _get_prediction_for_masked_item(self, batch, batch_idx=None) -> torch.Tensor:

@@ -402,3 +402,97 @@ def test_window_attention(asme, dev, dtype, b, n, h, kv, d, window, sinks, causa
                                     valid=valid.cuda() if padding else None)
     got = [out, *torch.autograd.grad(out, (q, k, v), dout)]
     check_window(got, dtype, q, k, v, dout, window, sinks, causal, valid, d ** -0.5, n)
+
+
+# ------------------------------------------------------------------------------------------------ streams and graphs
+def history_call(asme, kind, dtype, seed):
+    """(inputs to be refilled, a call of them that returns everything it computes)"""
+    ops = asme.ops
+    if kind == "attention":
+        q, k, v, dout = (rand(2, 150, x, 32, seed=seed + i, dtype=dtype) for i, x in enumerate((4, 2, 2, 4)))
+        valid = (torch.arange(150) < torch.tensor([[150], [70]])).cuda()
+        for t in (q, k, v):
+            t.requires_grad_()
+
+        def call():
+            out = ops.window_attention(q, k, v, 20, sinks=3, valid=valid)
+            return [out, *torch.autograd.grad(out, (q, k, v), dout)]
+        return [q, k, v, dout], call
+    if kind == "step":
+        q, k, v = rand(3, 4, 32, seed=seed, dtype=dtype), rand(3, 2, 32, seed=seed + 1, dtype=dtype), rand(3, 2, 32, seed=seed + 2, dtype=dtype)
+        ck, cv = rand(3, 2, 600, 32, seed=seed + 3, dtype=dtype), rand(3, 2, 600, 32, seed=seed + 4, dtype=dtype)
+        n = torch.tensor([5, 700, 1300]).cuda()
+
+        def call():
+            return [ops.window_attention_step(q, k, v, ck, cv, n, sinks=2), ck.clone(), cv.clone()]
+        return [q, k, v, ck, cv], call
+    if kind == "distill":
+        x = rand(20, 5003, seed=seed, dtype=dtype).requires_grad_()
+        ids, t = distill_lists(20, 5003, 9, 3)
+
+        def call():
+            loss = ops.distill_cross_entropy(x, ids, t, 2.0)
+            return [loss, *torch.autograd.grad(loss, x)]
+        return [x], call
+    res, y, gate = rand(3, 40, 72, seed=seed, dtype=dtype), rand(3, 40, 72, seed=seed + 1, dtype=dtype), rand(3, 1, 72, seed=seed + 2, dtype=dtype)
+    w, b = 1 + rand(72, seed=5, scale=0.1), rand(72, seed=6, scale=0.1)
+    ds = rand(3, 40, 72, seed=seed + 3, dtype=dtype)
+    leaves = [t.requires_grad_() for t in (res, y, gate, w, b)]
+
+    def call():
+        s, z = ops.gated_residual_norm(res, y, w, b, w, b, gate=gate)
+        return [s, z, *torch.autograd.grad((s, z), leaves, (ds, ds))]
+    return [res, y, gate, ds], call
+
+
+KINDS = ["attention", "step", "distill", "norm"]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("kind", KINDS)
+def test_captured_and_replayed(asme, dev, kind, dtype):
+    """two graphs of one call on other inputs, replayed in turn with eager calls in between: each replay gives what an
+    eager call gives (the same kernels in the same order: the same bits)"""
+    (in1, call1), (in2, call2) = history_call(asme, kind, dtype, 10), history_call(asme, kind, dtype, 50)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            call1(), call2()
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = []
+    for call in (call1, call2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = call()
+        graphs.append((g, out))
+    for turn in range(4):
+        for (g, out), ins, call in zip(graphs, (in1, in2), (call1, call2)):
+            with torch.no_grad():
+                for i, t in enumerate(ins):
+                    t.copy_(rand(*t.shape, seed=100 * turn + i, dtype=dtype))
+            g.replay()
+            torch.cuda.synchronize()
+            got = [t.detach().clone() for t in out]
+            with torch.no_grad():
+                for i, t in enumerate(ins):
+                    t.copy_(rand(*t.shape, seed=100 * turn + i, dtype=dtype))
+            for a, b in zip(got, call()):
+                assert torch.equal(a, b), (kind, turn)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_on_another_stream_and_in_any_order(asme, dev, kind):
+    """calls in flight on two streams at once, and again one after the other: the same bits"""
+    (_, call1), (_, call2) = history_call(asme, kind, torch.float32, 10), history_call(asme, kind, torch.float32, 50)
+    want = [t.detach().clone() for t in call1()], [t.detach().clone() for t in call2()]
+    side = torch.cuda.Stream()
+    for _ in range(5):
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            b = call2()
+        a = call1()
+        torch.cuda.current_stream().wait_stream(side)
+        for got, ref in zip((a, b), want):
+            assert all(torch.equal(x, y) for x, y in zip(got, ref))
+        torch.cuda.synchronize()
