@@ -462,17 +462,28 @@ int asme_ws_linear_residual_ln(const float* X, int64_t M, int64_t K, const float
 
 /* Distillation (csrc/distill.hip), next to asme_cross_entropy_*: the KL divergence of softmax(logits / temperature) over
  * the catalogue from softmax(teacher / temperature) over row r's list ids[r][0..top) (entries outside [0, V) are absent;
- * an item twice on a list counts twice), times temperature^2, mean over the rows whose list is not empty (NaN if none).
+ * an item twice on a list counts twice), times weight * temperature^2, mean over the rows whose list is not empty (NaN
+ * if none).
  * logits (n, V) rows ld apart; ids, teacher (n, top), top <= 1024.  out[0] = loss, out[1] = rows with a list; state
  * (n, 2) and prob (n, top) are for the backward.  Workspace: bytes from the *_workspace query. */
 int64_t asme_distill_xent_workspace(int64_t n, int64_t V);
 int asme_distill_xent_fwd(const void* logits, int64_t ld, int64_t n, int64_t V, const int64_t* ids,
-                          const float* teacher, int64_t top, float temperature, int dtype, float* state, float* prob,
-                          void* workspace, int64_t ws_bytes, float* out, void* stream);
+                          const float* teacher, int64_t top, float temperature, float weight, int dtype, float* state,
+                          float* prob, void* workspace, int64_t ws_bytes, float* out, void* stream);
+/* The forward with the gradient of the mean written as well, 2 n V elements moved in all (n >= 512 rows that a workgroup
+ * holds, 4096 to 32768 fp32 or 65536 bf16 items: *_grad_supported): dlogits (n, V) contiguous, rows aligned like those of
+ * logits.  What is left of the backward is the upstream factor: asme_scale_by(dlogits, n * V, dtype, dloss). */
+int asme_distill_xent_grad_supported(int64_t n, int64_t V, int dtype);
+int64_t asme_distill_xent_grad_workspace(int64_t n);
+int asme_distill_xent_fwd_grad(const void* logits, int64_t ld, int64_t n, int64_t V, const int64_t* ids,
+                               const float* teacher, int64_t top, float temperature, float weight, int dtype,
+                               float* state, float* prob, void* dlogits, void* workspace, int64_t ws_bytes, float* out, void* stream);
+/* x[i] *= factor[0], i < n (x 16-byte aligned); returns at once on the device where the factor is 1 */
+int asme_scale_by(void* x, int64_t n, int dtype, const float* factor, void* stream);
 /* dlogits (rows ld_d apart; not logits itself) = dloss[0] times the gradient; rows without a list: 0.  stats = the
  * forward's out. */
 int asme_distill_xent_bwd(const void* logits, int64_t ld, int64_t n, int64_t V, const int64_t* ids, int64_t top,
-                          float temperature, int dtype, const float* state, const float* prob, const float* stats,
+                          float temperature, float weight, int dtype, const float* state, const float* prob, const float* stats,
                           const float* dloss, void* dlogits, int64_t ld_d, void* stream);
 
 /* Gated residual between two norms (csrc/gatednorm.hip), next to asme_residual_ln_*:

@@ -124,8 +124,12 @@ SIGNATURES = {
     "asme_cloze_mask": [p, p, i64, i64, i64, i64, i64, f64, f64, p, p, u64, p, p, p],
     "asme_padding_mask": [p, i64, i64, p, p],
     "asme_distill_xent_workspace": [i64, i64],
-    "asme_distill_xent_fwd": [p, i64, i64, i64, p, p, i64, f32, i32, p, p, p, i64, p, p],
-    "asme_distill_xent_bwd": [p, i64, i64, i64, p, i64, f32, i32, p, p, p, p, p, i64, p],
+    "asme_distill_xent_fwd": [p, i64, i64, i64, p, p, i64, f32, f32, i32, p, p, p, i64, p, p],
+    "asme_distill_xent_grad_supported": [i64, i64, i32],
+    "asme_distill_xent_grad_workspace": [i64],
+    "asme_distill_xent_fwd_grad": [p, i64, i64, i64, p, p, i64, f32, f32, i32, p, p, p, p, i64, p, p],
+    "asme_scale_by": [p, i64, i32, p, p],
+    "asme_distill_xent_bwd": [p, i64, i64, i64, p, i64, f32, f32, i32, p, p, p, p, p, i64, p],
     "asme_gated_residual_norm_fwd": [p, p, p, i64, p, p, p, p, i64, i64, f32, f32, i32, i32, p, p, p, p],
     "asme_gated_residual_norm_bwd_workspace": [i64, i64, i64],
     "asme_gated_residual_norm_bwd": [p, p, p, i64, p, p, p, i64, i64, f32, i32, i32, p, p, p, p, p, p, p, p, i64, p],
@@ -146,7 +150,7 @@ _RESTYPES = {"asme_mi_last_error": ctypes.c_char_p, "asme_dedup_workspace_bytes"
              "asme_linear_xent_fwd_dh_workspace": ctypes.c_int64, "asme_linear_xent_bwd_dw_workspace": ctypes.c_int64, "asme_logits_workspace": ctypes.c_int64, "asme_bucket_by_owner_workspace": ctypes.c_int64, "asme_occurrence_csr_workspace": ctypes.c_int64,
              "asme_table_grad_workspace": ctypes.c_int64, "asme_catalog_planes_bytes": ctypes.c_int64,
              "asme_catalog_x6_workspace": ctypes.c_int64,
-             "asme_distill_xent_workspace": ctypes.c_int64,
+             "asme_distill_xent_workspace": ctypes.c_int64, "asme_distill_xent_grad_workspace": ctypes.c_int64,
              "asme_gated_residual_norm_bwd_workspace": ctypes.c_int64,
              "asme_window_attention_bwd_workspace": ctypes.c_int64,
              "asme_window_step_workspace": ctypes.c_int64}

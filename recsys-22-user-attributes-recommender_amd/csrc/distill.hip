@@ -3,11 +3,17 @@
 //
 //   list of row r: the entries j with 0 <= ids[r][j] < V;  p = softmax over the list of t[r][j] / tau
 //   q = softmax over the catalogue of s[r][v] / tau
-//   loss = mean over the rows with a list of  tau^2 sum_j p_j (log p_j - log q_{id_j})
-//   dL/ds[r][v] = tau / rows with a list * (q_v - sum_{j: id_j = v} p_j)
+//   loss = w * mean over the rows with a list of  tau^2 sum_j p_j (log p_j - log q_{id_j})
+//   dL/ds[r][v] = w tau / rows with a list * (q_v - sum_{j: id_j = v} p_j)
 //
-// One pass over the logits forward (running maximum and sum in base-2 exponentials) and one read and one write backward:
-// memory bound, 3 n V elements for the 2 n V that any schedule has to move.  Rows are split over workgroups when there
+// Two schedules, both memory bound.
+//   apart: one pass over the logits forward (running maximum and sum in base-2 exponentials), one read and one write
+//   backward: 3 n V elements, for any row.
+//   together (asme_distill_xent_fwd_grad): a workgroup holds its row in registers, so that the forward writes the gradient
+//   of the mean as well: the 2 n V elements that any schedule has to move.  The backward has the upstream factor left to
+//   apply, which costs nothing where it is 1 and 2 n V more where it is not: a loss that is one part of another takes its
+//   weight w here.
+// Rows are split over workgroups when there
 // are fewer rows than the chip needs workgroups; the splits' (maximum, sum) pairs are merged in a fixed order, so results
 // do not depend on the schedule.  Statistics, probabilities and the loss are fp32; the gradient is rounded once, on store.
 #include "elem.h"
@@ -200,6 +206,170 @@ __global__ __launch_bounds__(1024) void mean_kernel(const float* __restrict__ su
     }
 }
 
+// One wave per row: p (n x top), and the workgroup's number of rows with a list
+__global__ __launch_bounds__(1024) void teacher_kernel(const int64_t* __restrict__ ids, const float* __restrict__ teacher,
+                                                       int64_t n, int64_t V, int top, float inv_tau,
+                                                       float* __restrict__ prob, float* __restrict__ counts) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t row = (int64_t)blockIdx.x * 16 + wave;
+    bool there = false;
+    if (row < n) {
+        const int64_t* id = ids + row * top;
+        const float* t = teacher + row * top;
+        float tm = -INFINITY, ts = 0.f;
+        for (int j = lane; j < top; j += 64)
+            if ((uint64_t)id[j] < (uint64_t)V) tm = fmaxf(tm, t[j]);
+        tm = wave_max(tm);
+        there = !(tm == -INFINITY);
+        for (int j = lane; j < top; j += 64)
+            if (there && (uint64_t)id[j] < (uint64_t)V) ts += expf((t[j] - tm) * inv_tau);
+        const float log_ts = logf(wave_sum(ts));
+        for (int j = lane; j < top; j += 64)
+            prob[row * top + j] = there && (uint64_t)id[j] < (uint64_t)V ? expf((t[j] - tm) * inv_tau - log_ts) : 0.f;
+    }
+    __shared__ float w[16];
+    if (lane == 0) w[wave] = there ? 1.f : 0.f;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        float c = 0.f;
+        for (int k = 0; k < 16; ++k) c += w[k];
+        counts[2 * blockIdx.x] = 0.f;
+        counts[2 * blockIdx.x + 1] = c;
+    }
+}
+
+constexpr int kRowThreads = 512, kMostVecs = 16;  // 16-byte vectors a thread: rows to 32 K fp32 or 64 K bf16 items
+
+// A whole row per workgroup: its state, its loss and the gradient of the mean (stats[1]: the rows with a list).  Two
+// or three workgroups a CU, so that one's loads are on their way while another reduces.
+template <class T, int kRowVecs>
+__global__ __launch_bounds__(kRowThreads, kRowVecs == kMostVecs ? 4 : 6) void fused_kernel(const T* __restrict__ logits, int64_t ld, int V,
+                                                               const int64_t* __restrict__ ids, int top, float scale,
+                                                               float tau2, float tau1, const float* __restrict__ prob,
+                                                               const float* __restrict__ stats,
+                                                               float2* __restrict__ state, float* __restrict__ sums,
+                                                               T* __restrict__ dlogits, int64_t ld_d) {
+    constexpr int E = Elem<T>::V;
+    typedef T Vec __attribute__((ext_vector_type(E)));
+    __shared__ int list[kMaxTop];
+    __shared__ float lp[kMaxTop];
+    __shared__ float red[2][kRowThreads / 64];
+    const int64_t row = blockIdx.x;
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    const T* p = logits + row * ld;
+    T* d = dlogits + row * ld_d;
+    // whole vectors, and the elements before and behind them: fewer than 16, one a thread
+    const int head = (int)(((16 - ((uintptr_t)p & 15)) & 15) / sizeof(T)), vecs = (V - head) / E, tail = head + vecs * E;
+    const int edge = t < head ? t : tail + t - head;
+    const bool has_edge = t < head + V - tail;
+    // (a thread's vectors: t, t + 512, ...; behind the row its last one again)
+    Vec raw[kRowVecs];
+#pragma unroll
+    for (int u = 0; u < kRowVecs; ++u)
+        raw[u] = reinterpret_cast<const Vec*>(p + head)[(unsigned)min(t + u * kRowThreads, vecs - 1)];
+    const float ex = has_edge ? Elem<T>::get(p + edge) : -INFINITY;
+    float listed = 0.f;
+    for (int j = t; j < top; j += kRowThreads) {
+        const int64_t v = ids[row * top + j];
+        list[j] = (uint64_t)v < (uint64_t)V ? (int)v : -1;
+        lp[j] = prob[row * top + j];
+        listed += lp[j];
+    }
+    // the row stays as it is stored: without this the compiler keeps a bf16 row's values as floats from one pass over it to
+    // the next, twice the registers
+    auto stored = [&]() {
+#pragma unroll
+        for (int u = 0; u < kRowVecs; ++u) {
+            floatx4 v = __builtin_bit_cast(floatx4, raw[u]);
+            asm volatile("" : "+v"(v));
+            raw[u] = __builtin_bit_cast(Vec, v);
+        }
+    };
+    float m = ex;  // (a vector seen twice does not change the maximum)
+#pragma unroll
+    for (int u = 0; u < kRowVecs; ++u)
+#pragma unroll
+        for (int e = 0; e < E; ++e) m = fmaxf(m, (float)raw[u][e]);
+    m = wave_max(m);
+    listed = wave_sum(listed);
+    if (lane == 0) red[0][wave] = m, red[1][wave] = listed;
+    __syncthreads();
+    m = red[0][0], listed = red[1][0];
+    for (int k = 1; k < kRowThreads / 64; ++k) m = fmaxf(m, red[0][k]), listed += red[1][k];
+    m *= scale;
+    const bool there = listed != 0.f;  // a list's p sum to 1; no list, no p (a NaN goes on)
+    const float base = m == -INFINITY ? 0.f : m;
+    float s = __builtin_amdgcn_exp2f(fmaf(ex, scale, -base));
+    stored();
+#pragma unroll
+    for (int u = 0; u < kRowVecs; ++u) {
+        float part = 0.f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) part += __builtin_amdgcn_exp2f(fmaf((float)raw[u][e], scale, -base));
+        s += t + u * kRowThreads < vecs ? part : 0.f;
+    }
+    s = wave_sum(s);
+    __syncthreads();
+    if (lane == 0) red[0][wave] = s;
+    __syncthreads();
+    s = red[0][0];
+    for (int k = 1; k < kRowThreads / 64; ++k) s += red[0][k];
+    const float inv = there ? 1.f / s : 0.f, g = there ? tau1 / stats[1] : 0.f, log_s = logf(s);
+    auto q = [&](float x) { return there ? __builtin_amdgcn_exp2f(fmaf(x, scale, -base)) * inv : 0.f; };
+    stored();
+#pragma unroll
+    for (int u = 0; u < kRowVecs; ++u)
+        if (t + u * kRowThreads < vecs) {
+            Vec o;
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] = (T)(g * q((float)raw[u][e]));
+            reinterpret_cast<Vec*>(d + head)[(unsigned)(t + u * kRowThreads)] = o;
+        }
+    if (has_edge) Elem<T>::put(d + edge, g * q(ex));
+    __syncthreads();  // the list's entries are stored after the row
+    float kl = 0.f;
+    for (int j = t; j < top; j += kRowThreads) {
+        const int v = list[j];
+        if (v < 0 || !there) continue;
+        const float x = Elem<T>::get(p + v);
+        if (!(lp[j] == 0.f)) kl += lp[j] * (logf(lp[j]) - (fmaf(x, scale, -base) * kLn2 - log_s));
+        float sum = 0.f;
+        bool first = true;
+        for (int k = 0; k < top; ++k) {
+            const bool same = list[k] == v;
+            first = first && !(same && k < j);
+            sum += same ? lp[k] : 0.f;
+        }
+        if (first) Elem<T>::put(d + v, g * (q(x) - sum));
+    }
+    kl = wave_sum(kl);
+    if (lane == 0) red[1][wave] = kl;  // (last read before the barrier above)
+    __syncthreads();
+    if (t == 0) {
+        for (int k = 1; k < kRowThreads / 64; ++k) kl += red[1][k];
+        state[row] = make_float2(there ? base : 0.f, inv);
+        sums[2 * row] = there ? kl * tau2 : 0.f;
+        sums[2 * row + 1] = there ? 1.f : 0.f;
+    }
+}
+
+// x *= f[0], nothing where that is 1
+template <class T>
+__global__ __launch_bounds__(kThreads) void scale_kernel(T* __restrict__ x, int64_t n, const float* __restrict__ f) {
+    constexpr int E = Elem<T>::V;
+    const float g = f[0];
+    if (g == 1.f) return;
+    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < n / E; i += (int64_t)gridDim.x * kThreads) {
+        float v[E];
+        Elem<T>::load(x + i * E, v);
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[e] *= g;
+        Elem<T>::store(x + i * E, v);
+    }
+    const int64_t j = n / E * E + threadIdx.x;
+    if (blockIdx.x == 0 && j < n) Elem<T>::put(x + j, Elem<T>::get(x + j) * g);
+}
+
 // dlogits of a row segment: g (q - 0) everywhere, then the list's entries of the segment once more with their p taken
 // off.  An item that is on the list twice is written by its first entry, with the sum of its p in list order.
 template <class T>
@@ -276,6 +446,12 @@ __global__ __launch_bounds__(kThreads) void grad_kernel(const T* __restrict__ lo
 constexpr int64_t kOneGroupRows = 256;  // up to here one workgroup finishes the rows and their mean
 int64_t finish_groups(int64_t n) { return n <= kOneGroupRows ? 1 : (n + 15) / 16; }
 
+// the rows that a workgroup holds, where there are enough of them to fill the chip (two workgroups a CU; 424 us for 8192 x 26747 fp32 at 1024 threads of 64 registers, which
+// spilled, 355 at 512 of 128)
+bool together(int64_t n, int64_t V, int dtype) {
+    return n >= 512 && V >= 4096 && V <= (int64_t)kRowThreads * kMostVecs * (dtype == kF32 ? 4 : 8);
+}
+
 bool shape_ok(int64_t n, int64_t V, int64_t top) {
     return n >= 0 && n < (1ll << 24) && V >= 1 && V < (1ll << 31) && top >= 1 && top <= kMaxTop;
 }
@@ -288,12 +464,13 @@ ASME_API int64_t asme_distill_xent_workspace(int64_t n, int64_t V) {
 }
 
 ASME_API int asme_distill_xent_fwd(const void* logits, int64_t ld, int64_t n, int64_t V, const int64_t* ids,
-                                   const float* teacher, int64_t top, float temperature, int dtype, float* state,
-                                   float* prob, void* workspace, int64_t ws_bytes, float* out, void* stream) {
+                                   const float* teacher, int64_t top, float temperature, float weight, int dtype,
+                                   float* state, float* prob, void* workspace, int64_t ws_bytes, float* out, void* stream) {
     ASME_CHECK_ARG(logits && ids && teacher && state && prob && workspace && out, "asme_distill_xent_fwd: null pointer");
     ASME_CHECK_ARG(dtype_ok(dtype), "asme_distill_xent_fwd: dtype is 0 (fp32) or 1 (bf16)");
     ASME_CHECK_ARG(n >= 1 && shape_ok(n, V, top) && ld >= V, "asme_distill_xent_fwd: bad size");
-    ASME_CHECK_ARG(temperature > 0.f && temperature < INFINITY, "asme_distill_xent_fwd: temperature > 0");
+    ASME_CHECK_ARG(temperature > 0.f && temperature < INFINITY && weight - weight == 0.f,
+                   "asme_distill_xent_fwd: temperature > 0, a finite weight");
     ASME_CHECK_ARG(ws_bytes >= asme_distill_xent_workspace(n, V), "asme_distill_xent_fwd: workspace too small");
     hipStream_t s = (hipStream_t)stream;
     const int splits = row_splits(n, V);
@@ -305,7 +482,7 @@ ASME_API int asme_distill_xent_fwd(const void* logits, int64_t ld, int64_t n, in
         hipLaunchKernelGGL(stats_kernel<T>, dim3((unsigned)(n * splits)), dim3(kThreads), 0, s, (const T*)logits, ld, V,
                            splits, split_len(V, splits), kLog2e / temperature, part);
         hipLaunchKernelGGL(rows_kernel<T>, dim3((unsigned)groups), dim3(1024), 0, s, (const T*)logits, ld, n, V, ids,
-                           teacher, (int)top, kLog2e / temperature, 1.f / temperature, temperature * temperature, splits,
+                           teacher, (int)top, kLog2e / temperature, 1.f / temperature, weight * temperature * temperature, splits,
                            part, (float2*)state, prob,
                            sums, groups == 1, out);
     });
@@ -313,20 +490,78 @@ ASME_API int asme_distill_xent_fwd(const void* logits, int64_t ld, int64_t n, in
     ASME_LAUNCH_CHECK("asme_distill_xent_fwd");
 }
 
+ASME_API int asme_distill_xent_grad_supported(int64_t n, int64_t V, int dtype) {
+    return dtype_ok(dtype) && n >= 1 && shape_ok(n, V, 1) && together(n, V, dtype);
+}
+ASME_API int64_t asme_distill_xent_grad_workspace(int64_t n) { return n >= 1 && shape_ok(n, 1, 1) ? n * 8 + (n + 15) / 16 * 8 : 0; }
+
+// The forward with the gradient of the mean (before the upstream factor): dlogits contiguous, its rows aligned like those
+// of logits.
+ASME_API int asme_distill_xent_fwd_grad(const void* logits, int64_t ld, int64_t n, int64_t V, const int64_t* ids,
+                                        const float* teacher, int64_t top, float temperature, float weight, int dtype,
+                                        float* state, float* prob, void* dlogits, void* workspace, int64_t ws_bytes, float* out,
+                                        void* stream) {
+    ASME_CHECK_ARG(logits && ids && teacher && state && prob && dlogits && workspace && out,
+                   "asme_distill_xent_fwd_grad: null pointer");
+    ASME_CHECK_ARG(logits != dlogits, "asme_distill_xent_fwd_grad: dlogits must not be logits");
+    ASME_CHECK_ARG(n >= 1 && shape_ok(n, V, top) && ld >= V && asme_distill_xent_grad_supported(n, V, dtype),
+                   "asme_distill_xent_fwd_grad: bad size");
+    ASME_CHECK_ARG(((uintptr_t)logits & 15) == ((uintptr_t)dlogits & 15) && (ld - V) * dtype_size(dtype) % 16 == 0,
+                   "asme_distill_xent_fwd_grad: rows of logits and dlogits are aligned alike");
+    ASME_CHECK_ARG(temperature > 0.f && temperature < INFINITY && weight - weight == 0.f,
+                   "asme_distill_xent_fwd_grad: temperature > 0, a finite weight");
+    ASME_CHECK_ARG(ws_bytes >= asme_distill_xent_grad_workspace(n), "asme_distill_xent_fwd_grad: workspace too small");
+    hipStream_t s = (hipStream_t)stream;
+    float* sums = (float*)workspace;
+    float* counts = sums + 2 * n;
+    const int64_t groups = (n + 15) / 16;
+    hipLaunchKernelGGL(teacher_kernel, dim3((unsigned)groups), dim3(1024), 0, s, ids, teacher, n, V, (int)top,
+                       1.f / temperature, prob, counts);
+    hipLaunchKernelGGL(mean_kernel, dim3(1), dim3(1024), 0, s, counts, groups, out);
+    with_dtype(dtype, [&](auto t) {
+        using T = decltype(t);
+        auto launch = [&](auto vecs) {
+            hipLaunchKernelGGL((fused_kernel<T, decltype(vecs)::value>), dim3((unsigned)n), dim3(kRowThreads), 0, s,
+                               (const T*)logits, ld, (int)V, ids, (int)top, kLog2e / temperature,
+                               weight * temperature * temperature, weight * temperature, prob, out, (float2*)state, sums,
+                               (T*)dlogits, V);
+        };
+        if (V <= kRowThreads * kMostVecs / 2 * Elem<T>::V) launch(std::integral_constant<int, kMostVecs / 2>{});
+        else launch(std::integral_constant<int, kMostVecs>{});
+    });
+    hipLaunchKernelGGL(mean_kernel, dim3(1), dim3(1024), 0, s, sums, n, out);
+    ASME_LAUNCH_CHECK("asme_distill_xent_fwd_grad");
+}
+
+// x (n values, 16-byte aligned) *= factor[0]
+ASME_API int asme_scale_by(void* x, int64_t n, int dtype, const float* factor, void* stream) {
+    ASME_CHECK_ARG(x && factor, "asme_scale_by: null pointer");
+    ASME_CHECK_ARG(dtype_ok(dtype) && n >= 0 && ((uintptr_t)x & 15) == 0, "asme_scale_by: bad argument");
+    if (n == 0) return 0;
+    with_dtype(dtype, [&](auto t) {
+        using T = decltype(t);
+        const int64_t groups = (n / Elem<T>::V + kThreads - 1) / kThreads;
+        hipLaunchKernelGGL(scale_kernel<T>, dim3((unsigned)std::max<int64_t>(1, std::min<int64_t>(groups, 4096))),
+                           dim3(kThreads), 0, (hipStream_t)stream, (T*)x, n, factor);
+    });
+    ASME_LAUNCH_CHECK("asme_scale_by");
+}
+
 ASME_API int asme_distill_xent_bwd(const void* logits, int64_t ld, int64_t n, int64_t V, const int64_t* ids, int64_t top,
-                                   float temperature, int dtype, const float* state, const float* prob,
+                                   float temperature, float weight, int dtype, const float* state, const float* prob,
                                    const float* stats, const float* dloss, void* dlogits, int64_t ld_d, void* stream) {
     ASME_CHECK_ARG(logits && ids && state && prob && stats && dloss && dlogits, "asme_distill_xent_bwd: null pointer");
     ASME_CHECK_ARG(logits != dlogits, "asme_distill_xent_bwd: dlogits must not be logits");
     ASME_CHECK_ARG(dtype_ok(dtype), "asme_distill_xent_bwd: dtype is 0 (fp32) or 1 (bf16)");
     ASME_CHECK_ARG(n >= 1 && shape_ok(n, V, top) && ld >= V && ld_d >= V, "asme_distill_xent_bwd: bad size");
-    ASME_CHECK_ARG(temperature > 0.f && temperature < INFINITY, "asme_distill_xent_bwd: temperature > 0");
+    ASME_CHECK_ARG(temperature > 0.f && temperature < INFINITY && weight - weight == 0.f,
+                   "asme_distill_xent_bwd: temperature > 0, a finite weight");
     const int splits = row_splits(n, V);
     with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
         hipLaunchKernelGGL(grad_kernel<T>, dim3((unsigned)(n * splits)), dim3(kThreads), 0, (hipStream_t)stream,
                            (const T*)logits, ld, V, ids, (int)top, splits, split_len(V, splits), kLog2e / temperature,
-                           temperature, (const float2*)state, prob, stats, dloss, (T*)dlogits, ld_d);
+                           weight * temperature, (const float2*)state, prob, stats, dloss, (T*)dlogits, ld_d);
     });
     ASME_LAUNCH_CHECK("asme_distill_xent_bwd");
 }

@@ -36,8 +36,10 @@ class TopKDistillationLoss(nn.Module):
             raise ValueError(f"weight {weight}: expected 0 to 1")
         self.temperature, self.weight = temperature, weight
 
-    def forward(self, teacher_ids: torch.Tensor, teacher_logits: torch.Tensor, logits: torch.Tensor) -> torch.Tensor:
-        return ops.distill_cross_entropy(logits, teacher_ids, teacher_logits, self.temperature)
+    def forward(self, teacher_ids: torch.Tensor, teacher_logits: torch.Tensor, logits: torch.Tensor,
+                weight: float = 1.0) -> torch.Tensor:
+        """`weight` times the divergence"""
+        return ops.distill_cross_entropy(logits, teacher_ids, teacher_logits, self.temperature, weight)
 
 
 class SASRecFullSequenceCrossEntropyLoss(nn.Module):

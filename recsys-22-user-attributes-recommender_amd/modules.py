@@ -322,7 +322,7 @@ def _rows_distillation(model, sequence, batch, rows, targets, pad: int, loss, in
     lists = [batch[k].reshape(-1, batch[k].shape[-1]).index_select(0, rows)
              for k in (TEACHER_IDS_ENTRY_NAME, TEACHER_LOGITS_ENTRY_NAME)]
     logits = model.forward_rows(sequence, rows, inverse)
-    return loss.weight * loss(*lists, logits) + (1.0 - loss.weight) * ops.cross_entropy(logits, targets, pad)
+    return loss(*lists, logits, weight=loss.weight) + (1.0 - loss.weight) * ops.cross_entropy(logits, targets, pad)
 
 
 def _single_target_cross_entropy(model, sequence, targets, pad: int) -> torch.Tensor:

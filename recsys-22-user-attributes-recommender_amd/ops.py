@@ -1990,43 +1990,61 @@ class _DistillFn(torch.autograd.Function):
     """tau^2 KL(teacher's list || softmax over the catalogue), mean over the rows with a list (csrc/distill.hip)."""
 
     @staticmethod
-    def forward(ctx, logits, ids, teacher, temperature: float):
+    def forward(ctx, logits, ids, teacher, temperature: float, weight: float):
         V, top = logits.shape[-1], ids.shape[-1]
-        x = logits.reshape(-1, V)
-        if x.stride(1) != 1 or x.stride(0) < V:
-            x = x.contiguous()
+        x = logits if logits.dim() == 2 and logits.stride(1) == 1 and logits.stride(0) >= V else logits.contiguous()
+        kept, x = x, x if x.dim() == 2 else x.view(-1, V)
         ids, teacher = _i64(ids), teacher.to(torch.float32).contiguous()
         n, dev = x.shape[0], x.device
         state = torch.empty(n, 2, device=dev, dtype=torch.float32)
         prob = torch.empty(n, top, device=dev, dtype=torch.float32)
         out = torch.empty(2, device=dev, dtype=torch.float32)
+        ctx.save_for_backward(kept, ids, state, prob, out)
+        ctx.meta, ctx.grad = (temperature, weight, logits.shape), None
+        code = _dtype_code(x)
+        # the gradient with the forward (csrc/distill.hip, "together") where a workgroup holds a row: at 8192 x 26747 fp32
+        # 375 us forward and backward in place of 580; 785 where an upstream factor other than 1 is left to apply
+        if (ctx.needs_input_grad[0] and x.is_contiguous() and x.data_ptr() % 16 == 0
+                and _lib.load().asme_distill_xent_grad_supported(n, V, code)):
+            ctx.grad = torch.empty(logits.shape, device=dev, dtype=x.dtype)
+            ws, nb = _ws_bytes("asme_distill_xent_grad_workspace", n, device=dev)
+            _call_on(x, "asme_distill_xent_fwd_grad", ptr(x), V, n, V, ptr(ids), ptr(teacher), top, temperature, weight, code,
+                     ptr(state), ptr(prob), ptr(ctx.grad), ptr(ws), nb, ptr(out))
+            return out[0]
         ws, nb = _ws_bytes("asme_distill_xent_workspace", n, V, device=dev)
-        _call_on(x, "asme_distill_xent_fwd", ptr(x), x.stride(0), n, V, ptr(ids), ptr(teacher), top, temperature,
-                 _dtype_code(x), ptr(state), ptr(prob), ptr(ws), nb, ptr(out))
-        ctx.save_for_backward(x, ids, state, prob, out)
-        ctx.meta = (temperature, logits.shape)
+        _call_on(x, "asme_distill_xent_fwd", ptr(x), x.stride(0), n, V, ptr(ids), ptr(teacher), top, temperature, weight, code,
+                 ptr(state), ptr(prob), ptr(ws), nb, ptr(out))
         return out[0]
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dloss):
         x, ids, state, prob, out = ctx.saved_tensors
-        temperature, shape = ctx.meta
-        n, V = x.shape
+        temperature, weight, shape = ctx.meta
+        V = shape[-1]
+        x = x if x.dim() == 2 else x.view(-1, V)
+        n = x.shape[0]
+        g, ctx.grad = ctx.grad, None
+        if g is not None:
+            _call_on(g, "asme_scale_by", ptr(g), g.numel(), _dtype_code(g), ptr(_f32(dloss)))
+            return g, None, None, None, None
+        # (also a second backward of one forward: the first one gave its gradient away)
         g = torch.empty(shape, device=x.device, dtype=x.dtype)
-        _call_on(x, "asme_distill_xent_bwd", ptr(x), x.stride(0), n, V, ptr(ids), ids.shape[-1], temperature,
+        _call_on(x, "asme_distill_xent_bwd", ptr(x), x.stride(0), n, V, ptr(ids), ids.shape[-1], temperature, weight,
                  _dtype_code(x), ptr(state), ptr(prob), ptr(out), ptr(_f32(dloss)), ptr(g), V)
-        return g, None, None, None
+        return g, None, None, None, None
 
 
 def distill_cross_entropy(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits: torch.Tensor,
-                          temperature: float = 1.0) -> torch.Tensor:
+                          temperature: float = 1.0, weight: float = 1.0) -> torch.Tensor:
     """Distillation from a teacher's best items: for logits (..., V) and the teacher's lists teacher_ids,
     teacher_logits (..., k <= 1024; e.g. of catalog_topk), the scalar
-        temperature^2 * KL(softmax(teacher_logits / temperature) over the list || softmax(logits / temperature) over V),
+        weight * temperature^2 * KL(softmax(teacher_logits / temperature) over the list || softmax(logits / temperature)
+        over V),
     mean over the rows whose list is not empty (NaN when all are).  Entries whose id is not in [0, V) (-1 ends a shorter
     list) are absent; an item twice on a list counts twice.  The gradient goes to `logits`; the teacher takes none.
-    logits float32 or bfloat16, the loss float32."""
+    logits float32 or bfloat16, the loss float32.  A loss that is one part of another is cheapest with its `weight` here:
+    the gradient is formed with the forward for that weight, and a factor other than 1 from above is one more pass."""
     V, top = logits.shape[-1], teacher_ids.shape[-1]
     if teacher_ids.shape != teacher_logits.shape or teacher_ids.shape[:-1] != logits.shape[:-1]:
         raise ValueError(f"logits {tuple(logits.shape)}, teacher_ids {tuple(teacher_ids.shape)} and teacher_logits "
@@ -2037,13 +2055,15 @@ def distill_cross_entropy(logits: torch.Tensor, teacher_ids: torch.Tensor, teach
         raise TypeError(f"teacher_ids are whole numbers, got {teacher_ids.dtype}")
     if not 0.0 < temperature < math.inf:
         raise ValueError(f"temperature {temperature}: expected a positive number")
+    if not math.isfinite(weight):
+        raise ValueError(f"weight {weight}: expected a finite number")
     if torch.is_grad_enabled() and teacher_logits.requires_grad:
         raise ValueError("distill_cross_entropy gives the teacher no gradient: detach teacher_logits")
     _dtype_code(logits)
     _alike(logits, teacher_ids=teacher_ids, teacher_logits=teacher_logits)
     if logits.numel() == 0:
         return logits.float().sum() * math.nan  # the mean over no rows
-    return _DistillFn.apply(logits, teacher_ids, teacher_logits, float(temperature))
+    return _DistillFn.apply(logits, teacher_ids, teacher_logits, float(temperature), float(weight))
 
 
 def linear_xent_ok(hidden: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None) -> bool:

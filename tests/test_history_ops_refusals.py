@@ -80,6 +80,8 @@ def test_distill_types(asme):
         op(f32(3, 7), t, t)
     with pytest.raises(TypeError, match="float32 or bfloat16"):
         op(f32(3, 7).double(), ids, t)
+    with pytest.raises(ValueError, match="weight"):
+        op(f32(3, 7), ids, t, 1.0, math.nan)
     with pytest.raises(ValueError, match="teacher"):
         op(f32(3, 7), ids, t.clone().requires_grad_())
     with pytest.raises(asme._lib.ASMEKernelError, match="no CPU fallback"):
@@ -171,15 +173,23 @@ def test_c_entries_refuse(asme):
     refused(lib.asme_window_cache_fill(p, p, 64, 16, 17, 64, 16, 16, p, 1, 4, 1, 16, 4, 0, 0, p, p, None), b"alignment")
     refused(lib.asme_window_cache_fill(p, p, 64, 16, 16, 64, 16, 16, p, 1, 0, 1, 16, 4, 0, 0, p, p, None), b"size")
 
-    def distill(x=p, ld=8, n=2, V=8, top=2, tau=1.0, dtype=0, nb=1 << 20):
-        return lib.asme_distill_xent_fwd(x, ld, n, V, p, p, top, tau, dtype, p, p, p, nb, p, None)
+    def distill(x=p, ld=8, n=2, V=8, top=2, tau=1.0, w=1.0, dtype=0, nb=1 << 20):
+        return lib.asme_distill_xent_fwd(x, ld, n, V, p, p, top, tau, w, dtype, p, p, p, nb, p, None)
 
     refused(distill(x=None), b"null")
     for bad in (dict(ld=7), dict(n=0), dict(V=0), dict(V=1 << 31, ld=1 << 31), dict(top=0), dict(top=1025)):
         refused(distill(**bad), b"size")
     refused(distill(tau=0.0), b"temperature")
+    refused(distill(w=math.inf), b"weight")
     refused(distill(nb=8), b"workspace")
-    refused(lib.asme_distill_xent_bwd(p, 8, 2, 8, p, 2, 1.0, 0, p, p, p, p, p, 8, None), b"must not be")
+    for n, V in ((511, 8192), (512, 4095), (512, 32769)):
+        assert lib.asme_distill_xent_grad_supported(n, V, 0) == 0
+        refused(lib.asme_distill_xent_fwd_grad(p, V, n, V, p, p, 2, 1.0, 1.0, 0, p, p, p + 16, p, 1 << 30, p, None), b"size")
+    assert lib.asme_distill_xent_grad_supported(512, 65536, 1) == 1
+    refused(lib.asme_distill_xent_fwd_grad(p, 8192, 512, 8192, p, p, 2, 1.0, 1.0, 0, p, p, p + 4, p, 1 << 30, p, None),
+            b"aligned")
+    refused(lib.asme_scale_by(p + 4, 8, 0, p, None), b"bad")
+    refused(lib.asme_distill_xent_bwd(p, 8, 2, 8, p, 2, 1.0, 1.0, 0, p, p, p, p, p, 8, None), b"must not be")
 
     def norm(res=p, n=4, d=8, per=1, gate=p, dtype=0, eps=1e-5, pre=None, z=None):
         return lib.asme_gated_residual_norm_fwd(res, p, gate, per, p, None, pre, None, n, d, 1.0, eps, 0, dtype, p, z, p,
