@@ -35,50 +35,68 @@ __device__ __forceinline__ float lanes_sum(float x) {
     return x;
 }
 
-// A row over TPR threads of N values each: VEC: whole 16-byte vectors, else single elements TPR apart
-template <class T, int TPR, int N, bool VEC>
+// A row over TPR threads of N values each, in vectors of 16 bytes.  EVEN: rows are whole vectors on their boundaries; else
+// vectors begin anywhere (global memory is read and written at any address) and the last one, part of a vector, goes
+// element by element -- a branch around a row's loads that costs even rows 8 % (16384 x 4096 bf16, backward: 211 us
+// without, 228 with it), but rows of 1024 threads less than the registers it saves (8192 x 4096 fp32: 333 us with it, 435
+// without), which therefore always take it.
+template <class T, int TPR, int N, bool EVEN>
 struct Row {
     static constexpr int kPer = N, TPRv = TPR;
     static constexpr int kThreads = TPR > 64 ? TPR : 256;
     static constexpr int kSlots = kThreads / TPR;  // rows at a time
-    static constexpr int E = VEC ? Elem<T>::V : 1, kVecs = N / E;
+    static constexpr int E = Elem<T>::V, kVecs = N / E;
+    // rows beyond 4096 values: the backward's weights and next row do not fit 128 registers beside its sums -- it reads
+    // them when they are due, and still spills some (4000 x 8192 fp32: 476 us forward and backward, 46 % of the bytes' time;
+    // 512 threads of 16 values and 256 registers took 562)
+    static constexpr bool kLean = TPR * N > 4096;
+    typedef T Vec __attribute__((ext_vector_type(E)));
+    typedef Vec AnyVec __attribute__((aligned(EVEN ? 16 : sizeof(T))));
     // a row's values as they are stored
     struct Raw {
-        typedef T Vec __attribute__((ext_vector_type(VEC ? E : 1)));
-        std::conditional_t<VEC, Vec, T> v[kVecs];
-        __device__ __forceinline__ void load(const T* p, int t, int D) {
+        Vec v[kVecs];
+        template <bool WHOLE>
+        __device__ __forceinline__ void load(const T* p, int t, int D, int c) {  // its vector c
+            const int j = (c * TPR + t) * E;
+            if constexpr (EVEN) {
+                v[c] = *reinterpret_cast<const AnyVec*>(p + (j < D ? j : 0));  // (behind the row: its first, not used)
+            } else if constexpr (WHOLE) {
+                v[c] = *reinterpret_cast<const AnyVec*>(p + j);
+            } else {
 #pragma unroll
-            for (int c = 0; c < kVecs; ++c) {
-                const int j = (c * TPR + t) * E;
-                // (behind the row: its first value, not used)
-                v[c] = *reinterpret_cast<const std::conditional_t<VEC, Vec, T>*>(p + (j < D ? j : 0));
+                for (int e = 0; e < E; ++e) v[c][e] = j + e < D ? p[j + e] : (T)0.f;
             }
         }
         __device__ __forceinline__ void get(int t, int D, float (&x)[N]) const {
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-                float f;
-                if constexpr (VEC) f = (float)v[i / E][i % E];
-                else f = (float)v[i];
-                x[i] = col(t, i) < D ? f : 0.f;
-            }
+            for (int i = 0; i < N; ++i) x[i] = EVEN && col(t, i) >= D ? 0.f : (float)v[i / E][i % E];
         }
     };
+    // f(vector, whether it is whole) for a thread's vectors: one branch around the loads of a row's tensors, not one around
+    // each
+    template <class F>
+    static __device__ __forceinline__ void loads(int t, int D, F&& f) {
+#pragma unroll
+        for (int c = 0; c < kVecs; ++c) {
+            if (EVEN || (c * TPR + t) * E + E <= D) f(c, std::true_type{});
+            else f(c, std::false_type{});
+        }
+    }
     static __device__ __forceinline__ int col(int t, int i) { return ((i / E) * TPR + t) * E + i % E; }
     static __device__ __forceinline__ void store(T* p, int t, int D, const float (&x)[N]) {
-        if constexpr (VEC) {
 #pragma unroll
-            for (int c = 0; c < kVecs; ++c) {
-                float v[E];
-                const int j = (c * TPR + t) * E;
+        for (int c = 0; c < kVecs; ++c) {
+            const int j = (c * TPR + t) * E;
+            Vec v;
 #pragma unroll
-                for (int e = 0; e < E; ++e) v[e] = x[c * E + e];
-                if (j < D) Elem<T>::store(p + j, v);
+            for (int e = 0; e < E; ++e) v[e] = (T)x[c * E + e];
+            if (j + E <= D) {
+                *reinterpret_cast<AnyVec*>(p + j) = v;
+            } else if constexpr (!EVEN) {
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    if (j + e < D) p[j + e] = v[e];
             }
-        } else {
-#pragma unroll
-            for (int i = 0; i < N; ++i)
-                if (i * TPR + t < D) Elem<T>::put(p + i * TPR + t, x[i]);
         }
     }
     static __device__ __forceinline__ void load_f32(const float* p, int t, int D, float def, float (&x)[N]) {
@@ -165,9 +183,13 @@ __global__ __launch_bounds__(R::kThreads) void fwd_kernel(Args a) {
     const int64_t step = (int64_t)gridDim.x * R::kSlots;
     auto fetch = [&](int64_t base) {  // the row that this thread's slot has from `base` on
         const int64_t row = min(base + slot, a.n - 1);
-        raw_y.load((const T*)a.y + row * D, t, D);
-        raw_s.load((const T*)a.res + row * D, t, D);
-        if (a.gate) raw_g.load((const T*)a.gate + row / a.rows_per_gate * D, t, D);
+        const T* g = (const T*)a.gate + (a.gate ? row / a.rows_per_gate * D : 0);
+        R::loads(t, D, [&](int c, auto whole) {
+            constexpr bool W = decltype(whole)::value;
+            raw_y.template load<W>((const T*)a.y + row * D, t, D, c);
+            raw_s.template load<W>((const T*)a.res + row * D, t, D, c);
+            if (a.gate) raw_g.template load<W>(g, t, D, c);
+        });
     };
     // (every thread of a workgroup makes the same number of turns: the row sums may hold a barrier)
     int64_t base = (int64_t)blockIdx.x * R::kSlots;
@@ -234,9 +256,12 @@ __global__ __launch_bounds__(R::kThreads) void bwd_kernel(Args a) {
     const int t = threadIdx.x % R::TPRv, slot = R::kSlots > 1 ? threadIdx.x / R::TPRv : 0, D = a.D;
     const float inv_d = 1.f / (float)D, centre = a.rms ? 0.f : 1.f;
     float pw[kPer], pb[kPer], qw[kPer];
-    R::load_f32(a.post_w, t, D, 1.f, pw);
-    R::load_f32(a.post_b, t, D, 0.f, pb);
-    R::load_f32(a.pre_w, t, D, 1.f, qw);
+    auto weights = [&]() {
+        R::load_f32(a.post_w, t, D, 1.f, pw);
+        R::load_f32(a.post_b, t, D, 0.f, pb);
+        R::load_f32(a.pre_w, t, D, 1.f, qw);
+    };
+    if (!R::kLean) weights();
     float acc[4][kPer], gacc[kPer];
 #pragma unroll
     for (int i = 0; i < kPer; ++i) acc[0][i] = acc[1][i] = acc[2][i] = acc[3][i] = gacc[i] = 0.f;
@@ -246,20 +271,24 @@ __global__ __launch_bounds__(R::kThreads) void bwd_kernel(Args a) {
     auto fetch = [&](int64_t base, int64_t end, int64_t group) {
         const int64_t row = min(base + slot, end - 1);
         next_st = *reinterpret_cast<const float4*>(a.stats + row * 4);
-        raw_y.load((const T*)a.y + row * D, t, D);
-        raw_s.load((const T*)a.res + row * D, t, D);
-        if (a.ds) raw_d.load((const T*)a.ds + row * D, t, D);
-        if (a.dz) raw_z.load((const T*)a.dz + row * D, t, D);
-        if (GATE) raw_g.load((const T*)a.gate + (GATE == 1 ? row : group) * D, t, D);
+        R::loads(t, D, [&](int c, auto whole) {
+            constexpr bool W = decltype(whole)::value;
+            raw_y.template load<W>((const T*)a.y + row * D, t, D, c);
+            raw_s.template load<W>((const T*)a.res + row * D, t, D, c);
+            if (GATE) raw_g.template load<W>((const T*)a.gate + (GATE == 1 ? row : group) * D, t, D, c);
+            if (a.ds) raw_d.template load<W>((const T*)a.ds + row * D, t, D, c);
+            if (a.dz) raw_z.template load<W>((const T*)a.dz + row * D, t, D, c);
+        });
     };
     for (int64_t item = blockIdx.x; item < a.items; item += gridDim.x) {
         const int64_t group = item / a.subs, first = (item % a.subs) * a.sub_rows;
         const int64_t begin = group * a.rows_per_gate + first;
         const int64_t end = group * a.rows_per_gate + min(a.rows_per_gate, first + a.sub_rows);
-        fetch(begin, end, group);
+        if (!R::kLean) fetch(begin, end, group);
         for (int64_t base = begin; base < end; base += R::kSlots) {
             const bool live = base + slot < end;
             const int64_t row = live ? base + slot : end - 1;
+            if (R::kLean) weights(), fetch(base, end, group);
             const float4 st = next_st;
             float y[kPer], s[kPer], d[kPer], g[kPer], dz[kPer];
             raw_y.get(t, D, y);
@@ -267,7 +296,7 @@ __global__ __launch_bounds__(R::kThreads) void bwd_kernel(Args a) {
             if (a.ds) raw_d.get(t, D, d);
             if (a.dz) raw_z.get(t, D, dz);
             if (GATE) raw_g.get(t, D, g);
-            if (base + R::kSlots < end) fetch(base + R::kSlots, end, group);  // on its way during this row's sums
+            if (!R::kLean && base + R::kSlots < end) fetch(base + R::kSlots, end, group);  // on its way during this row's sums
 #pragma unroll
             for (int i = 0; i < kPer; ++i) {
                 if (!live || !a.ds) d[i] = 0.f;
@@ -378,23 +407,23 @@ bool aligned(std::initializer_list<const void*> ps) {
     return true;
 }
 
-// f(Row<...>{}) for a checked dim: the fewest threads a row (at least 16) that hold it at one 16-byte vector each -- 8
-// single elements where rows are not whole vectors or not aligned, two fp32 vectors beyond 4096
+// f(Row<...>{}) for a checked dim: the fewest threads a row (at least 16) that hold it at one 16-byte vector each, 8
+// values beyond 4096
 template <class T, class F>
-void with_row(int64_t D, bool vec, F&& f) {
-    auto pick = [&](auto v) {
-        constexpr bool VEC = decltype(v)::value;
-        constexpr int N = VEC ? Elem<T>::V : 8;
-        if (D <= 16 * N) f(Row<T, 16, N, VEC>{});
-        else if (D <= 32 * N) f(Row<T, 32, N, VEC>{});
-        else if (D <= 64 * N) f(Row<T, 64, N, VEC>{});
-        else if (D <= 128 * N) f(Row<T, 128, N, VEC>{});
-        else if (D <= 256 * N) f(Row<T, 256, N, VEC>{});
-        else if (D <= 512 * N) f(Row<T, 512, N, VEC>{});
-        else if (N == 8 || D > 1024 * N) f(Row<T, 1024, 8, VEC>{});
-        else f(Row<T, 1024, N, VEC>{});
+void with_row(int64_t D, bool even, F&& f) {
+    constexpr int N = Elem<T>::V;
+    auto pick = [&](auto even) {
+        constexpr bool EVEN = decltype(even)::value;
+        if (D <= 16 * N) f(Row<T, 16, N, EVEN>{});
+        else if (D <= 32 * N) f(Row<T, 32, N, EVEN>{});
+        else if (D <= 64 * N) f(Row<T, 64, N, EVEN>{});
+        else if (D <= 128 * N) f(Row<T, 128, N, EVEN>{});
+        else if (D <= 256 * N) f(Row<T, 256, N, EVEN>{});
+        else if (EVEN || D <= 512 * N) f(Row<T, 512, N, EVEN>{});
+        else if (N == 4 && D <= 4096) f(Row<T, 1024, 4, false>{});
+        else f(Row<T, 1024, 8, false>{});
     };
-    if (vec) pick(std::true_type{});
+    if (even && D % N == 0 && D <= 512 * N) pick(std::true_type{});
     else pick(std::false_type{});
 }
 
@@ -404,10 +433,8 @@ template <class R>
 constexpr int64_t fill() {
     return fill_of(R::kThreads);
 }
-// the most of them that any layout of a dim takes: rows at 8 values a thread
-int64_t most_groups(int64_t D) {
-    return fill_of(D <= 512 ? 256 : D <= 1024 ? 128 : D <= 2048 ? 256 : D <= 4096 ? 512 : 1024);
-}
+// the most of them that any layout of a dim takes (at most 8 values a thread)
+int64_t most_groups(int64_t D) { return D <= 2048 ? 1024 : D <= 4096 ? fill_of(512) : fill_of(1024); }
 
 struct Plan {
     int64_t subs, sub_rows, items, grid;
@@ -448,7 +475,7 @@ ASME_API int asme_gated_residual_norm_fwd(const void* res, const void* y, const 
     a.rms = rms, a.s = s_out, a.z = z_out, a.stats = stats;
     with_dtype(dtype, [&](auto e) {
         using T = decltype(e);
-        with_row<T>(dim, dim % Elem<T>::V == 0 && aligned({res, y, gate, s_out, z_out}), [&](auto r) {
+        with_row<T>(dim, aligned({res, y, gate, s_out, z_out}), [&](auto r) {
             using R = decltype(r);
             const int64_t turns = (n + R::kSlots - 1) / R::kSlots;
             hipLaunchKernelGGL((fwd_kernel<T, R>), dim3((unsigned)std::min(turns, 2 * fill<R>())),
@@ -491,7 +518,7 @@ ASME_API int asme_gated_residual_norm_bwd(const void* res, const void* y, const 
     Plan p{};
     with_dtype(dtype, [&](auto e) {
         using T = decltype(e);
-        with_row<T>(dim, dim % Elem<T>::V == 0 && aligned({res, y, gate, ds, dz, dres, dy, dgate}), [&](auto r) {
+        with_row<T>(dim, aligned({res, y, gate, ds, dz, dres, dy, dgate}), [&](auto r) {
             using R = decltype(r);
             p = plan(n, rows, R::kSlots, fill<R>());
             a.gate_part = (float*)workspace + p.grid * 4 * dim;

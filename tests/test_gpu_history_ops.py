@@ -183,7 +183,7 @@ NORM_CASES = [  # batch, length, dim, gate
     (1, 1, 1, "none"), (2, 3, 8, "sequence"), (3, 5, 17, "row"), (2, 37, 128, "channel"), (3, 33, 100, "sequence"),
     (1, 50, 132, "channel"), (4, 9, 256, "row"), (5, 7, 300, "sequence"), (2, 11, 520, "none"), (1, 19, 1024, "channel"),
     (2, 6, 1111, "sequence"), (3, 4, 2048, "row"), (2, 5, 4096, "channel"), (2, 3, 5000, "sequence"),
-    (1, 4, 8192, "channel"), (1, 3, 8191, "row"), (40, 200, 64, "sequence"), (1, 5000, 64, "channel"),
+    (2, 3, 4100, "row"), (1, 4, 8192, "channel"), (1, 3, 8191, "row"), (40, 200, 64, "sequence"), (1, 5000, 64, "channel"),
     (2500, 2, 32, "sequence")]
 
 
