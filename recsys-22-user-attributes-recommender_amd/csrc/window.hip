@@ -24,9 +24,10 @@
 // (7 products for the 5 of a single pass), so no sum depends on the order of atomics.
 //
 // fp32 tensors are split exactly into three bf16 planes on the way into LDS and the products kept to fp32 level by six
-// MFMAs (common.h, bf16x6); bf16 tensors take one, P and dS rounded to bf16 for their second product (at most 2^-8 of
-// each term, the size of the output's own rounding, averaged over the row) -- but for dQ, where the terms cancel (a row of
-// dS sums to 0) and dS goes in as two bf16 terms: rounded to one, dQ was off by 1.5 times its own rounding.  Scores, softmax statistics and all sums are fp32.
+// MFMAs (common.h, bf16x6); bf16 tensors take one, P rounded to bf16 for its second product (at most 2^-8 of
+// each term, the size of the output's own rounding, averaged over the row; Pass::W).  dS, whose terms cancel (a row of it sums to
+// 0), goes into dQ and dK as two bf16 terms: rounded to one, they were off by 1.5 to 2 times their own rounding.  Scores,
+// softmax statistics and all sums are fp32.
 #include "elem.h"
 
 using namespace asme;
@@ -40,9 +41,6 @@ constexpr int kImage = kTS * kRowB;      // 16 KiB
 
 typedef short short4v __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) short4v lds_short4;
-
-// the streamed row of accumulator register i in lane half h (32x32 output)
-__device__ __forceinline__ int acc_row(int i, int h) { return (i & 3) + 8 * (i >> 2) + 4 * h; }
 
 // byte of 16-byte chunk ch in row r of an image of 256-byte rows: transposed reads without bank conflicts, row reads 2-way
 __device__ __forceinline__ int swz(int r, int ch) { return r * kRowB + 16 * (ch ^ (((r & 3) << 2) | ((r >> 2) & 3))); }
@@ -148,8 +146,21 @@ struct Pass {
     static constexpr int kImages = DP == 128 ? 2 : 1;
     static constexpr int kBytes = NP * kImages * kImage;
     using F = Frag<NP>;
-    using S = Frag<NP == 1 ? 2 : NP>;  // dS as a factor of dQ
+    static constexpr int SP = NP == 1 ? 2 : NP;  // planes of dS as a factor
+    using S = Frag<SP>;
+    // P as a factor: of bf16 in one term where the matrix and vector units bound the pass (eight waves; two cost 295 us for
+    // 248 forward at L = 8192 and 128 columns, dK and dV 616 for 506); in two where they do not, among them the shortest
+    // sequences, whose few terms' roundings do not average out
+    using W = Frag<NW < 8 ? SP : NP>;
 
+    // The compiler keeps the LDS addresses of a tile's reads and writes, which are the same in every round, in registers:
+    // faster by 10 % than forming them anew (L = 8192, bf16, 128 columns) where there are registers.  fp32 rows of 128
+    // columns leave none (up to 91 spilled values); there the thread's number is made new to it in every round.
+    static __device__ __forceinline__ int thread() {
+        int t = threadIdx.x;
+        if constexpr (NP == 3 && DP == 128) asm volatile("" : "+v"(t));
+        return t;
+    }
     static __device__ __forceinline__ int place(int op, int plane, int row, int ch) {
         if constexpr (DP == 128) return (plane * 2 + op) * kImage + swz(row, ch);
         return plane * kImage + swz(row, ch + op * (DP / 8));
@@ -185,10 +196,10 @@ struct Pass {
         }
     }
     static __device__ __forceinline__ void put(char* lds, Chunk<T> (&c)[kEach], uint64_t rows) {
-        const int ch = threadIdx.x % (DP / 8);
+        const int t = thread(), ch = t % (DP / 8);
 #pragma unroll
         for (int e = 0; e < kEach; ++e) {
-            const int row = e % (kEach / 2) * kRowStep + threadIdx.x / (DP / 8);
+            const int row = e % (kEach / 2) * kRowStep + t / (DP / 8);
             if (rows != ~0ull && !((rows >> row) & 1)) c[e].zero();
             const F f = c[e].frag();
 #pragma unroll
@@ -210,7 +221,7 @@ struct Pass {
     // together, so that a product waits for the first of them and not each for its own
     static constexpr int kStep = NP == 1 ? (KS < 4 ? KS : 4) : 2;
     static __device__ __forceinline__ floatx16 score(const char* lds, int op, int sub, const F (&st)[KS]) {
-        const int lane = threadIdx.x & 63, r32 = lane & 31, h = lane >> 5;
+        const int lane = thread() & 63, r32 = lane & 31, h = lane >> 5;
         floatx16 x;
 #pragma unroll
         for (int i = 0; i < 16; ++i) x[i] = 0.f;
@@ -229,12 +240,13 @@ struct Pass {
     }
     // Y^T[feature][stationary row] += streamed^T . x: rows 16 s2 + 8 (j >> 2) + 4 h + (j & 3) of the half are element j of
     // the lane's B fragment; 16-lane group (h, fh) reads rows + q x features 32 ft + 16 fh + 4 p4 .. + 3 transposed
-    static __device__ __forceinline__ void read_transposed(const char* lds, int op, int sub, int s2, F (&A)[NFT]) {
-        const int lane = threadIdx.x & 63, h = lane >> 5, fh = (lane >> 4) & 1, q = (lane & 15) >> 2, p4 = lane & 3;
+    template <int N>
+    static __device__ __forceinline__ void read_transposed(const char* lds, int op, int sub, int s2, int first, F (&A)[N]) {
+        const int lane = thread() & 63, h = lane >> 5, fh = (lane >> 4) & 1, q = (lane & 15) >> 2, p4 = lane & 3;
         const int lo = 32 * sub + 16 * s2 + 4 * h + q;
 #pragma unroll
-        for (int ft = 0; ft < NFT; ++ft) {
-            const int ch = 4 * ft + 2 * fh + (p4 >> 1);
+        for (int ft = 0; ft < N; ++ft) {
+            const int ch = 4 * (first + ft) + 2 * fh + (p4 >> 1);
 #pragma unroll
             for (int p = 0; p < NP; ++p) {
                 const short4v a = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
@@ -254,44 +266,34 @@ struct Pass {
         for (int j = 0; j < 8; ++j) v[j] = x[8 * s2 + j];
         return frag_of(v, (W*)nullptr);
     }
-    template <class W>
-    static __device__ __forceinline__ void gather(const char* lds, int op, int sub, const W (&w)[2], floatx16 (&y)[NFT]) {
+    // Y^T[features from 32 `first` on] += streamed^T . w of k step s2
+    template <class W, int N>
+    static __device__ __forceinline__ void gather(const char* lds, int op, int sub, int s2, int first, const W& w,
+                                                  floatx16 (&y)[N]) {
+        F A[N];
+        read_transposed(lds, op, sub, s2, first, A);
 #pragma unroll
-        for (int s2 = 0; s2 < 2; ++s2) {
-            F A[NFT];
-            read_transposed(lds, op, sub, s2, A);
+        for (int ft = 0; ft < N; ++ft) y[ft] = product(A[ft], w, y[ft]);
+    }
+    // a fragment in lane order: plane p is 1 KiB at `at` + p KiB
+    template <int N>
+    static __device__ __forceinline__ void pass_on(char* at, const Frag<N>& w) {
 #pragma unroll
-            for (int ft = 0; ft < NFT; ++ft) y[ft] = product(A[ft], w[s2], y[ft]);
-        }
+        for (int p = 0; p < N; ++p) *reinterpret_cast<bf16x8*>(at + p * 1024) = w.p[p];
     }
     template <class W>
-    static __device__ __forceinline__ void gather_as(const char* lds, int op, int sub, const floatx16& x,
-                                                     floatx16 (&y)[NFT]) {
-        const W w[2] = {weights_of<W>(x, 0), weights_of<W>(x, 1)};
-        gather(lds, op, sub, w, y);
-    }
-    // fragments in lane order: a wave's plane p of k step s2 is 1 KiB at `at` + (s2 NP + p) KiB
-    static __device__ __forceinline__ void pass_on(char* at, const floatx16& x) {
+    static __device__ __forceinline__ W passed(const char* at) {
+        W w;
 #pragma unroll
-        for (int s2 = 0; s2 < 2; ++s2) {
-            const F f = weights_of<F>(x, s2);
-#pragma unroll
-            for (int p = 0; p < NP; ++p) *reinterpret_cast<bf16x8*>(at + (s2 * NP + p) * 1024) = f.p[p];
-        }
-    }
-    static __device__ __forceinline__ void gather_passed(const char* at, const char* lds, int op, int sub,
-                                                         floatx16 (&y)[NFT]) {
-        F w[2];
-#pragma unroll
-        for (int s2 = 0; s2 < 2; ++s2)
-#pragma unroll
-            for (int p = 0; p < NP; ++p) w[s2].p[p] = *reinterpret_cast<const bf16x8*>(at + (s2 * NP + p) * 1024);
-        gather(lds, op, sub, w, y);
+        for (int p = 0; p < (int)(sizeof(W) / sizeof(bf16x8)); ++p)
+            w.p[p] = *reinterpret_cast<const bf16x8*>(at + p * 1024);
+        return w;
     }
     // row `row` (features 32 ft + 8 i + 4 h .. + 3 of this lane's stationary row) = y * f
-    static __device__ __forceinline__ void write_row(T* row, const floatx16 (&y)[NFT], float f, int h, int dim) {
+    template <int N>
+    static __device__ __forceinline__ void write_row(T* row, const floatx16 (&y)[N], float f, int h, int dim) {
 #pragma unroll
-        for (int ft = 0; ft < NFT; ++ft)
+        for (int ft = 0; ft < N; ++ft)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int c = 32 * ft + 8 * i + 4 * h;
@@ -308,9 +310,10 @@ struct Pass {
             }
     }
     // low = what rounding takes from y * f where write_row() stores it
-    static __device__ __forceinline__ void write_low(__bf16* row, const floatx16 (&y)[NFT], float f, int h, int dim) {
+    template <int N>
+    static __device__ __forceinline__ void write_low(__bf16* row, const floatx16 (&y)[N], float f, int h, int dim) {
 #pragma unroll
-        for (int ft = 0; ft < NFT; ++ft)
+        for (int ft = 0; ft < N; ++ft)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int c = 32 * ft + 8 * i + 4 * h;
@@ -326,23 +329,25 @@ struct Pass {
             }
     }
     // y += f * a row of fp32 values laid out like that
-    static __device__ __forceinline__ void add_row(const float* row, floatx16 (&y)[NFT], float f, int h, int dim) {
-        floatx4 x[NFT][4];
+    template <int N>
+    static __device__ __forceinline__ void add_row(const float* row, floatx16 (&y)[N], float f, int h, int dim) {
+        floatx4 x[N][4];
 #pragma unroll
-        for (int ft = 0; ft < NFT; ++ft)
+        for (int ft = 0; ft < N; ++ft)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int c = 32 * ft + 8 * i + 4 * h;
                 x[ft][i] = *reinterpret_cast<const floatx4*>(row + (DP > 32 || c < dim ? c : 0));
             }
 #pragma unroll
-        for (int ft = 0; ft < NFT; ++ft)
+        for (int ft = 0; ft < N; ++ft)
 #pragma unroll
             for (int e = 0; e < 16; ++e) y[ft][e] = fmaf(f, x[ft][e >> 2][e & 3], y[ft][e]);
     }
-    static __device__ __forceinline__ void clear(floatx16 (&y)[NFT]) {
+    template <int N>
+    static __device__ __forceinline__ void clear(floatx16 (&y)[N]) {
 #pragma unroll
-        for (int f = 0; f < NFT; ++f)
+        for (int f = 0; f < N; ++f)
 #pragma unroll
             for (int i = 0; i < 16; ++i) y[f][i] = 0.f;
     }
@@ -469,7 +474,9 @@ __global__ __launch_bounds__(NW * 64) void forward_kernel(Args a) {
                 x[e] = __builtin_amdgcn_exp2f(fmaf(x[e], c, -base));
                 sum += x[e];
             }
-            P::template gather_as<typename P::F>(lds, 1, sub, x, y);
+#pragma unroll
+            for (int s2 = 0; s2 < 2; ++s2)
+                P::gather(lds, 1, sub, s2, 0, P::template weights_of<typename P::W>(x, s2), y);
         }
     }
     sum += __shfl_xor(sum, 32, 64);
@@ -572,7 +579,9 @@ __global__ __launch_bounds__(NW * 64) void dq_kernel(Args a) {
 #pragma unroll
             for (int e = 0; e < 16; ++e)
                 x[e] = __builtin_amdgcn_exp2f(fmaf(x[e], c, -st.x)) * st.y * (dp[e] - delta);
-            P::template gather_as<typename P::S>(lds, 0, sub, x, y);
+#pragma unroll
+            for (int s2 = 0; s2 < 2; ++s2)
+                P::gather(lds, 0, sub, s2, 0, P::template weights_of<typename P::S>(x, s2), y);
         }
     }
     if (qi >= a.seq_len) return;
@@ -593,10 +602,11 @@ struct QueryTiles {
     }
 };
 
-// Two waves hold the same 32 keys.  Each forms P and dS of its half of the tile's queries and passes on what the other
-// sums: the first all of dV, the second all of dK.  With both sums in one wave the pass needs over 256 registers at 64 or
-// 128 columns and runs at one wave per SIMD, where the matrix and vector units take turns (395 us for the L = 8192 bf16
-// case in place of KVUS).
+// Two waves hold the same 32 keys.  Each forms P and dS of its half of the tile's queries and passes them on; each sums dK
+// and dV over all the queries, for its half of the columns.  With all columns in one wave the pass needs over 256 registers
+// at 128 columns and runs at one wave per SIMD, where the matrix and vector units take turns; with all of dV in one wave and
+// all of dK in the other, dS's second term would be a branch (800 us for L = 8192 in bf16 in place of 490).  Heads
+// of 32 columns have no halves: there a wave sums its half of the queries, and the pair adds up at the end.
 constexpr int kFarWaves = 4, kFarRows = 16 * kFarWaves;  // sinks of a workgroup of the far pass
 // where the far pass's sums of dK (0) or dV (1) of key kj begin
 __device__ __forceinline__ int64_t far_row(const Args& a, int64_t bk, int kj, int which) {
@@ -611,9 +621,13 @@ __device__ __forceinline__ int64_t far_row(const Args& a, int64_t bk, int kj, in
 template <class T, int DP, int NW, bool FAR>
 __global__ __launch_bounds__(NW * 64) void dkv_kernel(Args a) {
     using P = Pass<T, DP, NW>;
-    constexpr int kPassed = 2 * 64 * sizeof(typename P::F);
+    using W = std::conditional_t<FAR, typename P::F, typename P::W>;  // (the far pass goes with the long ones)
+    constexpr bool kHalves = DP > 32;
+    constexpr int N = kHalves ? P::NFT / 2 : 1;
+    constexpr int kP = 64 * sizeof(W), kS = 64 * sizeof(typename P::S);  // bytes of a wave's P, dS of a k step
+    constexpr int kPassed = kHalves ? 2 * kP + 2 * kS : 64 * sizeof(floatx16);
     __shared__ __attribute__((aligned(16))) char lds[P::kBytes];
-    __shared__ __attribute__((aligned(16))) char exchange[NW * kPassed];  // P or dS of a wave's half
+    __shared__ __attribute__((aligned(16))) char exchange[NW * kPassed];  // P, dS of a wave's half; or a sum
     __shared__ __attribute__((aligned(16))) float meta[3][kTS];  // maximum, 1 / sum, D of the tile's queries
     uint32_t item;
     if (!item_of(a, item)) return;
@@ -631,8 +645,9 @@ __global__ __launch_bounds__(NW * 64) void dkv_kernel(Args a) {
     typename P::F K[P::KS], V[P::KS];
     P::stationary(K, live ? a.k.at<T>(b, kh) + kj * a.k.st : nullptr, h, a.dim);
     P::stationary(V, live ? a.v.at<T>(b, kh) + kj * a.v.st : nullptr, h, a.dim);
-    floatx16 y[P::NFT];
-    P::clear(y);
+    floatx16 yv[N], yk[N];
+    P::clear(yv), P::clear(yk);
+    const int first = kHalves ? role * N : 0;
     const float c = a.scale * kLog2e;
     const QueryTiles near(a, block * NW * 16 / a.near_rows * a.near_rows, a.near_rows);
     // the near tiles, or those beside them: [0, lo) without causal, and [hi, all)
@@ -672,7 +687,7 @@ __global__ __launch_bounds__(NW * 64) void dkv_kernel(Args a) {
         auto seen_of = [&](int sub) {
             return any && (uint32_t)(queries >> (32 * sub)) ? block_seen(a, q0 + 32 * sub, w0) : 0;
         };
-        const int seen = seen_of(role), theirs = seen_of(role ^ 1);
+        const int seen = seen_of(role), theirs = kHalves ? seen_of(role ^ 1) : 0;
         if (seen) {
             floatx16 x = P::score(lds, 0, role, K);
             floatx16 dp = P::score(lds, 1, role, V);
@@ -688,27 +703,61 @@ __global__ __launch_bounds__(NW * 64) void dkv_kernel(Args a) {
                 x[e] = __builtin_amdgcn_exp2f(fmaf(x[e], c, -m[r])) * m[kTS + r];
                 dp[e] = x[e] * (dp[e] - m[2 * kTS + r]);
             }
-            // (one path for both waves: a branch for each had the pass spill)
-            P::pass_on(mine, role ? x : dp);
-            P::template gather_as<typename P::F>(lds, role ^ 1, role, role ? dp : x, y);
+#pragma unroll
+            for (int s2 = 0; s2 < 2; ++s2) {
+                const auto w = P::template weights_of<W>(x, s2);
+                if constexpr (kHalves) P::pass_on(mine + s2 * kP, w);
+                P::gather(lds, 1, role, s2, first, w, yv);
+            }
+#pragma unroll
+            for (int s2 = 0; s2 < 2; ++s2) {
+                const auto w = P::template weights_of<typename P::S>(dp, s2);
+                if constexpr (kHalves) P::pass_on(mine + 2 * kP + s2 * kS, w);
+                P::gather(lds, 0, role, s2, first, w, yk);
+            }
         }
+        if constexpr (!kHalves) continue;
         __syncthreads();
-        if (theirs) P::gather_passed(other, lds, role ^ 1, role ^ 1, y);
+        if (theirs) {
+#pragma unroll
+            for (int s2 = 0; s2 < 2; ++s2)
+                P::gather(lds, 1, role ^ 1, s2, first, P::template passed<W>(other + s2 * kP), yv);
+#pragma unroll
+            for (int s2 = 0; s2 < 2; ++s2)
+                P::gather(lds, 0, role ^ 1, s2, first, P::template passed<typename P::S>(other + 2 * kP + s2 * kS), yk);
+        }
+    }
+    if constexpr (!kHalves) {  // the first wave takes dV, the second dK
+        floatx16 *give = (floatx16*)exchange + wave * 64 + lane, *take = (floatx16*)exchange + (wave ^ 1) * 64 + lane;
+        __syncthreads();
+        *give = role ? yv[0] : yk[0];
+        __syncthreads();
+        yv[0] = (role ? yk[0] : yv[0]) + *take;
     }
     using PF = Pass<float, DP, NW>;
-    const float scale = role ? a.scale : 1.f;
+    // f(dK?, the sum, its first column): what of the two rows this wave holds
+    auto each = [&](auto f) {
+        if (kHalves || !role) f(0, yv, 32 * first);
+        if (kHalves) f(1, yk, 32 * first);
+        else if (role) f(1, yv, 0);
+    };
     if (FAR || pieces > 1) {  // slab (key head, block, piece): dK and dV of the block's rows, zeros where there is nothing
-        PF::write_row((FAR ? a.far_part : a.part) +
-                          (((int64_t)item * 2 + (role ^ 1)) * NW * 16 + (wave >> 1) * 32 + r32) * a.dim,
-                      y, scale, h, a.dim);
+        each([&](int is_k, auto& y, int col) {
+            PF::write_row((FAR ? a.far_part : a.part) +
+                              (((int64_t)item * 2 + !is_k) * NW * 16 + (wave >> 1) * 32 + r32) * a.dim + col,
+                          y, is_k ? a.scale : 1.f, h, a.dim - col);
+        });
         return;
     }
     if (kj >= a.seq_len) return;
-    if (w0 < kFarRows * a.far_groups)  // the far pass's sums, added up in its first slab (0 for rows that are no sinks)
-        P::add_row(a.far_part + far_row(a, bk, kj, role ^ 1), y, 1.f / scale, h, a.dim);
-    if (!live) P::clear(y);
-    const Tensor& t = role ? a.dk : a.dv;
-    P::write_row(t.at<T>(b, kh) + kj * t.st, y, scale, h, a.dim);
+    each([&](int is_k, auto& y, int col) {
+        const float f = is_k ? a.scale : 1.f;
+        if (w0 < kFarRows * a.far_groups)  // the far pass's sums, added up in its first slab (0 for rows that are no sinks)
+            P::add_row(a.far_part + far_row(a, bk, kj, !is_k) + col, y, 1.f / f, h, a.dim - col);
+        if (!live) P::clear(y);
+        const Tensor& t = is_k ? a.dk : a.dv;
+        P::write_row(t.at<T>(b, kh) + kj * t.st + col, y, f, h, a.dim - col);
+    });
 }
 
 // the far pass's slabs of a group of sinks added up in the first, in order, 4 columns a thread
@@ -763,14 +812,24 @@ int waves_kv(int64_t seq_len, int dtype, int dp) {  // (two to 32 rows)
     return seq_len <= 64 || dp == 32 || (dtype == kF32 && dp == 128) ? 4 : 8;
 }
 
-// pieces of the dK, dV passes: as many as it takes to give every CU a workgroup, each at least 6 tiles long (near) or 4
-void plan_kv(Args& a, int64_t batch, int nw) {
+// Pieces of the dK, dV passes.  Near: those that end first when the card takes its workgroups in rounds of `slots` and one
+// costs its steps and about 3 more (its keys, its sums; 4 with the rows it leaves to be added); at least 4 steps each.
+// 290 blocks in one piece are two rounds, the second nearly empty: 29 sequences of 1181, window 307 to both sides, 128
+// columns in bf16 take 292 us, in 4 pieces 254.  Far: as many as give every CU two workgroups, of at least 4 tiles.
+void plan_kv(Args& a, int64_t batch, int dtype) {
+    const int dp = padded_dim(a.dim), nw = waves_kv(a.seq_len, dtype, dp);
+    const int64_t slots = 256 * (nw == 8 || (dtype == kF32 && dp > 32) ? 1 : 2);  // (by the waves that registers allow)
     a.near_rows = nw * 16;
     a.blocks = (a.seq_len + a.near_rows - 1) / a.near_rows;
     const int64_t have = batch * a.kv_heads, all = (a.seq_len + kTS - 1) / kTS;
     const int64_t reach = std::min<int64_t>(a.seq_len, a.near_rows + (int64_t)a.window * (a.causal ? 1 : 2));
-    a.near_pieces = (int)std::max<int64_t>(
-        1, std::min<int64_t>({256 / (have * a.blocks), (reach + kTS - 1) / kTS * a.group / 6, 64}));
+    const int64_t steps = (reach + kTS - 1) / kTS * a.group;
+    a.near_pieces = 1;
+    int64_t best = INT64_MAX;
+    for (int p = 1; p <= 64 && (p == 1 || steps / p >= 4); ++p) {
+        const int64_t rounds = (have * a.blocks * p + slots - 1) / slots, cost = rounds * ((steps + p - 1) / p + 3 + (p > 1));
+        if (cost < best) best = cost, a.near_pieces = p;
+    }
     int64_t most = 0;  // tiles beside the near pass's, of the block that has the most
     for (int k0 = 0; k0 < a.sinks; k0 += a.near_rows) {
         const QueryTiles t(a, k0, a.near_rows);
@@ -865,7 +924,7 @@ ASME_API int64_t asme_window_attention_bwd_workspace(int64_t batch, int64_t head
                                                      int dtype) {
     if (!dtype_ok(dtype) || !sizes_ok(batch, heads, kv_heads, seq_len, head_dim, window, sinks)) return 0;
     Args a = make_args(batch, heads, kv_heads, seq_len, head_dim, window, sinks, causal, 1.f, nullptr);
-    plan_kv(a, batch, waves_kv(seq_len, dtype, padded_dim(head_dim)));
+    plan_kv(a, batch, dtype);
     return ((batch * heads * seq_len + 3) / 4 * 4 + slab_floats(a, batch) + far_floats(a, batch)) * 4;
 }
 
@@ -908,7 +967,7 @@ ASME_API int asme_window_attention_bwd(const void* q, const void* k, const void*
     const int64_t key_heads = batch * kv_heads;
     Args aq = a;
     aq.blocks = (int)((seq_len + nq * 32 - 1) / (nq * 32));
-    plan_kv(a, batch, nw);
+    plan_kv(a, batch, dtype);
     a.far_part = a.part + slab_floats(a, batch);
     const int64_t q_items = batch * heads * aq.blocks, k_items = key_heads * a.blocks * a.near_pieces;
     ASME_CHECK_ARG(q_items + 8 < (1ll << 31) && k_items + 8 < (1ll << 31) &&
