@@ -355,8 +355,13 @@ class TransformerLayer(nn.Module):
             ops.window_cache_fill(*caches.layers[i], k, v, caches.lengths, sinks=att.sinks)
             return att.attend(qkv, key_valid, True, 0.0)
 
-        caches.lengths.copy_(key_valid.sum(1))
-        caches.most = x.shape[1]
+        held = key_valid != 0
+        lengths = held.sum(1)
+        first = torch.arange(x.shape[1], device=x.device) < lengths[:, None]
+        caches.most, stray = torch.stack([lengths.amax(), (held != first).sum()]).tolist()
+        if stray:
+            raise ValueError("prefill takes right-padded prompts: a position behind padding is valid")
+        caches.lengths.copy_(lengths)
         return self._run(x, attend)
 
     def step(self, x: torch.Tensor, caches: WindowCaches) -> torch.Tensor:

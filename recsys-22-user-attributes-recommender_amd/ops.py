@@ -1852,6 +1852,8 @@ def _check_cache(cache_k, cache_v, sinks: int):
                          "sinks + window, head_dim)")
     if cache_k.shape[3] not in _HEAD_DIMS:
         raise ValueError(f"head_dim {cache_k.shape[3]}: expected one of {_HEAD_DIMS}")
+    if cache_k.shape[1] < 1:
+        raise ValueError("caches of no heads")
     if not 0 <= sinks < cache_k.shape[2]:
         raise ValueError(f"sinks {sinks}: expected 0 <= sinks < {cache_k.shape[2]} slots")
     _dtype_code(cache_k)

@@ -125,6 +125,22 @@ def test_decode_gives_what_the_whole_history_gives(asme, dev, window, sinks, gat
         m.decode(extra[0][:2], caches)
 
 
+def test_prompts_padded_to_the_models_length(asme, dev):
+    """how far decode() goes is the longest history's matter, not its padding's; padding in front is refused"""
+    m = model(asme, attention_window=5, attention_sinks=1).eval()
+    seq, lengths = histories(asme, 4, 9, 5)
+    whole = torch.zeros(4, L, dtype=torch.int64, device=dev)
+    whole[:, :9] = seq.sequence
+    mask = (torch.arange(L) < lengths[:, None]).cuda()
+    item = torch.full((4,), 3, dtype=torch.int64, device=dev)
+    want = m.decode(item, m.prefill(seq)[1])
+    rep, caches = m.prefill(asme.InputSequence(whole, mask))
+    assert caches.most == int(lengths.max()) < L
+    assert torch.equal(m.decode(item, caches), want)
+    with pytest.raises(ValueError, match="right-padded"):
+        m.prefill(asme.InputSequence(whole.flip(1), mask.flip(1)))
+
+
 def cloze_batch(asme, b, seed, users=False):
     seq, lengths = histories(asme, b, L, seed, shortest=4)
     g = torch.Generator().manual_seed(seed + 1)

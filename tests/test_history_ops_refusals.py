@@ -48,7 +48,8 @@ def test_window_cache_refusals(asme):
     ops = asme.ops
     c, n = f32(2, 2, 10, 32), torch.zeros(2, dtype=torch.int64)
     q, k = f32(2, 4, 32), f32(2, 2, 32)
-    for bad in ((f32(2, 10, 32), f32(2, 10, 32)), (c, f32(2, 2, 9, 32)), (f32(2, 2, 10, 24), f32(2, 2, 10, 24))):
+    for bad in ((f32(2, 10, 32), f32(2, 10, 32)), (c, f32(2, 2, 9, 32)), (f32(2, 2, 10, 24), f32(2, 2, 10, 24)),
+                (f32(2, 0, 10, 32), f32(2, 0, 10, 32))):
         with pytest.raises(ValueError):
             ops.window_attention_step(q, k, k, *bad, n)
     for sinks in (-1, 10, 11):
