@@ -813,8 +813,8 @@ int waves_kv(int64_t seq_len, int dtype, int dp) {  // (two to 32 rows)
 }
 
 // Pieces of the dK, dV passes.  Near: those that end first when the card takes its workgroups in rounds of `slots` and one
-// costs its steps and about 3 more (its keys, its sums; 4 with the rows it leaves to be added); at least 4 steps each.
-// 290 blocks in one piece are two rounds, the second nearly empty: 29 sequences of 1181, window 307 to both sides, 128
+// costs its steps and about 3 more (its keys, its sums; 4 with the rows it leaves to be added); at least 4 steps each, at most
+// 8 rounds (the partial rows' memory).  290 blocks in one piece are two rounds, the second nearly empty: 29 sequences of 1181, window 307 to both sides, 128
 // columns in bf16 take 292 us, in 4 pieces 254.  Far: as many as give every CU two workgroups, of at least 4 tiles.
 void plan_kv(Args& a, int64_t batch, int dtype) {
     const int dp = padded_dim(a.dim), nw = waves_kv(a.seq_len, dtype, dp);
@@ -826,7 +826,7 @@ void plan_kv(Args& a, int64_t batch, int dtype) {
     const int64_t steps = (reach + kTS - 1) / kTS * a.group;
     a.near_pieces = 1;
     int64_t best = INT64_MAX;
-    for (int p = 1; p <= 64 && (p == 1 || steps / p >= 4); ++p) {
+    for (int p = 1; p == 1 || (p <= 64 && steps / p >= 4 && have * a.blocks * p <= 8 * slots); ++p) {
         const int64_t rounds = (have * a.blocks * p + slots - 1) / slots, cost = rounds * ((steps + p - 1) / p + 3 + (p > 1));
         if (cost < best) best = cost, a.near_pieces = p;
     }
