@@ -13,9 +13,11 @@
 //   of the mean as well: the 2 n V elements that any schedule has to move.  The backward has the upstream factor left to
 //   apply, which costs nothing where it is 1 and 2 n V more where it is not: a loss that is one part of another takes its
 //   weight w here.
-// Rows are split over workgroups when there
-// are fewer rows than the chip needs workgroups; the splits' (maximum, sum) pairs are merged in a fixed order, so results
-// do not depend on the schedule.  Statistics, probabilities and the loss are fp32; the gradient is rounded once, on store.
+// Rows are split over workgroups when there are fewer rows than the chip needs workgroups; the splits' (maximum, sum) pairs
+// are merged in a fixed order, so results do not depend on the schedule.  Statistics, probabilities and the loss are fp32;
+// the gradient is rounded once, on store.
+// Measured: together, 8192 x 26747 fp32 with lists of 50, 372 us forward and backward -- 1758 MB at 4.7 TB/s, what a copy
+// reaches on this card; apart, 580 us.  64 x 10007 bf16: 30 us of kernels, of 110 that the calls and autograd take.
 #include "elem.h"
 
 using namespace asme;
@@ -446,8 +448,8 @@ __global__ __launch_bounds__(kThreads) void grad_kernel(const T* __restrict__ lo
 constexpr int64_t kOneGroupRows = 256;  // up to here one workgroup finishes the rows and their mean
 int64_t finish_groups(int64_t n) { return n <= kOneGroupRows ? 1 : (n + 15) / 16; }
 
-// the rows that a workgroup holds, where there are enough of them to fill the chip (two workgroups a CU; 424 us for 8192 x 26747 fp32 at 1024 threads of 64 registers, which
-// spilled, 355 at 512 of 128)
+// the rows that a workgroup holds, where there are enough of them to fill the chip (two workgroups a CU; 424 us for
+// 8192 x 26747 fp32 at 1024 threads of 64 registers, which spilled, 355 at 512 of 128)
 bool together(int64_t n, int64_t V, int dtype) {
     return n >= 512 && V >= 4096 && V <= (int64_t)kRowThreads * kMostVecs * (dtype == kF32 ? 4 : 8);
 }

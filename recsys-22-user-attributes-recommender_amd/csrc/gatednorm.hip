@@ -14,6 +14,8 @@
 // thread (16 .. 1024 threads: a row's sums are lane moves within a wave, and one LDS exchange beyond it), and the next row
 // is on its way during its sums.  Weights stay in registers over a workgroup's rows.  Column sums: registers
 // over a workgroup's rows, then partial rows summed in a fixed order -- no atomics.
+// Measured (forward + backward): 16384 x 4096 bf16, gate per channel, 120 + 215 us for 403 + 671 MB (3.2 TB/s);
+// 204800 x 128 fp32, gate per sequence, 81 + 144 us for 839 MB in all (3.7 TB/s).
 #include "elem.h"
 
 using namespace asme;

@@ -24,10 +24,14 @@
 // (7 products for the 5 of a single pass), so no sum depends on the order of atomics.
 //
 // fp32 tensors are split exactly into three bf16 planes on the way into LDS and the products kept to fp32 level by six
-// MFMAs (common.h, bf16x6); bf16 tensors take one, P rounded to bf16 for its second product (at most 2^-8 of
-// each term, the size of the output's own rounding, averaged over the row; Pass::W).  dS, whose terms cancel (a row of it sums to
-// 0), goes into dQ and dK as two bf16 terms: rounded to one, they were off by 1.5 to 2 times their own rounding.  Scores,
-// softmax statistics and all sums are fp32.
+// MFMAs (common.h, bf16x6); bf16 tensors take one, P rounded to bf16 for its second product (at most 2^-8 of each term, the
+// size of the output's own rounding, averaged over the row; Pass::W).  dS, whose terms cancel (a row of it sums to 0), goes
+// into dQ and dK as two bf16 terms: rounded to one, they were off by 1.5 to 2 times their own rounding.  Scores, softmax
+// statistics and all sums are fp32.
+// Measured: 2 sequences of 8192, 16 heads on 4, 128 columns, window 1024 and 4 sinks, causal, bf16: forward 240 us (540
+// TFLOP/s of visible pairs, half of what the library's large product reaches), dQ 370 (520), dK and dV 475 + 50 for what
+// queries outside the window see of the sinks (490).  Counters: forward MFMA busy 26 %, vector units 32 %, LDS 18 %, waves
+// waiting 42 % of their cycles; no bank conflicts.
 #include "elem.h"
 
 using namespace asme;
@@ -594,7 +598,12 @@ __global__ __launch_bounds__(NW * 64) void dq_kernel(Args a) {
 // of.  What a sink is seen by beyond them is the far pass's.
 struct QueryTiles {
     int lo, hi;
+    // without a far pass, a block with sinks takes all
     __host__ __device__ QueryTiles(const Args& a, int k0, int rows) {
+        if (a.far_groups == 0 && k0 < a.sinks) {
+            lo = a.causal ? k0 / kTS : 0, hi = (a.seq_len + kTS - 1) / kTS;
+            return;
+        }
         const int64_t k1 = k0 + rows < a.seq_len ? k0 + rows : a.seq_len, end = k1 - 1 + a.window;
         const int first = a.causal ? k0 : k0 - a.window + 1;
         lo = first > 0 ? first / kTS : 0;
@@ -813,9 +822,12 @@ int waves_kv(int64_t seq_len, int dtype, int dp) {  // (two to 32 rows)
 }
 
 // Pieces of the dK, dV passes.  Near: those that end first when the card takes its workgroups in rounds of `slots` and one
-// costs its steps and about 3 more (its keys, its sums; 4 with the rows it leaves to be added); at least 4 steps each, at most
-// 8 rounds (the partial rows' memory).  290 blocks in one piece are two rounds, the second nearly empty: 29 sequences of 1181, window 307 to both sides, 128
-// columns in bf16 take 292 us, in 4 pieces 254.  Far: as many as give every CU two workgroups, of at least 4 tiles.
+// costs its steps and about 3 more (its keys, its sums; 4 with the rows it leaves to be added); at least 4 steps each, at
+// most 8 rounds (the partial rows' memory).  290 blocks in one piece are two rounds, the second nearly empty: 29 sequences
+// of 1181, window 307 to both sides, 128 columns in bf16 take 292 us, in 4 pieces 254.  Far: as many as give every CU two
+// workgroups, of at least 4 tiles; none where kAlong tiles or fewer are left to it, which the near pass takes along (256
+// ragged sequences of up to 200, 2 heads of 64, window 64, fp32: 126 us with a far pass, 105 without).
+constexpr int kAlong = 4;
 void plan_kv(Args& a, int64_t batch, int dtype) {
     const int dp = padded_dim(a.dim), nw = waves_kv(a.seq_len, dtype, dp);
     const int64_t slots = 256 * (nw == 8 || (dtype == kF32 && dp > 32) ? 1 : 2);  // (by the waves that registers allow)
@@ -823,6 +835,13 @@ void plan_kv(Args& a, int64_t batch, int dtype) {
     a.blocks = (a.seq_len + a.near_rows - 1) / a.near_rows;
     const int64_t have = batch * a.kv_heads, all = (a.seq_len + kTS - 1) / kTS;
     const int64_t reach = std::min<int64_t>(a.seq_len, a.near_rows + (int64_t)a.window * (a.causal ? 1 : 2));
+    a.far_groups = (a.sinks + kFarRows - 1) / kFarRows;
+    int64_t most = 0;  // tiles beside the near pass's, of the block that has the most
+    for (int k0 = 0; k0 < a.sinks; k0 += a.near_rows) {
+        const QueryTiles t(a, k0, a.near_rows);
+        most = std::max<int64_t>(most, all - t.hi + (a.causal ? 0 : t.lo));
+    }
+    if (most * a.group <= kAlong) a.far_groups = 0;
     const int64_t steps = (reach + kTS - 1) / kTS * a.group;
     a.near_pieces = 1;
     int64_t best = INT64_MAX;
@@ -830,12 +849,6 @@ void plan_kv(Args& a, int64_t batch, int dtype) {
         const int64_t rounds = (have * a.blocks * p + slots - 1) / slots, cost = rounds * ((steps + p - 1) / p + 3 + (p > 1));
         if (cost < best) best = cost, a.near_pieces = p;
     }
-    int64_t most = 0;  // tiles beside the near pass's, of the block that has the most
-    for (int k0 = 0; k0 < a.sinks; k0 += a.near_rows) {
-        const QueryTiles t(a, k0, a.near_rows);
-        most = std::max<int64_t>(most, all - t.hi + (a.causal ? 0 : t.lo));
-    }
-    a.far_groups = most > 0 ? (a.sinks + kFarRows - 1) / kFarRows : 0;
     a.far_pieces = a.far_groups ? (int)std::max<int64_t>(
         1, std::min<int64_t>({512 / (have * a.far_groups), most * a.group / 4, 64})) : 1;
 }

