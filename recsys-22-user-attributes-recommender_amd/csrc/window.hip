@@ -812,10 +812,14 @@ __global__ __launch_bounds__(256) void add_pieces_kernel(Args a, int64_t total) 
 int padded_dim(int64_t dim) { return dim <= 32 ? 32 : (int)dim; }
 
 // Waves (of 32 stationary rows) per workgroup: eight share a streamed tile's way through LDS, at 256 registers each; four
-// (512 registers) where a pass's fragments and sums need more; two where the sequence has no more rows.
-int waves(int64_t seq_len, int dtype, int dp) {
-    if (seq_len <= 64) return 2;
-    return dp == 32 || (dtype == kF32 && dp == 128) ? 4 : 8;
+// (512 registers) where a pass's fragments and sums need more; two where the sequence has no more rows; half of them, twice
+// if need be, where each workgroup still has a CU of its own (one sequence of 2000, 4 heads of 128 columns, window 256,
+// bf16: forward 30 us, dQ 41 in 32 workgroups of eight waves, 23 and 25 in 126 of two; beyond that the tiles' way costs
+// more: 3 of 2049, 6 heads of 64, fp32, 63 us in 162 of eight, 70 in 306 of four).
+int waves(int64_t seqs, int64_t seq_len, int dtype, int dp) {  // seqs: sequences and heads
+    int w = seq_len <= 64 ? 2 : dp == 32 || (dtype == kF32 && dp == 128) ? 4 : 8;
+    while (w > 2 && seqs * ((seq_len + 16 * w - 1) / (16 * w)) <= 256) w /= 2;
+    return w;
 }
 int waves_kv(int64_t seq_len, int dtype, int dp) {  // (two to 32 rows)
     return seq_len <= 64 || dp == 32 || (dtype == kF32 && dp == 128) ? 4 : 8;
@@ -919,7 +923,7 @@ ASME_API int asme_window_attention_fwd(const void* q, const void* k, const void*
     ASME_CHECK_ARG(!out_low || (dtype == kBF16 && ((uintptr_t)out_low & 15) == 0),
                    "asme_window_attention_fwd: out_low is of bf16, 16-byte aligned");
     a.state = (float2*)state, a.out_low = out_low;
-    const int dp = padded_dim(head_dim), nw = waves(seq_len, dtype, dp);
+    const int dp = padded_dim(head_dim), nw = waves(batch * heads, seq_len, dtype, dp);
     a.blocks = (int)((seq_len + nw * 32 - 1) / (nw * 32));
     const int64_t items = batch * heads * a.blocks;
     a.items = (uint32_t)items, a.per_xcd = (uint32_t)((items + 7) / 8);
@@ -970,7 +974,7 @@ ASME_API int asme_window_attention_bwd(const void* q, const void* k, const void*
     a.state = (float2*)const_cast<float*>(state), a.out_low = const_cast<void*>(out_low);
     a.delta = (float*)workspace;
     a.part = a.delta + (batch * heads * seq_len + 3) / 4 * 4;
-    const int dp = padded_dim(head_dim), nq = waves(seq_len, dtype, dp), nw = waves_kv(seq_len, dtype, dp);
+    const int dp = padded_dim(head_dim), nq = waves(batch * heads, seq_len, dtype, dp), nw = waves_kv(seq_len, dtype, dp);
     hipStream_t s = (hipStream_t)stream;
     // the whole grid of `items` workgroups of a pass
     auto grid = [](Args& x, int64_t items) {
