@@ -152,9 +152,9 @@ struct Pass {
     using F = Frag<NP>;
     static constexpr int SP = NP == 1 ? 2 : NP;  // planes of dS as a factor
     using S = Frag<SP>;
-    // P as a factor: of bf16 in one term where the matrix and vector units bound the pass (eight waves; two cost 295 us for
-    // 248 forward at L = 8192 and 128 columns, dK and dV 616 for 506); in two where they do not, among them the shortest
-    // sequences, whose few terms' roundings do not average out
+    // P as a factor: of bf16 in one term where a workgroup has eight waves (long sequences of 64 or 128 columns: two cost
+    // 295 us for 248 forward at L = 8192 and 128 columns, dK and dV 616 for 506); in two elsewhere, where sequences are short
+    // and their few terms' roundings do not average out (a tenth of the time for long sequences of 32 columns)
     using W = Frag<NW < 8 ? SP : NP>;
 
     // The compiler keeps the LDS addresses of a tile's reads and writes, which are the same in every round, in registers:
