@@ -252,7 +252,8 @@ class SASRecModel(TransformerEncoderModel):
 
     @torch.no_grad()
     def decode(self, items: torch.Tensor, caches) -> torch.Tensor:
-        """the representation (B, d) of one more item (B,) per user; `caches` go on to it"""
+        """the representation (B, d) of one more item (B,) per user; `caches` go on to it.  (The replays of a captured step
+        are not counted: a position behind max_seq_len is refused only by a call from the host.)"""
         layer = self._servable()
         if items.shape != caches.lengths.shape:
             raise ValueError(f"items {tuple(items.shape)}: expected one for each of {caches.lengths.shape[0]} users")
