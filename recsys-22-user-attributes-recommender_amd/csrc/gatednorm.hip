@@ -13,7 +13,7 @@
 // again from res and y, in fp32, instead of being read back rounded).  A row is held in registers, one 16-byte vector a
 // thread (16 .. 1024 threads: a row's sums are lane moves within a wave, and one LDS exchange beyond it), and the next row
 // is on its way during its sums.  Weights stay in registers over a workgroup's rows.  Column sums: registers
-// over a workgroup's rows, then partial rows summed in a fixed order -- no atomics.
+// (LDS beyond 4096 columns) over a workgroup's rows, then partial rows summed in a fixed order -- no atomics.
 // Measured (forward + backward): 16384 x 4096 bf16, gate per channel, 120 + 215 us for 403 + 671 MB (3.2 TB/s);
 // 204800 x 128 fp32, gate per sequence, 81 + 144 us for 839 MB in all (3.7 TB/s).
 #include "elem.h"
@@ -48,9 +48,9 @@ struct Row {
     static constexpr int kThreads = TPR > 64 ? TPR : 256;
     static constexpr int kSlots = kThreads / TPR;  // rows at a time
     static constexpr int E = Elem<T>::V, kVecs = N / E;
-    // rows beyond 4096 values: the backward's weights and next row do not fit 128 registers beside its sums -- it reads
-    // them when they are due, and still spills some (4000 x 8192 fp32: 476 us forward and backward, 46 % of the bytes' time;
-    // 512 threads of 16 values and 256 registers took 562)
+    // rows beyond 4096 values: the backward's column sums of the weights' gradients are held in LDS (128 KiB, a thread's own
+    // vectors) and its rows read when they are due; beside them in 128 registers they spilled up to 173 values (forward and
+    // backward, 4000 x 8192 fp32: 473 us, 303 with the sums in LDS; 2 x 2000 x 8192 bf16, a gate a row: 546, 254)
     static constexpr bool kLean = TPR * N > 4096;
     typedef T Vec __attribute__((ext_vector_type(E)));
     typedef Vec AnyVec __attribute__((aligned(EVEN ? 16 : sizeof(T))));
@@ -258,15 +258,38 @@ __global__ __launch_bounds__(R::kThreads) void bwd_kernel(Args a) {
     const int t = threadIdx.x % R::TPRv, slot = R::kSlots > 1 ? threadIdx.x / R::TPRv : 0, D = a.D;
     const float inv_d = 1.f / (float)D, centre = a.rms ? 0.f : 1.f;
     float pw[kPer], pb[kPer], qw[kPer];
-    auto weights = [&]() {
-        R::load_f32(a.post_w, t, D, 1.f, pw);
-        R::load_f32(a.post_b, t, D, 0.f, pb);
-        R::load_f32(a.pre_w, t, D, 1.f, qw);
-    };
-    if (!R::kLean) weights();
-    float acc[4][kPer], gacc[kPer];
+    R::load_f32(a.post_w, t, D, 1.f, pw);
+    R::load_f32(a.post_b, t, D, 0.f, pb);
+    R::load_f32(a.pre_w, t, D, 1.f, qw);
+    float acc[4][R::kLean ? 1 : kPer], gacc[kPer];
+    __shared__ floatx4 far[R::kLean ? 4 * kPer / 4 * R::kThreads : 1];  // (a thread's own columns: no barrier)
+    // the sums k = 0 .. 3 of the thread's columns: f(i, so far) is the new one of value i
+    auto add = [&](int k, auto f) {
+        if constexpr (R::kLean) {
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) acc[0][i] = acc[1][i] = acc[2][i] = acc[3][i] = gacc[i] = 0.f;
+            for (int c = 0; c < kPer / 4; ++c) {
+                floatx4& p = far[(k * (kPer / 4) + c) * R::kThreads + threadIdx.x];
+                floatx4 v = p;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = f(4 * c + e, v[e]);
+                p = v;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) acc[k][i] = f(i, acc[k][i]);
+        }
+    };
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        if constexpr (R::kLean) {
+            for (int c = 0; c < kPer / 4; ++c)
+                far[(k * (kPer / 4) + c) * R::kThreads + threadIdx.x] = floatx4{0.f, 0.f, 0.f, 0.f};
+        } else {
+            for (int i = 0; i < kPer; ++i) acc[k][i] = 0.f;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) gacc[i] = 0.f;
     typename R::Raw raw_y, raw_s, raw_d, raw_z, raw_g;
     float4 next_st;
     // this thread's slot of the rows from `base` on (the last one again behind `end`)
@@ -290,7 +313,7 @@ __global__ __launch_bounds__(R::kThreads) void bwd_kernel(Args a) {
         for (int64_t base = begin; base < end; base += R::kSlots) {
             const bool live = base + slot < end;
             const int64_t row = live ? base + slot : end - 1;
-            if (R::kLean) weights(), fetch(base, end, group);
+            if (R::kLean) fetch(base, end, group);
             const float4 st = next_st;
             float y[kPer], s[kPer], d[kPer], g[kPer], dz[kPer];
             raw_y.get(t, D, y);
@@ -313,8 +336,11 @@ __global__ __launch_bounds__(R::kThreads) void bwd_kernel(Args a) {
 #pragma unroll
                 for (int i = 0; i < kPer; ++i) {
                     if (!live) dz[i] = 0.f;
-                    acc[2][i] = fmaf(dz[i], s[i], acc[2][i]);
-                    acc[3][i] += dz[i];
+                }
+                add(2, [&](int i, float v) { return fmaf(dz[i], s[i], v); });
+                add(3, [&](int i, float v) { return v + dz[i]; });
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) {
                     dz[i] *= qw[i];
                     v[0] = fmaf(dz[i], s[i], v[0]);
                     v[1] += dz[i];
@@ -342,10 +368,13 @@ __global__ __launch_bounds__(R::kThreads) void bwd_kernel(Args a) {
             for (int i = 0; i < kPer; ++i) {
                 if (R::col(t, i) >= D) d[i] = 0.f;
                 if (GATE == 2) gacc[i] = fmaf(d[i], fmaf(y[i], pw[i], pb[i]), gacc[i]);
-                const float db = GATE ? d[i] * g[i] : d[i];
-                acc[0][i] = fmaf(db, y[i], acc[0][i]);
-                acc[1][i] += db;
-                d[i] = db * pw[i];
+                if (GATE) d[i] *= g[i];
+            }
+            add(0, [&](int i, float v) { return fmaf(d[i], y[i], v); });
+            add(1, [&](int i, float v) { return v + d[i]; });
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                d[i] *= pw[i];
                 v[0] = fmaf(d[i], y[i], v[0]);
                 v[1] += d[i];
             }
@@ -370,9 +399,14 @@ __global__ __launch_bounds__(R::kThreads) void bwd_kernel(Args a) {
     }
     if (a.part)
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-            column_sums<R>(acc[k], t, slot, D, buf,
-                           [&](int j, float v) { a.part[((int64_t)blockIdx.x * 4 + k) * D + j] = v; });
+        for (int k = 0; k < 4; ++k) {
+            float v[kPer];
+#pragma unroll
+            for (int i = 0; i < kPer; ++i)
+                v[i] = R::kLean ? far[(k * (kPer / 4) + i / 4) * R::kThreads + threadIdx.x][i % 4] : acc[k][R::kLean ? 0 : i];
+            column_sums<R>(v, t, slot, D, buf,
+                           [&](int j, float x) { a.part[((int64_t)blockIdx.x * 4 + k) * D + j] = x; });
+        }
 }
 
 // out[g][j] = sum over m < rows of part[g * rows + m][j], j < width: 16 columns x 64 row lanes a workgroup, then the
@@ -422,8 +456,12 @@ void with_row(int64_t D, bool even, F&& f) {
         else if (D <= 128 * N) f(Row<T, 128, N, EVEN>{});
         else if (D <= 256 * N) f(Row<T, 256, N, EVEN>{});
         else if (EVEN || D <= 512 * N) f(Row<T, 512, N, EVEN>{});
-        else if (N == 4 && D <= 4096) f(Row<T, 1024, 4, false>{});
-        else f(Row<T, 1024, 8, false>{});
+        else {
+            if constexpr (N == 4) {
+                if (D <= 4096) return f(Row<T, 1024, 4, false>{});
+            }
+            f(Row<T, 1024, 8, false>{});
+        }
     };
     if (even && D % N == 0 && D <= 512 * N) pick(std::true_type{});
     else pick(std::false_type{});
