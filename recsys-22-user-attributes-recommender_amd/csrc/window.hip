@@ -392,12 +392,13 @@ __device__ __forceinline__ bool item_of(const Args& a, uint32_t& item) {
     return item < a.items;
 }
 
-// The streamed key tiles of queries [q0, q1): those of the sinks in front of the window's first tile, then the window's.
+// The streamed key tiles of queries [q0, q1): those of the sinks in front of the window's first tile, then the window's,
+// without causal up to the last sink where that lies beyond the window (every key in between is a sink).
 struct KeyTiles {
     int sink_tiles, lo, count;
     __device__ KeyTiles(const Args& a, int q0, int q1) {
         lo = max(0, q0 - a.window + 1) / kTS * kTS;
-        const int hi = a.causal ? q1 : (int)min((int64_t)a.seq_len, (int64_t)q1 - 1 + a.window);
+        const int hi = a.causal ? q1 : max(a.sinks, (int)min((int64_t)a.seq_len, (int64_t)q1 - 1 + a.window));
         sink_tiles = (min(a.sinks, lo) + kTS - 1) / kTS;
         count = sink_tiles + (hi - lo + kTS - 1) / kTS;
     }
