@@ -24,14 +24,16 @@
 // (7 products for the 5 of a single pass), so no sum depends on the order of atomics.
 //
 // fp32 tensors are split exactly into three bf16 planes on the way into LDS and the products kept to fp32 level by six
-// MFMAs (common.h, bf16x6); bf16 tensors take one, P rounded to bf16 for its second product (at most 2^-8 of each term, the
-// size of the output's own rounding, averaged over the row; Pass::W).  dS, whose terms cancel (a row of it sums to 0), goes
-// into dQ and dK as two bf16 terms: rounded to one, they were off by 1.5 to 2 times their own rounding.  Scores, softmax
-// statistics and all sums are fp32.
-// Measured: 2 sequences of 8192, 16 heads on 4, 128 columns, window 1024 and 4 sinks, causal, bf16: forward 240 us (540
-// TFLOP/s of visible pairs, half of what the library's large product reaches), dQ 370 (520), dK and dV 475 + 50 for what
-// queries outside the window see of the sinks (490).  Counters: forward MFMA busy 26 %, vector units 32 %, LDS 18 %, waves
-// waiting 42 % of their cycles; no bank conflicts.
+// MFMAs (common.h, bf16x6).  bf16 tensors take one, and two where a factor is formed here: P and dS go into O, dV, dQ and
+// dK as two bf16 terms (to 2^-16), whatever the sizes, so that an output is off by little beside its own rounding and a
+// sequence's does not depend on what else is in its batch.  P in one term doubled the square of O's and dV's error (0.0023
+// of the output in place of 0.0017; L = 8192 below: forward 246 us, dK and dV 500); dS in one, whose terms cancel (a row of
+// it sums to 0), put dQ and dK off by 1.5 to 2 times their rounding.  Scores, softmax statistics and all sums are fp32.
+// Measured: 2 sequences of 8192, 16 heads on 4, 128 columns, window 1024 and 4 sinks, causal, bf16: forward 285 us (450
+// TFLOP/s of visible pairs, 40 % of what the library's large product reaches), dQ 376 (510), dK and dV 587 + 52 for what
+// queries outside the window see of the sinks (400).  Counters (profiles/history_ops_counters.json), of forward, dQ and
+// dK / dV: MFMA busy 29, 29 and 27 %, vector units 36, 29 and 25 %, LDS 13, 13 and 22 %, waves waiting 37, 45 and 52 % of
+// their cycles; no bank conflicts.
 #include "elem.h"
 
 using namespace asme;
@@ -150,12 +152,8 @@ struct Pass {
     static constexpr int kImages = DP == 128 ? 2 : 1;
     static constexpr int kBytes = NP * kImages * kImage;
     using F = Frag<NP>;
-    static constexpr int SP = NP == 1 ? 2 : NP;  // planes of dS as a factor
+    static constexpr int SP = NP == 1 ? 2 : NP;  // planes of P and dS as factors
     using S = Frag<SP>;
-    // P as a factor: of bf16 in one term where a workgroup has eight waves (long sequences of 64 or 128 columns: two cost
-    // 295 us for 248 forward at L = 8192 and 128 columns, dK and dV 616 for 506); in two elsewhere, where sequences are short
-    // and their few terms' roundings do not average out (a tenth of the time for long sequences of 32 columns)
-    using W = Frag<NW < 8 ? SP : NP>;
 
     // The compiler keeps the LDS addresses of a tile's reads and writes, which are the same in every round, in registers:
     // faster by 10 % than forming them anew (L = 8192, bf16, 128 columns) where there are registers.  fp32 rows of 128
@@ -481,7 +479,7 @@ __global__ __launch_bounds__(NW * 64) void forward_kernel(Args a) {
             }
 #pragma unroll
             for (int s2 = 0; s2 < 2; ++s2)
-                P::gather(lds, 1, sub, s2, 0, P::template weights_of<typename P::W>(x, s2), y);
+                P::gather(lds, 1, sub, s2, 0, P::template weights_of<typename P::S>(x, s2), y);
         }
     }
     sum += __shfl_xor(sum, 32, 64);
@@ -631,11 +629,11 @@ __device__ __forceinline__ int64_t far_row(const Args& a, int64_t bk, int kj, in
 template <class T, int DP, int NW, bool FAR>
 __global__ __launch_bounds__(NW * 64) void dkv_kernel(Args a) {
     using P = Pass<T, DP, NW>;
-    using W = std::conditional_t<FAR, typename P::F, typename P::W>;  // (the far pass goes with the long ones)
+    using S = typename P::S;
     constexpr bool kHalves = DP > 32;
     constexpr int N = kHalves ? P::NFT / 2 : 1;
-    constexpr int kP = 64 * sizeof(W), kS = 64 * sizeof(typename P::S);  // bytes of a wave's P, dS of a k step
-    constexpr int kPassed = kHalves ? 2 * kP + 2 * kS : 64 * sizeof(floatx16);
+    constexpr int kS = 64 * sizeof(S);  // bytes of a wave's P or dS of a k step
+    constexpr int kPassed = kHalves ? 4 * kS : 64 * sizeof(floatx16);
     __shared__ __attribute__((aligned(16))) char lds[P::kBytes];
     __shared__ __attribute__((aligned(16))) char exchange[NW * kPassed];  // P, dS of a wave's half; or a sum
     __shared__ __attribute__((aligned(16))) float meta[3][kTS];  // maximum, 1 / sum, D of the tile's queries
@@ -715,14 +713,14 @@ __global__ __launch_bounds__(NW * 64) void dkv_kernel(Args a) {
             }
 #pragma unroll
             for (int s2 = 0; s2 < 2; ++s2) {
-                const auto w = P::template weights_of<W>(x, s2);
-                if constexpr (kHalves) P::pass_on(mine + s2 * kP, w);
+                const auto w = P::template weights_of<S>(x, s2);
+                if constexpr (kHalves) P::pass_on(mine + s2 * kS, w);
                 P::gather(lds, 1, role, s2, first, w, yv);
             }
 #pragma unroll
             for (int s2 = 0; s2 < 2; ++s2) {
-                const auto w = P::template weights_of<typename P::S>(dp, s2);
-                if constexpr (kHalves) P::pass_on(mine + 2 * kP + s2 * kS, w);
+                const auto w = P::template weights_of<S>(dp, s2);
+                if constexpr (kHalves) P::pass_on(mine + (2 + s2) * kS, w);
                 P::gather(lds, 0, role, s2, first, w, yk);
             }
         }
@@ -731,10 +729,10 @@ __global__ __launch_bounds__(NW * 64) void dkv_kernel(Args a) {
         if (theirs) {
 #pragma unroll
             for (int s2 = 0; s2 < 2; ++s2)
-                P::gather(lds, 1, role ^ 1, s2, first, P::template passed<W>(other + s2 * kP), yv);
+                P::gather(lds, 1, role ^ 1, s2, first, P::template passed<S>(other + s2 * kS), yv);
 #pragma unroll
             for (int s2 = 0; s2 < 2; ++s2)
-                P::gather(lds, 0, role ^ 1, s2, first, P::template passed<typename P::S>(other + 2 * kP + s2 * kS), yk);
+                P::gather(lds, 0, role ^ 1, s2, first, P::template passed<S>(other + (2 + s2) * kS), yk);
         }
     }
     if constexpr (!kHalves) {  // the first wave takes dV, the second dK

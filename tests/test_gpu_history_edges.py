@@ -6,7 +6,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_history_ops import check_window, rand
+from test_gpu_history_ops import check_window, near, rand, window64
 
 pytestmark = pytest.mark.gpu
 
@@ -46,3 +46,45 @@ def test_window_attention_with_many_sinks(asme, dev, dtype, b, n, h, kv, d, wind
     valid = ragged(b, n, 1) if padding else torch.ones(b, n, dtype=torch.bool)
     (q, k, v, dout), got = window_call(asme, dtype, b, n, h, kv, d, window, sinks, causal, valid if padding else None)
     check_window(got, dtype, q, k, v, dout, window, sinks, causal, valid, d ** -0.5, n)
+
+
+def check_close(got, dtype, q, k, v, dout, window, sinks, causal, valid, scale, n):
+    """check_window's counting for the accuracy that bf16 is meant to have: P, dS and the output that D is formed from are
+    each the sum of two bf16 terms.  The first leaves at most 2^-8 of the value and the second at most 2^-8 of that: 2^-16
+    = 2^8 u of each term in place of 2^16 u"""
+    res, sizes, terms, more = window64(q, k, v, dout, window, sinks, causal, valid, scale)
+    for x, ref, size, term, extra, name in zip(got, res, sizes, terms, more, ("out", "dq", "dk", "dv")):
+        room = size + (n / 16 + 32) * term
+        if dtype == torch.bfloat16:
+            room = room + 2.0 ** 8 * (term + extra)
+        near(x, ref, room, 1, name)
+
+
+# (waves of 32 queries a workgroup: eight for heads of 64 and bf16 heads of 128 and four else, halved while all workgroups
+# have a CU of their own)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("b,n,h,kv,d,window,sinks,causal", [
+    (33, 200, 4, 2, 64, 4, 2, True), (33, 200, 4, 2, 64, 33, 5, False), (33, 200, 4, 2, 128, 64, 3, True),
+    (33, 200, 4, 1, 128, 5, 66, False), (33, 201, 4, 4, 32, 16, 1, True), (70, 135, 2, 1, 16, 7, 0, False),
+    (25, 160, 4, 2, 64, 21, 1, True),                                      # four waves of heads of 64
+    (3, 700, 4, 2, 64, 50, 9, True), (1, 1100, 4, 1, 128, 300, 2, True),   # two; the second in pieces of key blocks
+    (2, 1200, 4, 2, 128, 3, 200, True)])                                   # sinks far behind the window
+def test_window_attention_in_workgroups_of_every_size(asme, dev, dtype, b, n, h, kv, d, window, sinks, causal):
+    valid = ragged(b, n, 5)
+    (q, k, v, dout), got = window_call(asme, dtype, b, n, h, kv, d, window, sinks, causal, valid, seed=20)
+    check_window(got, dtype, q, k, v, dout, window, sinks, causal, valid, d ** -0.5, n)
+    check_close(got, dtype, q, k, v, dout, window, sinks, causal, valid, d ** -0.5, n)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,h,d,window,sinks,causal", [(200, 4, 64, 40, 2, True), (130, 4, 128, 9, 1, False),
+                                                       (300, 2, 32, 100, 5, True)])
+def test_a_sequence_does_not_depend_on_its_batch(asme, dev, dtype, n, h, d, window, sinks, causal):
+    """a workgroup's size follows from the batch; what a query sees, the order of its sums and their roundings do not"""
+    valid = torch.ones(130, n, dtype=torch.bool)
+    valid[:, n - 3:] = False
+    (q, k, v, dout), (out, dq, _, _) = window_call(asme, dtype, 130, n, h, h, d, window, sinks, causal, valid)
+    one = [t[7:8].detach().clone().requires_grad_() for t in (q, k, v)]
+    alone = asme.ops.window_attention(*one, window, sinks=sinks, causal=causal, valid=valid[7:8].cuda())
+    (grad,) = torch.autograd.grad(alone, one[0], dout[7:8])
+    assert torch.equal(alone[0], out[7]) and torch.equal(grad[0], dq[7])
