@@ -472,12 +472,17 @@ int asme_distill_xent_fwd(const void* logits, int64_t ld, int64_t n, int64_t V, 
                           float* prob, void* workspace, int64_t ws_bytes, float* out, void* stream);
 /* The forward with the gradient of the mean written as well, 2 n V elements moved in all (n >= 512 rows that a workgroup
  * holds, 4096 to 32768 fp32 or 65536 bf16 items: *_grad_supported): dlogits (n, V) contiguous, rows aligned like those of
- * logits.  What is left of the backward is the upstream factor: asme_scale_by(dlogits, n * V, dtype, dloss). */
+ * logits.  What is left of the backward is the upstream factor: asme_scale_by(dlogits, n * V, dtype, dloss), which rounds
+ * once more, or asme_distill_xent_bwd_again, which forms the gradient anew from the logits where dloss is not 1 (the same
+ * bytes moved, one rounding). */
 int asme_distill_xent_grad_supported(int64_t n, int64_t V, int dtype);
 int64_t asme_distill_xent_grad_workspace(int64_t n);
 int asme_distill_xent_fwd_grad(const void* logits, int64_t ld, int64_t n, int64_t V, const int64_t* ids,
                                const float* teacher, int64_t top, float temperature, float weight, int dtype,
                                float* state, float* prob, void* dlogits, void* workspace, int64_t ws_bytes, float* out, void* stream);
+int asme_distill_xent_bwd_again(const void* logits, int64_t ld, int64_t n, int64_t V, const int64_t* ids, int64_t top,
+                                float temperature, float weight, int dtype, const float* state, const float* prob,
+                                const float* stats, const float* dloss, void* dlogits, void* stream);
 /* x[i] *= factor[0], i < n (x 16-byte aligned); returns at once on the device where the factor is 1 */
 int asme_scale_by(void* x, int64_t n, int dtype, const float* factor, void* stream);
 /* dlogits (rows ld_d apart; not logits itself) = dloss[0] times the gradient; rows without a list: 0.  stats = the

@@ -130,6 +130,7 @@ SIGNATURES = {
     "asme_distill_xent_fwd_grad": [p, i64, i64, i64, p, p, i64, f32, f32, i32, p, p, p, p, i64, p, p],
     "asme_scale_by": [p, i64, i32, p, p],
     "asme_distill_xent_bwd": [p, i64, i64, i64, p, i64, f32, f32, i32, p, p, p, p, p, i64, p],
+    "asme_distill_xent_bwd_again": [p, i64, i64, i64, p, i64, f32, f32, i32, p, p, p, p, p, p],
     "asme_gated_residual_norm_fwd": [p, p, p, i64, p, p, p, p, i64, i64, f32, f32, i32, i32, p, p, p, p],
     "asme_gated_residual_norm_bwd_workspace": [i64, i64, i64],
     "asme_gated_residual_norm_bwd": [p, p, p, i64, p, p, p, i64, i64, f32, i32, i32, p, p, p, p, p, p, p, p, i64, p],

@@ -12,10 +12,11 @@
 //   together (asme_distill_xent_fwd_grad): a workgroup holds its row in registers, so that the forward writes the gradient
 //   of the mean as well: the 2 n V elements that any schedule has to move.  The backward has the upstream factor left to
 //   apply, which costs nothing where it is 1 and 2 n V more where it is not: a loss that is one part of another takes its
-//   weight w here.
+//   weight w here.  fp32 is then scaled in place (a second rounding of 2^-24, below what the row's sum leaves); bf16 is
+//   formed anew from the logits, since scaling would round it to 8 bits twice.
 // Rows are split over workgroups when there are fewer rows than the chip needs workgroups; the splits' (maximum, sum) pairs
 // are merged in a fixed order, so results do not depend on the schedule.  Statistics, probabilities and the loss are fp32;
-// the gradient is rounded once, on store.
+// a bf16 gradient is rounded once, on store.
 // Measured: together, 8192 x 26747 fp32 with lists of 50, 372 us forward and backward -- 1758 MB at 4.7 TB/s, what a copy
 // reaches on this card; apart, 580 us.  64 x 10007 bf16: 30 us of kernels, of 110 that the calls and autograd take.
 #include "elem.h"
@@ -373,7 +374,8 @@ __global__ __launch_bounds__(kThreads) void scale_kernel(T* __restrict__ x, int6
 }
 
 // dlogits of a row segment: g (q - 0) everywhere, then the list's entries of the segment once more with their p taken
-// off.  An item that is on the list twice is written by its first entry, with the sum of its p in list order.
+// off.  An item that is on the list twice is written by its first entry, with the sum of its p in list order.  `again`:
+// dlogits holds the gradient for dloss = 1 already, and nothing is left to do where it is 1.
 template <class T>
 __global__ __launch_bounds__(kThreads) void grad_kernel(const T* __restrict__ logits, int64_t ld, int64_t V,
                                                         const int64_t* __restrict__ ids, int top, int splits,
@@ -381,11 +383,12 @@ __global__ __launch_bounds__(kThreads) void grad_kernel(const T* __restrict__ lo
                                                         const float2* __restrict__ state,
                                                         const float* __restrict__ prob,
                                                         const float* __restrict__ stats,
-                                                        const float* __restrict__ dloss, T* __restrict__ dlogits,
-                                                        int64_t ld_d) {
+                                                        const float* __restrict__ dloss, int again,
+                                                        T* __restrict__ dlogits, int64_t ld_d) {
     constexpr int E = Elem<T>::V;
     __shared__ int list[kMaxTop];
     __shared__ float lp[kMaxTop];
+    if (again && dloss[0] == 1.f) return;  // (the whole grid)
     const int64_t row = blockIdx.x / splits;
     const int64_t begin = (int64_t)(blockIdx.x % splits) * seg_len;
     const int64_t len = max((int64_t)0, min(seg_len, V - begin));
@@ -549,9 +552,9 @@ ASME_API int asme_scale_by(void* x, int64_t n, int dtype, const float* factor, v
     ASME_LAUNCH_CHECK("asme_scale_by");
 }
 
-ASME_API int asme_distill_xent_bwd(const void* logits, int64_t ld, int64_t n, int64_t V, const int64_t* ids, int64_t top,
-                                   float temperature, float weight, int dtype, const float* state, const float* prob,
-                                   const float* stats, const float* dloss, void* dlogits, int64_t ld_d, void* stream) {
+static int distill_bwd(const void* logits, int64_t ld, int64_t n, int64_t V, const int64_t* ids, int64_t top,
+                       float temperature, float weight, int dtype, const float* state, const float* prob,
+                       const float* stats, const float* dloss, int again, void* dlogits, int64_t ld_d, void* stream) {
     ASME_CHECK_ARG(logits && ids && state && prob && stats && dloss && dlogits, "asme_distill_xent_bwd: null pointer");
     ASME_CHECK_ARG(logits != dlogits, "asme_distill_xent_bwd: dlogits must not be logits");
     ASME_CHECK_ARG(dtype_ok(dtype), "asme_distill_xent_bwd: dtype is 0 (fp32) or 1 (bf16)");
@@ -563,7 +566,23 @@ ASME_API int asme_distill_xent_bwd(const void* logits, int64_t ld, int64_t n, in
         using T = decltype(t);
         hipLaunchKernelGGL(grad_kernel<T>, dim3((unsigned)(n * splits)), dim3(kThreads), 0, (hipStream_t)stream,
                            (const T*)logits, ld, V, ids, (int)top, splits, split_len(V, splits), kLog2e / temperature,
-                           weight * temperature, (const float2*)state, prob, stats, dloss, (T*)dlogits, ld_d);
+                           weight * temperature, (const float2*)state, prob, stats, dloss, again, (T*)dlogits, ld_d);
     });
     ASME_LAUNCH_CHECK("asme_distill_xent_bwd");
+}
+
+ASME_API int asme_distill_xent_bwd(const void* logits, int64_t ld, int64_t n, int64_t V, const int64_t* ids, int64_t top,
+                                   float temperature, float weight, int dtype, const float* state, const float* prob,
+                                   const float* stats, const float* dloss, void* dlogits, int64_t ld_d, void* stream) {
+    return distill_bwd(logits, ld, n, V, ids, top, temperature, weight, dtype, state, prob, stats, dloss, 0, dlogits, ld_d,
+                       stream);
+}
+
+// What is left to do behind asme_distill_xent_fwd_grad: dlogits (contiguous) formed anew where dloss is not 1
+ASME_API int asme_distill_xent_bwd_again(const void* logits, int64_t ld, int64_t n, int64_t V, const int64_t* ids,
+                                         int64_t top, float temperature, float weight, int dtype, const float* state,
+                                         const float* prob, const float* stats, const float* dloss, void* dlogits,
+                                         void* stream) {
+    return distill_bwd(logits, ld, n, V, ids, top, temperature, weight, dtype, state, prob, stats, dloss, 1, dlogits, V,
+                       stream);
 }

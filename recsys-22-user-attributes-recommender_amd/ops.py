@@ -2027,8 +2027,12 @@ class _DistillFn(torch.autograd.Function):
         x = x if x.dim() == 2 else x.view(-1, V)
         n = x.shape[0]
         g, ctx.grad = ctx.grad, None
-        if g is not None:
+        if g is not None and g.dtype == torch.float32:
             _call_on(g, "asme_scale_by", ptr(g), g.numel(), _dtype_code(g), ptr(_f32(dloss)))
+            return g, None, None, None, None
+        if g is not None:  # (scaled, a bf16 gradient would be rounded twice)
+            _call_on(x, "asme_distill_xent_bwd_again", ptr(x), V, n, V, ptr(ids), ids.shape[-1], temperature, weight,
+                     _dtype_code(x), ptr(state), ptr(prob), ptr(out), ptr(_f32(dloss)), ptr(g))
             return g, None, None, None, None
         # (also a second backward of one forward: the first one gave its gradient away)
         g = torch.empty(shape, device=x.device, dtype=x.dtype)

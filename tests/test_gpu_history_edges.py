@@ -6,7 +6,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_history_ops import check_window, near, rand, window64
+from test_gpu_history_ops import check_window, distill64, distill_lists, near, rand, window64
 
 pytestmark = pytest.mark.gpu
 
@@ -88,3 +88,21 @@ def test_a_sequence_does_not_depend_on_its_batch(asme, dev, dtype, n, h, d, wind
     alone = asme.ops.window_attention(*one, window, sinks=sinks, causal=causal, valid=valid[7:8].cuda())
     (grad,) = torch.autograd.grad(alone, one[0], dout[7:8])
     assert torch.equal(alone[0], out[7]) and torch.equal(grad[0], dq[7])
+
+
+# ------------------------------------------------------------------------------------------------ distillation
+@pytest.mark.parametrize("factor", [0.75, 3.0, 1.0, -0.1])
+@pytest.mark.parametrize("n,V", [(600, 4100), (513, 40007)])
+def test_distill_rounds_a_bf16_gradient_once(asme, dev, n, V, factor):
+    """where the forward formed the gradient too, an upstream factor is applied before the one rounding: within half a step
+    of the exact gradient, and the bits of a backward that forms its own"""
+    x = rand(n, V, seed=3, dtype=torch.bfloat16, scale=2.0).requires_grad_()
+    ids, t = distill_lists(n, V, 6, 4)
+    f = torch.tensor(factor, device=dev)
+    loss = asme.ops.distill_cross_entropy(x, ids, t, 1.5)
+    (a,) = torch.autograd.grad(loss, x, f, retain_graph=True)
+    (b,) = torch.autograd.grad(loss, x, f)  # (the second one of a forward)
+    want, grad, q, on, count = distill64(x, ids, t, 1.5)
+    m, r = x.detach().abs().max().item() / 1.5 + math.log(V) + 1, t.abs().max().item() * 2 / 1.5 + 4  # (as in test_distill)
+    near(a, factor * grad, abs(factor) * 1.5 / count * (q * (4 * m + V / 256 + 40) + on * (2 * r + 8)), 1, "gradient")
+    assert torch.equal(a, b)
