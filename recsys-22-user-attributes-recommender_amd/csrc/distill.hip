@@ -119,6 +119,20 @@ __global__ __launch_bounds__(kThreads) void stats_kernel(const T* __restrict__ l
     }
 }
 
+// The wave's maximum of a list's present logits; `there`: the row has a list -- a present entry above -infinity, or a NaN,
+// which the maximum skips and which is to reach the loss
+__device__ __forceinline__ float list_max(const int64_t* id, const float* t, int top, int64_t V, bool& there) {
+    float m = -INFINITY;
+    bool any = false;
+    for (int j = threadIdx.x & 63; j < top; j += 64)
+        if ((uint64_t)id[j] < (uint64_t)V) {
+            m = fmaxf(m, t[j]);
+            any = any || !(t[j] == -INFINITY);
+        }
+    there = __any(any);
+    return wave_max(m);
+}
+
 // One wave per row: its softmax state (maximum in base 2, 1 / sum; 0 for a row without a list) -- kept apart, since
 // lse rounded to fp32 would cost every q of the row |lse| 2^-24 --, p (n x top, 0 for absent entries), and the workgroup's (loss,
 // rows) sums in the order of its waves; `finish` (one workgroup in all): the mean at once.
@@ -138,15 +152,12 @@ __global__ __launch_bounds__(1024) void rows_kernel(const T* __restrict__ logits
         const float log_s = logf(a.s);
         const int64_t* id = ids + row * top;
         const float* t = teacher + row * top;
-        float tm = -INFINITY;
-        for (int j = lane; j < top; j += 64)
-            if ((uint64_t)id[j] < (uint64_t)V) tm = fmaxf(tm, t[j]);
-        tm = wave_max(tm);
+        bool there;
+        const float tm = list_max(id, t, top, V, there);
         float ts = 0.f;
         for (int j = lane; j < top; j += 64)
-            if ((uint64_t)id[j] < (uint64_t)V && tm > -INFINITY) ts += expf((t[j] - tm) * inv_tau);
+            if ((uint64_t)id[j] < (uint64_t)V && there) ts += expf((t[j] - tm) * inv_tau);
         ts = wave_sum(ts);
-        const bool there = !(tm == -INFINITY);
         const float log_ts = logf(ts);
         float kl = 0.f;
         for (int j = lane; j < top; j += 64) {
@@ -219,11 +230,8 @@ __global__ __launch_bounds__(1024) void teacher_kernel(const int64_t* __restrict
     if (row < n) {
         const int64_t* id = ids + row * top;
         const float* t = teacher + row * top;
-        float tm = -INFINITY, ts = 0.f;
-        for (int j = lane; j < top; j += 64)
-            if ((uint64_t)id[j] < (uint64_t)V) tm = fmaxf(tm, t[j]);
-        tm = wave_max(tm);
-        there = !(tm == -INFINITY);
+        float ts = 0.f;
+        const float tm = list_max(id, t, top, V, there);
         for (int j = lane; j < top; j += 64)
             if (there && (uint64_t)id[j] < (uint64_t)V) ts += expf((t[j] - tm) * inv_tau);
         const float log_ts = logf(wave_sum(ts));

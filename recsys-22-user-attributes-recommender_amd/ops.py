@@ -2048,7 +2048,7 @@ def distill_cross_entropy(logits: torch.Tensor, teacher_ids: torch.Tensor, teach
         weight * temperature^2 * KL(softmax(teacher_logits / temperature) over the list || softmax(logits / temperature)
         over V),
     mean over the rows whose list is not empty (NaN when all are).  Entries whose id is not in [0, V) (-1 ends a shorter
-    list) are absent; an item twice on a list counts twice.  The gradient goes to `logits`; the teacher takes none.
+    list) are absent, and a list of nothing but -inf is empty; an item twice on a list counts twice.  The gradient goes to `logits`; the teacher takes none.
     logits float32 or bfloat16, the loss float32.  A loss that is one part of another is cheapest with its `weight` here:
     the gradient is formed with the forward for that weight, and a factor other than 1 from above is one more pass."""
     V, top = logits.shape[-1], teacher_ids.shape[-1]

@@ -106,3 +106,28 @@ def test_distill_rounds_a_bf16_gradient_once(asme, dev, n, V, factor):
     m, r = x.detach().abs().max().item() / 1.5 + math.log(V) + 1, t.abs().max().item() * 2 / 1.5 + 4  # (as in test_distill)
     near(a, factor * grad, abs(factor) * 1.5 / count * (q * (4 * m + V / 256 + 40) + on * (2 * r + 8)), 1, "gradient")
     assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("n,V", [(3, 50), (600, 4100)])
+def test_distill_does_not_lose_a_nan_of_the_teacher(asme, dev, n, V):
+    """a NaN among a row's present logits makes the loss NaN, also where nothing else is on the list; absent entries may
+    hold one; a list of -inf alone is empty"""
+    x = rand(n, V, seed=5).requires_grad_()
+    ids = torch.tensor([[3, 40, -1]] * n, device=dev)
+    ids[1] = torch.tensor([7, -1, V])
+    t = torch.tensor([[1.0, 0.5, math.nan]] * n, device=dev)
+    assert torch.isfinite(asme.ops.distill_cross_entropy(x, ids, t))
+    for row, col in ((1, 0), (2, 0), (2, 1)):
+        bad = t.clone()
+        bad[row, col] = math.nan
+        loss = asme.ops.distill_cross_entropy(x, ids, bad)
+        (g,) = torch.autograd.grad(loss, x)
+        assert torch.isnan(loss) and torch.isnan(g[row, ids[row, col]]), (row, col)
+        assert torch.isfinite(g[torch.arange(n, device=dev) != row]).all()
+    low = t.clone()
+    low[1] = -math.inf
+    loss = asme.ops.distill_cross_entropy(x, ids, low)
+    (g,) = torch.autograd.grad(loss, x)
+    gone = ids.clone()
+    gone[1] = -1
+    assert torch.equal(loss, asme.ops.distill_cross_entropy(x, gone, t)) and (g[1] == 0).all()
