@@ -2001,6 +2001,8 @@ class _DistillFn(torch.autograd.Function):
         state = torch.empty(n, 2, device=dev, dtype=torch.float32)
         prob = torch.empty(n, top, device=dev, dtype=torch.float32)
         out = torch.empty(2, device=dev, dtype=torch.float32)
+        # out[0] as a tensor of its own: autograd lets no one change a view that a Function returns (loss += ...)
+        loss = torch.empty(0, device=dev, dtype=torch.float32).set_(out.untyped_storage(), 0, ())
         ctx.save_for_backward(kept, ids, state, prob, out)
         ctx.meta, ctx.grad = (temperature, weight, logits.shape), None
         code = _dtype_code(x)
@@ -2012,11 +2014,11 @@ class _DistillFn(torch.autograd.Function):
             ws, nb = _ws_bytes("asme_distill_xent_grad_workspace", n, device=dev)
             _call_on(x, "asme_distill_xent_fwd_grad", ptr(x), V, n, V, ptr(ids), ptr(teacher), top, temperature, weight, code,
                      ptr(state), ptr(prob), ptr(ctx.grad), ptr(ws), nb, ptr(out))
-            return out[0]
+            return loss
         ws, nb = _ws_bytes("asme_distill_xent_workspace", n, V, device=dev)
         _call_on(x, "asme_distill_xent_fwd", ptr(x), x.stride(0), n, V, ptr(ids), ptr(teacher), top, temperature, weight, code,
                  ptr(state), ptr(prob), ptr(ws), nb, ptr(out))
-        return out[0]
+        return loss
 
     @staticmethod
     @once_differentiable

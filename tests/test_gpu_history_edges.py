@@ -131,3 +131,17 @@ def test_distill_does_not_lose_a_nan_of_the_teacher(asme, dev, n, V):
     gone = ids.clone()
     gone[1] = -1
     assert torch.equal(loss, asme.ops.distill_cross_entropy(x, gone, t)) and (g[1] == 0).all()
+
+
+@pytest.mark.parametrize("n,V", [(3, 50), (600, 4100)])
+def test_distill_loss_is_added_to_in_place(asme, dev, n, V):
+    x = rand(n, V, seed=5).requires_grad_()
+    ids, t = distill_lists(n, V, 6, 4)
+    loss = asme.ops.distill_cross_entropy(x, ids, t)
+    (want,) = torch.autograd.grad(loss, x)
+    total = asme.ops.distill_cross_entropy(x, ids, t)
+    total += x.square().sum()
+    total *= 2
+    (g,) = torch.autograd.grad(total, x)
+    assert loss.shape == () and torch.equal(total, 2 * (loss + x.square().sum()))
+    near(g, 2 * (want.double() + 2 * x.double()), 4 * x.abs() + 4 * want.abs(), 4, "gradient")
