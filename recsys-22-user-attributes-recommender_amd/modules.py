@@ -19,6 +19,7 @@ Batch keys: item, item.target, positive_samples, negative_samples (data/datasets
 from __future__ import annotations
 
 import inspect
+import math
 from typing import Dict, Optional, Tuple
 
 import torch
@@ -311,7 +312,8 @@ def _rows_cross_entropy(model, sequence, rows, targets, pad: int, inverse=None) 
 
 def _rows_distillation(model, sequence, batch, rows, targets, pad: int, loss, inverse=None) -> torch.Tensor:
     """_rows_cross_entropy mixed with `loss` (losses.TopKDistillationLoss) over the same rows' teacher lists, both on
-    logits that are formed once"""
+    logits that are formed once.  Rows without a list have the cross-entropy alone, and so has a batch in which no row has
+    one (the mean over no rows would be NaN)"""
     if TEACHER_IDS_ENTRY_NAME not in batch or TEACHER_LOGITS_ENTRY_NAME not in batch:
         raise Exception(f"The batch does not contain {TEACHER_IDS_ENTRY_NAME} and {TEACHER_LOGITS_ENTRY_NAME}. "
                         f"Found the following batch entries: {', '.join(batch.keys())}")
@@ -319,10 +321,12 @@ def _rows_distillation(model, sequence, batch, rows, targets, pad: int, loss, in
         if batch[k].shape[:-1] != batch[TARGET_ENTRY_NAME].shape:
             raise ValueError(f"{k} {tuple(batch[k].shape)}: expected a list for each of the targets "
                              f"{tuple(batch[TARGET_ENTRY_NAME].shape)}")
-    lists = [batch[k].reshape(-1, batch[k].shape[-1]).index_select(0, rows)
-             for k in (TEACHER_IDS_ENTRY_NAME, TEACHER_LOGITS_ENTRY_NAME)]
+    ids, teacher = (batch[k].reshape(-1, batch[k].shape[-1]).index_select(0, rows)
+                    for k in (TEACHER_IDS_ENTRY_NAME, TEACHER_LOGITS_ENTRY_NAME))
     logits = model.forward_rows(sequence, rows, inverse)
-    return loss(*lists, logits, weight=loss.weight) + (1.0 - loss.weight) * ops.cross_entropy(logits, targets, pad)
+    there = ((ids >= 0) & (ids < logits.shape[-1]) & (teacher != -math.inf)).any()
+    return (torch.where(there, loss(ids, teacher, logits, weight=loss.weight), 0.0)
+            + (1.0 - loss.weight) * ops.cross_entropy(logits, targets, pad))
 
 
 def _single_target_cross_entropy(model, sequence, targets, pad: int) -> torch.Tensor:

@@ -6,6 +6,7 @@ import math
 import pytest
 import torch
 
+from test_gpu_history_models import V, cloze_batch, model
 from test_gpu_history_ops import check_window, distill64, distill_lists, near, rand, window64
 
 pytestmark = pytest.mark.gpu
@@ -145,3 +146,32 @@ def test_distill_loss_is_added_to_in_place(asme, dev, n, V):
     (g,) = torch.autograd.grad(total, x)
     assert loss.shape == () and torch.equal(total, 2 * (loss + x.square().sum()))
     near(g, 2 * (want.double() + 2 * x.double()), 4 * x.abs() + 4 * want.abs(), 4, "gradient")
+
+
+# ------------------------------------------------------------------------------------------------ training and serving
+@pytest.mark.parametrize("weight", [0.0, 0.3, 1.0])
+def test_training_on_batches_without_lists(asme, dev, weight):
+    """a batch in which no row has a list has the cross-entropy alone; a teacher's NaN is no missing list"""
+    m = model(asme, "BERT4RecModel", attention_window=6, attention_sinks=1)
+    train = asme.MaskedTrainingModule(model=m, item_tokenizer=asme.tokenization.Tokenizer(V - 3), metrics=None)
+    batch = cloze_batch(asme, 6, 11)
+    loss = train.training_step(dict(batch), 0)["loss"]
+    names, leaves = zip(*m.named_parameters())
+    want = dict(zip(names, torch.autograd.grad(loss, leaves, allow_unused=True)))
+    train.distillation = asme.losses.TopKDistillationLoss(temperature=2.0, weight=weight)
+    for ids, logits in ((-1, 0.0), (V, 0.0), (5, -math.inf)):
+        none = {**batch, "teacher.ids": torch.full_like(batch["teacher.ids"], ids),
+                "teacher.logits": torch.full_like(batch["teacher.logits"], logits)}
+        mixed = train.training_step(none, 0)["loss"]
+        # (fused logits and cross-entropy there, logits first here: a few roundings of O(1) terms)
+        assert abs(mixed.item() - (1 - weight) * loss.item()) < 1e-5 * loss.item()
+        for name, g in zip(names, torch.autograd.grad(mixed, leaves, allow_unused=True)):
+            assert (g is None) == (want[name] is None), name
+            if g is not None:  # (the keys' bias: what the roundings leave of a sum of terms as large as the weights')
+                size = want[name.replace("bias", "weight") if name.endswith("linear_layers.1.bias") else name]
+                assert (g - (1 - weight) * want[name]).abs().max() <= 5e-5 * size.abs().max().clamp(min=1e-3), name
+    if weight:
+        batch["teacher.logits"] = batch["teacher.logits"].clone()
+        batch["teacher.ids"][:, 0, 0] = 5
+        batch["teacher.logits"][:, 0, 0] = math.nan
+        assert torch.isnan(train.training_step(batch, 0)["loss"])
