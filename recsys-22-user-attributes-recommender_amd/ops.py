@@ -2003,32 +2003,34 @@ class _DistillFn(torch.autograd.Function):
         out = torch.empty(2, device=dev, dtype=torch.float32)
         # out[0] as a tensor of its own: autograd lets no one change a view that a Function returns (loss += ...)
         loss = torch.empty(0, device=dev, dtype=torch.float32).set_(out.untyped_storage(), 0, ())
-        ctx.save_for_backward(kept, ids, state, prob, out)
-        ctx.meta, ctx.grad = (temperature, weight, logits.shape), None
-        code = _dtype_code(x)
+        ctx.meta, ctx.given = (temperature, weight, logits.shape), False
+        code, grad = _dtype_code(x), None
         # the gradient with the forward (csrc/distill.hip, "together") where a workgroup holds a row: at 8192 x 26747 fp32
         # 375 us forward and backward in place of 580; 785 where an upstream factor other than 1 is left to apply
         if (ctx.needs_input_grad[0] and x.is_contiguous() and x.data_ptr() % 16 == 0
                 and _lib.load().asme_distill_xent_grad_supported(n, V, code)):
-            ctx.grad = torch.empty(logits.shape, device=dev, dtype=x.dtype)
+            grad = torch.empty(logits.shape, device=dev, dtype=x.dtype)
             ws, nb = _ws_bytes("asme_distill_xent_grad_workspace", n, device=dev)
             _call_on(x, "asme_distill_xent_fwd_grad", ptr(x), V, n, V, ptr(ids), ptr(teacher), top, temperature, weight, code,
-                     ptr(state), ptr(prob), ptr(ctx.grad), ptr(ws), nb, ptr(out))
+                     ptr(state), ptr(prob), ptr(grad), ptr(ws), nb, ptr(out))
+            ctx.save_for_backward(kept, ids, state, prob, out, grad)
             return loss
         ws, nb = _ws_bytes("asme_distill_xent_workspace", n, V, device=dev)
         _call_on(x, "asme_distill_xent_fwd", ptr(x), x.stride(0), n, V, ptr(ids), ptr(teacher), top, temperature, weight, code,
                  ptr(state), ptr(prob), ptr(ws), nb, ptr(out))
+        ctx.save_for_backward(kept, ids, state, prob, out, grad)
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dloss):
-        x, ids, state, prob, out = ctx.saved_tensors
+        x, ids, state, prob, out, g = ctx.saved_tensors
         temperature, weight, shape = ctx.meta
         V = shape[-1]
         x = x if x.dim() == 2 else x.view(-1, V)
         n = x.shape[0]
-        g, ctx.grad = ctx.grad, None
+        # (.data: the caller may change what it is given, which is no change of a saved tensor)
+        g, ctx.given = None if g is None or ctx.given else g.data, True
         if g is not None and g.dtype == torch.float32:
             _call_on(g, "asme_scale_by", ptr(g), g.numel(), _dtype_code(g), ptr(_f32(dloss)))
             return g, None, None, None, None

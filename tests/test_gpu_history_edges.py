@@ -5,6 +5,7 @@ import math
 
 import pytest
 import torch
+import torch.utils.checkpoint
 
 from test_gpu_history_models import V, cloze_batch, model
 from test_gpu_history_ops import check_window, distill64, distill_lists, near, rand, window64
@@ -146,6 +147,32 @@ def test_distill_loss_is_added_to_in_place(asme, dev, n, V):
     (g,) = torch.autograd.grad(total, x)
     assert loss.shape == () and torch.equal(total, 2 * (loss + x.square().sum()))
     near(g, 2 * (want.double() + 2 * x.double()), 4 * x.abs() + 4 * want.abs(), 4, "gradient")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_distill_saves_its_gradient_where_hooks_see_it(asme, dev, dtype):
+    """what the forward keeps goes through saved-tensor hooks: offloaded to the host, or formed again by a checkpoint"""
+    n, V = 2048, 4100
+    x = rand(n, V, seed=5, dtype=dtype).requires_grad_()
+    ids, t = distill_lists(n, V, 6, 4)
+    f = torch.tensor(2.5, device=dev)
+    (want,) = torch.autograd.grad(asme.ops.distill_cross_entropy(x, ids, t), x, f)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    with torch.autograd.graph.save_on_cpu():
+        loss = asme.ops.distill_cross_entropy(x, ids, t)
+    torch.cuda.synchronize()
+    assert torch.cuda.memory_allocated() - before < x.numel() * x.element_size() / 4
+    (g,) = torch.autograd.grad(loss, x, f, retain_graph=True)
+    assert torch.equal(g, want)
+    (again,) = torch.autograd.grad(loss, x, f)
+    # the first was formed with the forward and scaled, this one formed anew: q rounded (or not, where it is contracted into
+    # q - p) before the subtraction on either side, then at most three products each -- up to 8 u of the terms q and p
+    _, _, q, on, count = distill64(x, ids, t, 1.0)
+    near(again, want, 2.5 / count * (q + on), 8, "again")
+    loss = torch.utils.checkpoint.checkpoint(asme.ops.distill_cross_entropy, x, ids, t, use_reentrant=False)
+    (g,) = torch.autograd.grad(loss, x, f)
+    assert torch.equal(g, want)
 
 
 # ------------------------------------------------------------------------------------------------ training and serving
