@@ -1792,11 +1792,14 @@ def window_cache_fill(cache_k: torch.Tensor, cache_v: torch.Tensor, k: torch.Ten
     _alike(cache_k, lengths=lengths)
     if lengths.shape != (B,):
         raise ValueError(f"lengths {tuple(lengths.shape)}: expected ({B},)")
+    if torch.is_grad_enabled() and (cache_k.requires_grad or cache_v.requires_grad):
+        raise RuntimeError("window_cache_fill has no gradient: the caches require none")
     if B == 0 or k.shape[1] == 0:
         return
     k, v = _strided_heads(k.detach()), _strided_heads(v.detach())
     _call_on(k, "asme_window_cache_fill", ptr(k), ptr(v), *k.stride()[:3], *v.stride()[:3], ptr(_i64(lengths)), B,
              k.shape[1], KV, D, slots, sinks, _dtype_code(cache_k), ptr(cache_k), ptr(cache_v))
+    torch.autograd.graph.increment_version((cache_k, cache_v))
 
 
 def window_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache_k: torch.Tensor,
@@ -1826,6 +1829,7 @@ def window_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cac
     ws, nb = _ws_bytes("asme_window_step_workspace", B, q.shape[1], KV, D, slots, device=q.device)
     _call_on(q, "asme_window_step", ptr(q), ptr(k), ptr(v), ptr(cache_k), ptr(cache_v), ptr(_i64(lengths)), B, q.shape[1],
              KV, D, slots, sinks, D ** -0.5 if scale is None else scale, _dtype_code(q), ptr(ws), nb, ptr(out))
+    torch.autograd.graph.increment_version((cache_k, cache_v))
     return out
 
 

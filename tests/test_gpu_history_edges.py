@@ -92,6 +92,34 @@ def test_a_sequence_does_not_depend_on_its_batch(asme, dev, dtype, n, h, d, wind
     assert torch.equal(alone[0], out[7]) and torch.equal(grad[0], dq[7])
 
 
+# ------------------------------------------------------------------------------------------------ the ring cache
+def cache_calls(asme, dev):
+    q, k = rand(2, 4, 32, seed=1), rand(2, 2, 32, seed=2)
+    prompt, n = rand(2, 5, 2, 32, seed=3), torch.tensor([4, 9], device=dev)
+    return {"step": lambda ck, cv: asme.ops.window_attention_step(q, k, k, ck, cv, n, sinks=1),
+            "fill": lambda ck, cv: asme.ops.window_cache_fill(ck, cv, prompt, prompt, n, sinks=1)}
+
+
+@pytest.mark.parametrize("kind", ["step", "fill"])
+def test_changed_caches_are_noticed(asme, dev, kind):
+    call = cache_calls(asme, dev)[kind]
+    ck, cv = rand(2, 2, 7, 32, seed=4), rand(2, 2, 7, 32, seed=5)
+    w = torch.ones(32, device=dev, requires_grad=True)
+    for cache in (ck, cv):
+        y = (cache * w).sum()
+        with torch.no_grad():
+            call(ck, cv)
+        with pytest.raises(RuntimeError, match="modified by an inplace"):
+            y.backward()
+    with pytest.raises(RuntimeError, match="no gradient"):
+        call(ck.clone().requires_grad_(), cv)
+    with torch.inference_mode():  # (tensors without a counter)
+        a, b = ck.clone(), cv.clone()
+        call(a, b)
+    call(ck, cv)
+    assert torch.equal(a, ck) and torch.equal(b, cv)
+
+
 # ------------------------------------------------------------------------------------------------ distillation
 @pytest.mark.parametrize("factor", [0.75, 3.0, 1.0, -0.1])
 @pytest.mark.parametrize("n,V", [(600, 4100), (513, 40007)])
