@@ -1844,7 +1844,7 @@ def _strided_heads(t: torch.Tensor) -> torch.Tensor:
     per = 16 // t.element_size()
     ok = (t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(s % per == 0 and s >= 0 for s in t.stride()[:3])
           and t.stride(1) < 2 ** 23)
-    return t if ok else t.contiguous().clone() if t.is_contiguous() else t.contiguous()
+    return t if ok else t.clone(memory_format=torch.contiguous_format)  # (whatever strides its axes of size 1 have)
 
 
 _HEAD_DIMS = (16, 32, 64, 128)

@@ -92,6 +92,22 @@ def test_a_sequence_does_not_depend_on_its_batch(asme, dev, dtype, n, h, d, wind
     assert torch.equal(alone[0], out[7]) and torch.equal(grad[0], dq[7])
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_one_sequence_of_a_buffer_with_odd_rows(asme, dev, dtype):
+    q, k, v = (rand(2, 1283, seed=i, dtype=dtype)[:, :1280].view(2, 5, 4, 64)[:1].requires_grad_() for i in (1, 2, 3))
+    dout = rand(2, 1283, seed=4, dtype=dtype)[:, :1280].view(2, 5, 4, 64)[:1]
+    out = asme.ops.window_attention(q, k, v, 3, sinks=1)
+    got = [out, *torch.autograd.grad(out, (q, k, v), dout)]
+    same = [t.detach().clone(memory_format=torch.contiguous_format).requires_grad_() for t in (q, k, v)]
+    other = asme.ops.window_attention(*same, 3, sinks=1)
+    for a, b in zip(got, [other, *torch.autograd.grad(other, same, dout)]):
+        assert torch.equal(a, b)
+    ck = torch.zeros(1, 4, 4, 64, device=dev, dtype=dtype)
+    cv, n = torch.zeros_like(ck), torch.tensor([5], device=dev)
+    asme.ops.window_cache_fill(ck, cv, k, v, n, sinks=1)
+    assert torch.equal(ck[0, :, 1:], k.detach()[0].transpose(0, 1)[:, [4, 2, 3]])
+
+
 # ------------------------------------------------------------------------------------------------ the ring cache
 def cache_calls(asme, dev):
     q, k = rand(2, 4, 32, seed=1), rand(2, 2, 32, seed=2)

@@ -18,3 +18,20 @@ def test_distill_bwd_again_refuses(asme):
                        (dict(top=1025), b"size"), (dict(dtype=2), b"dtype"), (dict(tau=0.0), b"temperature"),
                        (dict(w=math.inf), b"weight")):
         assert call(**bad) == -1 and words in lib.asme_mi_last_error(), (bad, lib.asme_mi_last_error())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("make", [
+    lambda t: t(2, 1283)[:, :1280].view(2, 5, 4, 64)[:1],                # one sequence of a buffer with odd rows
+    lambda t: t(1283 * 3)[3:1283].view(1, 5, 4, 64),                     # from an odd position on
+    lambda t: t(5, 64 * 4 + 1)[:, :256].view(5, 4, 64)[None],            # odd rows
+    lambda t: t(4, 5, 64).transpose(0, 1)[None],                         # heads outermost: read in place
+    lambda t: t(2, 5, 64, 4).transpose(2, 3),                            # head values apart
+    lambda t: t(2, 5, 1, 64).expand(2, 5, 4, 64)])                       # one head for all: read in place
+def test_strides_that_the_attention_kernels_take(asme, dtype, make):
+    """every (B, L, heads, head_dim) view comes out with rows on 16-byte boundaries, axes of size 1 included"""
+    x = make(lambda *n: torch.randn(*n).to(dtype))
+    y = asme.ops._strided_heads(x)
+    per = 16 // y.element_size()
+    assert torch.equal(x, y) and y.stride(3) == 1 and y.data_ptr() % 16 == 0
+    assert all(s % per == 0 for s in y.stride()[:3])
