@@ -1565,8 +1565,8 @@ def gated_residual_norm(res: torch.Tensor, y: torch.Tensor, post_w: torch.Tensor
                              "or that with 1 in trailing axes before the channels")
         per = n // max(1, gate.numel() // D)
     if n == 0:
-        zero = res + y * post_w.to(y.dtype)
-        return zero, (zero if pre_w is not None else None)
+        s = res + y + 0 * sum(t.sum() for t in (gate, *weights.values()) if t is not None)  # (of every input)
+        return s, (s * 1 if pre_w is not None else None)
     return _GatedResidualNormFn.apply(res, y, gate, *weights.values(), per, float(residual_scale), float(eps), bool(rms))
 
 
@@ -1756,7 +1756,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     scale = _check_window(q, q.shape[2], k.shape[2], q.shape[3], window, sinks, valid, scale)
     _alike(q, q.dtype, k=k, v=v)
     if q.numel() == 0:
-        return q * 1
+        return q * (1 + 0 * (k.sum() + v.sum()))  # (of every input, which all have a gradient)
     return _WindowAttentionFn.apply(*(_strided_heads(t) for t in (q, k, v)), None if valid is None else as_u8(valid),
                                     int(window), int(sinks), bool(causal), scale)
 

@@ -108,6 +108,25 @@ def test_one_sequence_of_a_buffer_with_odd_rows(asme, dev, dtype):
     assert torch.equal(ck[0, :, 1:], k.detach()[0].transpose(0, 1)[:, [4, 2, 3]])
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("b,n", [(0, 5), (3, 0)])
+def test_nothing_to_do_has_gradients_too(asme, dev, dtype, b, n):
+    """no sequences, or sequences of no positions: outputs of the right shape and type, and a gradient of every input"""
+    q, k, v, qkv = (torch.zeros(b, n, *x, device=dev, dtype=dtype, requires_grad=True)
+                    for x in ((4, 32), (2, 32), (2, 32), (192,)))
+    out, fused = asme.ops.window_attention(q, k, v, 3), asme.ops.window_attention_qkv(qkv, 2, 3)
+    assert out.shape == (b, n, 4, 32) and fused.shape == (b, n, 64) and out.dtype == fused.dtype == dtype
+    for t, g in zip((q, k, v, qkv), torch.autograd.grad(out.sum() + fused.sum(), (q, k, v, qkv))):
+        assert g.shape == t.shape and g.dtype == dtype
+    res, y = (torch.zeros(b, n, 8, device=dev, dtype=dtype, requires_grad=True) for _ in range(2))
+    gate = torch.full((b, 1, 8), math.inf, device=dev, dtype=dtype, requires_grad=True)
+    w = [torch.ones(8, device=dev, requires_grad=True) for _ in range(4)]
+    s, z = asme.ops.gated_residual_norm(res, y, *w, gate=gate)
+    assert s.shape == z.shape == res.shape and s.dtype == z.dtype == dtype and s is not z
+    for t, g in zip((res, y, gate, *w), torch.autograd.grad((s, z), (res, y, gate, *w), (s, z))):
+        assert g.shape == t.shape and g.dtype == t.dtype and (g == 0).all()
+
+
 # ------------------------------------------------------------------------------------------------ the ring cache
 def cache_calls(asme, dev):
     q, k = rand(2, 4, 32, seed=1), rand(2, 2, 32, seed=2)
