@@ -239,7 +239,8 @@ class SASRecModel(TransformerEncoderModel):
     # catalog_query() pairs with the item table; memory per user is sinks + window positions a block, for any history.
     @torch.no_grad()
     def prefill(self, sequence):
-        """(representations, layers.WindowCaches) of right-padded histories"""
+        """(representations, layers.WindowCaches) of right-padded histories; a user without any gets zeros, and may be
+        decoded from the first item on"""
         layer = self._servable()
         mask = sequence.padding_mask if sequence.padding_mask is not None else torch.ones_like(sequence.sequence,
                                                                                                dtype=torch.bool)
@@ -247,8 +248,8 @@ class SASRecModel(TransformerEncoderModel):
         B, L, _ = emb.shape
         caches = Ly.WindowCaches(layer.transformer_blocks, B, emb.device)
         rep = layer.prefill(emb, Ly.key_valid_mask(mask, emb.shape), caches)
-        rows = torch.arange(B, device=rep.device) * L + (caches.lengths - 1).clamp(min=0)
-        return ops.gather_rows(rows, rep.view(B * L, -1)), caches
+        last = torch.arange(B, device=rep.device) * L + caches.lengths - 1
+        return ops.gather_rows(last.masked_fill(caches.lengths == 0, -1), rep.view(B * L, -1)), caches
 
     @torch.no_grad()
     def decode(self, items: torch.Tensor, caches) -> torch.Tensor:

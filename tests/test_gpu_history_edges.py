@@ -7,7 +7,7 @@ import pytest
 import torch
 import torch.utils.checkpoint
 
-from test_gpu_history_models import V, cloze_batch, model
+from test_gpu_history_models import L, V, cloze_batch, histories, model
 from test_gpu_history_ops import check_window, distill64, distill_lists, near, rand, window64
 
 pytestmark = pytest.mark.gpu
@@ -265,3 +265,28 @@ def test_training_on_batches_without_lists(asme, dev, weight):
         batch["teacher.ids"][:, 0, 0] = 5
         batch["teacher.logits"][:, 0, 0] = math.nan
         assert torch.isnan(train.training_step(batch, 0)["loss"])
+
+
+def test_prefill_of_a_user_without_history(asme, dev):
+    """zeros for that user, nothing else changed, and its first items decoded from an empty cache"""
+    m = model(asme, attention_window=5, attention_sinks=1).eval()
+    seq, lengths = histories(asme, 4, 9, 5)
+    want, _ = m.prefill(seq)
+    mask = seq.padding_mask.clone()
+    mask[1:3] = False
+    rep, caches = m.prefill(asme.InputSequence(seq.sequence * mask, mask))
+    assert (rep[1:3] == 0).all() and torch.equal(rep[[0, 3]], want[[0, 3]])
+    assert caches.lengths.tolist() == [9, 0, 0, int(lengths[3])]
+    whole = torch.zeros(4, L, dtype=torch.int64, device=dev)
+    whole[:, :9] = seq.sequence * mask
+    for t in range(7):
+        items = torch.tensor([3 + t, 20 + t, 40 - t, 7], device=dev)
+        whole[torch.arange(4), caches.lengths] = items
+        rep = m.decode(items, caches)
+        mask = torch.arange(L, device=dev) < caches.lengths[:, None]
+        with torch.no_grad():
+            want = m.encode(asme.InputSequence(whole, mask))[torch.arange(4), caches.lengths - 1]
+        assert (rep - want).abs().max() < 2e-5 * want.abs().max(), t  # (as in test_gpu_history_models.py)
+    nobody = torch.zeros_like(mask)
+    rep, caches = m.prefill(asme.InputSequence(whole * 0, nobody))
+    assert (rep == 0).all() and caches.most == 0
