@@ -535,7 +535,7 @@ int asme_window_attention_bwd(const void* q, const void* k, const void* v, const
  * step: stores the new token's k, v (batch, kv_heads, head_dim) at position lengths[b] (tokens before this one; negative:
  * the sequence takes no step, its output is 0 and its cache stays) and writes out (batch, heads, head_dim) = the
  * attention of q (the same shape) to everything the cache then holds.  lengths stay as they are (several layers share
- * them).  head_dim 16, 32, 64 or 128; heads a multiple of kv_heads; pointers 16-byte aligned. */
+ * them).  head_dim 16, 32, 64 or 128; heads a multiple of kv_heads; scale > 0; pointers 16-byte aligned. */
 int64_t asme_window_step_workspace(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t slots);
 int asme_window_step(const void* q, const void* k, const void* v, void* cache_k, void* cache_v, const int64_t* lengths,
                      int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t slots, int64_t sinks,

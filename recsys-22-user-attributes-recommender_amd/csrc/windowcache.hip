@@ -265,6 +265,7 @@ ASME_API int asme_window_step(const void* q, const void* k, const void* v, void*
     ASME_CHECK_ARG(q && k && v && cache_k && cache_v && lengths && out, "asme_window_step: null pointer");
     ASME_CHECK_ARG(dtype_ok(dtype), "asme_window_step: dtype is 0 (fp32) or 1 (bf16)");
     ASME_CHECK_ARG(sizes_ok(batch, heads, kv_heads, head_dim, slots, sinks), "asme_window_step: bad size");
+    ASME_CHECK_ARG(scale > 0.f && scale < INFINITY, "asme_window_step: scale > 0");
     ASME_CHECK_ARG(aligned({q, k, v, cache_k, cache_v, out}), "asme_window_step: 16-byte alignment");
     ASME_CHECK_ARG(ws_bytes >= asme_window_step_workspace(batch, heads, kv_heads, head_dim, slots),
                    "asme_window_step: workspace too small");

@@ -1725,6 +1725,12 @@ class _WindowAttentionQKVFn(torch.autograd.Function):
         return (grad, None, None, *([None] * len(ctx.how)))
 
 
+def _attention_scale(scale: Optional[float], D: int) -> float:
+    if scale is not None and not 0.0 < scale < math.inf:
+        raise ValueError(f"scale {scale}: expected a positive number")
+    return D ** -0.5 if scale is None else float(scale)
+
+
 def _check_window(q, heads: int, kv_heads: int, D: int, window: int, sinks: int, valid, scale):
     if heads < 1 or kv_heads < 1 or heads % kv_heads:
         raise ValueError(f"{heads} query heads for {kv_heads} key heads: expected a multiple")
@@ -1732,13 +1738,12 @@ def _check_window(q, heads: int, kv_heads: int, D: int, window: int, sinks: int,
         raise ValueError(f"head_dim {D}: expected one of {_HEAD_DIMS}")
     if window < 1 or sinks < 0:
         raise ValueError(f"window {window}, sinks {sinks}: expected window >= 1, sinks >= 0")
-    if scale is not None and not 0.0 < scale < math.inf:
-        raise ValueError(f"scale {scale}: expected a positive number")
+    scale = _attention_scale(scale, D)
     if valid is not None and (valid.shape != q.shape[:2] or valid.dtype not in (torch.bool, torch.uint8)):
         raise ValueError(f"valid {tuple(valid.shape)} of {valid.dtype}: expected {tuple(q.shape[:2])} of bool")
     _dtype_code(q)
     _alike(q, valid=valid)
-    return D ** -0.5 if scale is None else float(scale)
+    return scale
 
 
 def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: int, sinks: int = 0,
@@ -1820,6 +1825,7 @@ def window_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cac
     _alike(cache_k, lengths=lengths)
     if lengths.shape != (B,):
         raise ValueError(f"lengths {tuple(lengths.shape)}: expected ({B},)")
+    scale = _attention_scale(scale, D)
     if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, cache_k, cache_v)):
         raise RuntimeError("window_attention_step has no gradient: call it under torch.no_grad()")
     q, k, v = (_aligned(t) for t in (q, k, v))
@@ -1828,7 +1834,7 @@ def window_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cac
         return out
     ws, nb = _ws_bytes("asme_window_step_workspace", B, q.shape[1], KV, D, slots, device=q.device)
     _call_on(q, "asme_window_step", ptr(q), ptr(k), ptr(v), ptr(cache_k), ptr(cache_v), ptr(_i64(lengths)), B, q.shape[1],
-             KV, D, slots, sinks, D ** -0.5 if scale is None else scale, _dtype_code(q), ptr(ws), nb, ptr(out))
+             KV, D, slots, sinks, scale, _dtype_code(q), ptr(ws), nb, ptr(out))
     torch.autograd.graph.increment_version((cache_k, cache_v))
     return out
 

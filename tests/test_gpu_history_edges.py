@@ -155,6 +155,19 @@ def test_changed_caches_are_noticed(asme, dev, kind):
     assert torch.equal(a, ck) and torch.equal(b, cv)
 
 
+def test_the_step_takes_a_scale(asme, dev):
+    """and refuses what window_attention refuses"""
+    q, k, ck, cv = rand(2, 4, 32, seed=1), rand(2, 2, 32, seed=2), rand(2, 2, 7, 32, seed=4), rand(2, 2, 7, 32, seed=5)
+    n = torch.tensor([3, 9], device=dev)
+    for scale in (0.0, -0.1, math.inf, math.nan):
+        with pytest.raises(ValueError, match="scale"):
+            asme.ops.window_attention_step(q, k, k, ck, cv, n, sinks=1, scale=scale)
+    got = asme.ops.window_attention_step(q, k, k, ck.clone(), cv.clone(), n, sinks=1, scale=0.5)
+    # (a factor that is a power of two rounds nothing, wherever it is applied)
+    want = asme.ops.window_attention_step(q * 0.5, k, k, ck, cv, n, sinks=1, scale=1.0)
+    assert torch.equal(got, want)
+
+
 # ------------------------------------------------------------------------------------------------ distillation
 @pytest.mark.parametrize("factor", [0.75, 3.0, 1.0, -0.1])
 @pytest.mark.parametrize("n,V", [(600, 4100), (513, 40007)])

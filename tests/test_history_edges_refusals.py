@@ -35,3 +35,12 @@ def test_strides_that_the_attention_kernels_take(asme, dtype, make):
     per = 16 // y.element_size()
     assert torch.equal(x, y) and y.stride(3) == 1 and y.data_ptr() % 16 == 0
     assert all(s % per == 0 for s in y.stride()[:3])
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.1, math.inf, math.nan])
+def test_the_step_refuses_the_scales_that_attention_refuses(asme, scale):
+    lib = asme._lib.load()
+    one = ctypes.create_string_buffer(4096)
+    p = (ctypes.addressof(one) + 63) // 64 * 64  # never read
+    assert lib.asme_window_step(p, p, p, p, p, p, 1, 1, 1, 16, 4, 0, scale, 0, None, 0, p, None) == -1
+    assert b"scale" in lib.asme_mi_last_error()
