@@ -315,12 +315,13 @@ class WindowCaches:
     """The ring caches of every block's keys and values while sequences are served (ops.window_attention_step), and the
     tokens that each sequence has so far.  `most` is the longest sequence's count as the host knows it."""
 
-    def __init__(self, blocks, batch: int, device, dtype=torch.float32):
+    def __init__(self, blocks, batch: int, device):
         att = [b.attention for b in blocks]
         if not att or any(a.window is None for a in att):
             raise ValueError("only blocks with an attention_window are served from ring caches")
         self.sinks = att[0].sinks
-        self.layers = [tuple(torch.zeros(batch, a.heads, a.sinks + a.window, a.d_k, device=device, dtype=dtype)
+        self.layers = [tuple(torch.zeros(batch, a.heads, a.sinks + a.window, a.d_k, device=device,
+                                         dtype=torch.float32)
                              for _ in range(2)) for a in att]
         self.lengths = torch.zeros(batch, dtype=torch.int64, device=device)
         self.most = 0
