@@ -277,6 +277,9 @@ class GatedNorm(nn.Module):
 
     def residual(self, res, y, nxt: Optional[nn.LayerNorm]):
         """(res + gate * norm(y), nxt of it or None)"""
+        if has_forward_hooks(self.norm):
+            s = torch.addcmul(res, self.gate, self.norm(y))
+            return s, None if nxt is None else nxt(s)
         if nxt is not None and (has_forward_hooks(nxt) or nxt.eps != self.norm.eps):
             s, _ = ops.gated_residual_norm(res, y, self.norm.weight, self.norm.bias, gate=self.gate, eps=self.norm.eps)
             return s, nxt(s)

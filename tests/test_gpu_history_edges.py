@@ -303,3 +303,27 @@ def test_prefill_of_a_user_without_history(asme, dev):
     nobody = torch.zeros_like(mask)
     rep, caches = m.prefill(asme.InputSequence(whole * 0, nobody))
     assert (rep == 0).all() and caches.most == 0
+
+
+def test_hooks_on_every_norm_of_gated_blocks_run(asme, dev):
+    """norms with forward hooks are called as modules, and what a hook returns is used"""
+    m = model(asme, attention_window=5, attention_sinks=1, gated_norms=True).eval()
+    seq, _ = histories(asme, 4, L, 5)
+    layer = m._sequence_representation_layer.transformer_layer
+    norms = {n: x for n, x in layer.named_modules() if isinstance(x, torch.nn.LayerNorm)}
+    assert len(norms) == 8
+    with torch.no_grad():
+        want = m.encode(seq)
+        for name, norm in norms.items():
+            seen = []
+            handle = norm.register_forward_hook(lambda mod, args, out: seen.append(out.clone()))
+            got = m.encode(seq)
+            handle.remove()
+            # (another kernel's order of sums in two blocks: a few hundred roundings of O(1) terms)
+            assert len(seen) == 1 and (got - want).abs().max() < 2e-5 * want.abs().max(), name
+            handle = norm.register_forward_hook(lambda mod, args, out: out * 0.5)
+            half = m.encode(seq)
+            handle.remove()
+            norm.weight.mul_(0.5), norm.bias.mul_(0.5)
+            assert (half - m.encode(seq)).abs().max() < 2e-5 * half.abs().max(), name
+            norm.weight.mul_(2.0), norm.bias.mul_(2.0)
