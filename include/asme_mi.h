@@ -35,6 +35,8 @@ extern "C" {
 /* ---- status ------------------------------------------------------------------------------ */
 const char* asme_mi_last_error(void);
 int asme_mi_abi_version(void);
+/* the number of the graph capture that a stream is in, 0 outside of one */
+int64_t asme_stream_capture_id(void* stream);
 
 /* ---- embedding (core/models/common/layers/transformer_layers.py:55-80 TransformerEmbedding.forward,
  *      core/models/kebert4rec/components.py:54-63 PreFusion...forward) ------------------------------

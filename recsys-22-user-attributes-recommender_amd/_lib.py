@@ -22,6 +22,7 @@ f64 = ctypes.c_double
 SIGNATURES = {
     "asme_mi_last_error": [],
     "asme_mi_abi_version": [],
+    "asme_stream_capture_id": [p],
     "asme_embedding_fwd": [p, i64, i64, p, i64, i64, p, p, p, f32, f32, u64, p, p, p, f32, f32, u64, p, p, p, p, p],
     "asme_embedding_bwd": [p, i64, i64, p, i64, i64, p, p, p, f32, u64, p, p, f32, u64, p, p, p, p, p, p, i64, p],
     "asme_embedding_bwd_partials_count": [],
@@ -154,7 +155,7 @@ _RESTYPES = {"asme_mi_last_error": ctypes.c_char_p, "asme_dedup_workspace_bytes"
              "asme_distill_xent_workspace": ctypes.c_int64, "asme_distill_xent_grad_workspace": ctypes.c_int64,
              "asme_gated_residual_norm_bwd_workspace": ctypes.c_int64,
              "asme_window_attention_bwd_workspace": ctypes.c_int64,
-             "asme_window_step_workspace": ctypes.c_int64}
+             "asme_window_step_workspace": ctypes.c_int64, "asme_stream_capture_id": ctypes.c_int64}
 
 _lib: Optional[ctypes.CDLL] = None
 

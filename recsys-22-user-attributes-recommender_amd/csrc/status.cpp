@@ -23,3 +23,10 @@ int hip_status(hipError_t e, const char* where) {
 ASME_API const char* asme_mi_last_error(void) { return asme::g_last_error.c_str(); }
 
 ASME_API int asme_mi_abi_version(void) { return 1; }
+
+ASME_API int64_t asme_stream_capture_id(void* stream) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    if (hipStreamGetCaptureInfo((hipStream_t)stream, &status, &id) != hipSuccess) return 0;
+    return status == hipStreamCaptureStatusActive ? (int64_t)id : 0;
+}

@@ -1998,6 +1998,13 @@ def cross_entropy(logits, targets, ignore_index: int):
     return _CrossEntropyFn.apply(logits, targets, ignore_index)
 
 
+def _capture_id(t: torch.Tensor) -> int:
+    """the number of the graph capture that the current stream of t's device is in, 0 outside of one"""
+    if not torch.cuda.is_current_stream_capturing():
+        return 0
+    return _lib.load().asme_stream_capture_id(torch._C._cuda_getCurrentRawStream(t.get_device()))
+
+
 class _DistillFn(torch.autograd.Function):
     """tau^2 KL(teacher's list || softmax over the catalogue), mean over the rows with a list (csrc/distill.hip)."""
 
@@ -2024,6 +2031,7 @@ class _DistillFn(torch.autograd.Function):
             _call_on(x, "asme_distill_xent_fwd_grad", ptr(x), V, n, V, ptr(ids), ptr(teacher), top, temperature, weight, code,
                      ptr(state), ptr(prob), ptr(grad), ptr(ws), nb, ptr(out))
             ctx.save_for_backward(kept, ids, state, prob, out, grad)
+            ctx.capture = _capture_id(x)
             return loss
         ws, nb = _ws_bytes("asme_distill_xent_workspace", n, V, device=dev)
         _call_on(x, "asme_distill_xent_fwd", ptr(x), x.stride(0), n, V, ptr(ids), ptr(teacher), top, temperature, weight, code,
@@ -2039,8 +2047,10 @@ class _DistillFn(torch.autograd.Function):
         V = shape[-1]
         x = x if x.dim() == 2 else x.view(-1, V)
         n = x.shape[0]
-        # (.data: the caller may change what it is given, which is no change of a saved tensor)
-        g, ctx.given = None if g is None or ctx.given else g.data, True
+        # A backward that is captured apart from its forward may be replayed more often than that, and would find the
+        # gradient as its last replay left it: it forms its own.  (.data: the caller may change what it is given, which is
+        # no change of a saved tensor)
+        g, ctx.given = None if g is None or ctx.given or ctx.capture != _capture_id(x) else g.data, True
         if g is not None and g.dtype == torch.float32:
             _call_on(g, "asme_scale_by", ptr(g), g.numel(), _dtype_code(g), ptr(_f32(dloss)))
             return g, None, None, None, None

@@ -251,6 +251,63 @@ def test_distill_saves_its_gradient_where_hooks_see_it(asme, dev, dtype):
     assert torch.equal(g, want)
 
 
+class Distilled(torch.nn.Module):
+    def __init__(self, asme, ids, t):
+        super().__init__()
+        self.op = asme.ops.distill_cross_entropy
+        self.register_buffer("ids", ids), self.register_buffer("t", t)
+
+    def forward(self, x):
+        return self.op(x, self.ids, self.t)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_distill_backward_captured_apart_and_replayed(asme, dev, dtype):
+    """a backward with a graph of its own, replayed several times for one replay of the forward's"""
+    n, V = 600, 4100
+    ids, t = distill_lists(n, V, 6, 4)
+    graphed = torch.cuda.make_graphed_callables(Distilled(asme, ids, t), (rand(n, V, seed=5, dtype=dtype).requires_grad_(),))
+    for turn in range(3):
+        x = rand(n, V, seed=6 + turn, dtype=dtype).requires_grad_()
+        loss, eager = graphed(x), asme.ops.distill_cross_entropy(x, ids, t)
+        assert torch.equal(loss, eager)
+        _, _, q, on, count = distill64(x, ids, t, 1.0)
+        for f in (2.0, 1.0, 0.5, 2.0):
+            (g,) = torch.autograd.grad(loss, x, torch.tensor(f, device=dev), retain_graph=True)
+            (want,) = torch.autograd.grad(eager, x, torch.tensor(f, device=dev), retain_graph=True)
+            # (as in the test before)
+            near(g.clone(), want, f / count * (q + on), 8 if dtype == torch.float32 else 0, (turn, f))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_distill_captured_with_its_gradient(asme, dev, dtype):
+    """forward and backward in one graph where the forward forms the gradient: every replay gives an eager call's bits"""
+    n, V = 600, 4100
+    x, f = rand(n, V, seed=5, dtype=dtype).requires_grad_(), torch.tensor(2.0, device=dev)
+    ids, t = distill_lists(n, V, 6, 4)
+
+    def call():
+        loss = asme.ops.distill_cross_entropy(x, ids, t, 2.0)
+        return [loss, *torch.autograd.grad(loss, x, f)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for turn, factor in enumerate((2.0, 1.0, 0.3, 1.0)):
+        with torch.no_grad():
+            x.copy_(rand(n, V, seed=20 + turn, dtype=dtype)), f.fill_(factor)
+        graph.replay()
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [o.detach().clone() for o in out]
+        for a, b in zip(got, call()):
+            assert torch.equal(a, b), turn
+
+
 # ------------------------------------------------------------------------------------------------ training and serving
 @pytest.mark.parametrize("weight", [0.0, 0.3, 1.0])
 def test_training_on_batches_without_lists(asme, dev, weight):
