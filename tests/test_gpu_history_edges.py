@@ -8,7 +8,7 @@ import torch
 import torch.utils.checkpoint
 
 from test_gpu_history_models import L, V, cloze_batch, histories, model
-from test_gpu_history_ops import check_window, distill64, distill_lists, near, rand, window64
+from test_gpu_history_ops import check_window, distill64, distill_lists, near, rand, ring, window64
 
 pytestmark = pytest.mark.gpu
 
@@ -127,6 +127,80 @@ def test_nothing_to_do_has_gradients_too(asme, dev, dtype, b, n):
         assert g.shape == t.shape and g.dtype == t.dtype and (g == 0).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("scale", [0.03, 1.3])
+def test_window_attention_takes_a_scale(asme, dev, dtype, scale):
+    valid = ragged(3, 150, 7)
+    (q, k, v, dout), got = window_call(asme, dtype, 3, 150, 4, 2, 32, 20, 3, True, valid, scale=scale)
+    check_close(got, dtype, q, k, v, dout, 20, 3, True, valid, scale, 150)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("causal", [True, False])
+def test_window_attention_of_one_projection(asme, dev, dtype, causal):
+    """window_attention_qkv, also of a projection whose rows are apart: what separate q, k and v give, bit for bit"""
+    b, n, h, d = 3, 130, 4, 64
+    wide = rand(b, n, 3 * h * d + 8, seed=3, dtype=dtype, scale=1.5)
+    valid, dout = ragged(b, n, 8).cuda(), rand(b, n, h * d, seed=4, dtype=dtype)
+    parts = [t.clone().view(b, n, h, d).requires_grad_() for t in wide[..., :3 * h * d].split(h * d, -1)]
+    want = asme.ops.window_attention(*parts, 20, sinks=3, causal=causal, valid=valid)
+    grads = torch.autograd.grad(want, parts, dout.view(b, n, h, d))
+    for qkv in (wide[..., :3 * h * d].contiguous().requires_grad_(), wide[..., :3 * h * d].detach().requires_grad_()):
+        out = asme.ops.window_attention_qkv(qkv, h, 20, sinks=3, causal=causal, valid=valid)
+        (g,) = torch.autograd.grad(out, qkv, dout)
+        assert torch.equal(out, want.reshape(b, n, h * d))
+        assert torch.equal(g, torch.cat([t.reshape(b, n, h * d) for t in grads], -1))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_window_attention_of_views(asme, dev, dtype):
+    """inputs and an output's gradient in other orders, broadcast ones, and gradients of some inputs alone"""
+    b, n, h, d = 2, 90, 4, 32
+    q = rand(b, h, n, d, seed=1, dtype=dtype).transpose(1, 2)       # heads outermost
+    k = rand(n, b, 2, d, seed=2, dtype=dtype).transpose(0, 1)       # tokens outermost
+    v = rand(b, n, 1, d, seed=3, dtype=dtype).expand(b, n, 2, d)    # one value head for all key heads
+    dout = rand(d, h, n, b, seed=4, dtype=dtype).permute(3, 2, 1, 0)
+    plain = [t.clone(memory_format=torch.contiguous_format) for t in (q, k, v, dout)]
+
+    def grads(q, k, v, dout, which=(0, 1, 2)):
+        leaves = [t.detach().requires_grad_(i in which) for i, t in enumerate((q, k, v))]
+        out = asme.ops.window_attention(*leaves, 11, sinks=2)
+        return [out.detach(), *torch.autograd.grad(out, [leaves[i] for i in which], dout)]
+
+    want = grads(*plain)
+    for a, b_ in zip(grads(q, k, v, dout), want):
+        assert torch.equal(a, b_)
+    for which in ((0,), (1,), (2,), (0, 2)):
+        for a, i in zip(grads(q, k, v, dout, which)[1:], which):
+            assert torch.equal(a, want[1 + i]), which
+    ones = torch.ones((), device=dev, dtype=dtype).expand(b, n, h, d)
+    for a, b_ in zip(grads(q, k, v, ones), grads(*plain[:3], torch.ones_like(plain[3]))):
+        assert torch.equal(a, b_)
+    one = rand(b, n, 1, d, seed=3, dtype=dtype).requires_grad_()  # a broadcast input's gradient is the sum over its copies
+    out = asme.ops.window_attention(q, k, one.expand(b, n, 2, d), 11, sinks=2)
+    (g,) = torch.autograd.grad(out, one, dout)
+    half = want[3].double()
+    near(g, half.sum(2, keepdim=True), half.abs().sum(2, keepdim=True), 2, "broadcast v")
+
+
+def test_window_attention_beyond_32_bit_offsets(asme, dev):
+    """tokens so far apart that a sequence spans 2^32 values: the bits of a compact copy"""
+    n, h, d, apart = 1100, 2, 32, 1 << 22
+    compact = [rand(1, n, h, d, seed=i, dtype=torch.bfloat16) for i in range(1, 5)]
+
+    def spread(t):
+        big = torch.empty(n * apart, device=dev, dtype=torch.bfloat16).as_strided((1, n, h, d), (n * apart, apart, d, 1))
+        return big.copy_(t)
+
+    def grads(q, k, v, dout):
+        leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+        out = asme.ops.window_attention(*leaves, 70, sinks=3)
+        return [out, *torch.autograd.grad(out, leaves, dout)]
+
+    for a, b in zip(grads(*map(spread, compact)), grads(*compact)):
+        assert torch.equal(a, b)
+
+
 # ------------------------------------------------------------------------------------------------ the ring cache
 def cache_calls(asme, dev):
     q, k = rand(2, 4, 32, seed=1), rand(2, 2, 32, seed=2)
@@ -166,6 +240,31 @@ def test_the_step_takes_a_scale(asme, dev):
     # (a factor that is a power of two rounds nothing, wherever it is applied)
     want = asme.ops.window_attention_step(q * 0.5, k, k, ck, cv, n, sinks=1, scale=1.0)
     assert torch.equal(got, want)
+
+
+def test_a_cache_beyond_32_bit_offsets(asme, dev):
+    """two sequences of 2^26 slots of 64: one token against them, and a prompt laid in, behind the 2^32nd value"""
+    d, window, sinks = 64, (1 << 26) - 5, 5
+    slots = window + sinks
+    ck = torch.zeros(2, 1, slots, d, device=dev, dtype=torch.bfloat16)
+    cv = torch.zeros_like(ck)
+    q = torch.ones(2, 2, d, device=dev, dtype=torch.bfloat16)
+    k, v = q[:, :1] * 0.125, q[:, :1] * 3
+    far = slots - 3  # a key whose score is 64 above all others has all of the weight: 2^26 e^-64 of it elsewhere
+    ck[:, 0, far], cv[:, 0, far] = 8.0, torch.arange(d, device=dev).to(torch.bfloat16)
+    n = torch.tensor([slots - 2, 5 * window + slots - 2], device=dev)
+    out = asme.ops.window_attention_step(q, k, v, ck, cv, n, sinks=sinks)
+    # (whole numbers up to 63, exact in bf16; what the others add, at most 3 (2^26 e^-64 + e^-63) < 1e-19, is seen at 0 alone)
+    assert (out.double() - cv[:, :, far].double()).abs().max() < 1e-18
+    for b in range(2):
+        to = ring(int(n[b]), sinks, window)
+        assert to == slots - 2 and torch.equal(ck[b, 0, to], k[b, 0]) and torch.equal(cv[b, 0, to], v[b, 0])
+    ck.zero_()
+    prompt = rand(2, 40, 1, d, seed=3, dtype=torch.bfloat16)
+    asme.ops.window_cache_fill(ck, cv, prompt, prompt, torch.tensor([40, 0], device=dev), sinks=sinks)
+    assert torch.equal(ck[0, 0, :40], prompt[0, :, 0]) and not ck[0, 0, 40:].any() and not ck[1].any()
+    assert torch.equal(cv[0, 0, :40], prompt[0, :, 0]) and torch.equal(cv[:, 0, far], torch.arange(
+        d, device=dev).to(torch.bfloat16).expand(2, d))
 
 
 # ------------------------------------------------------------------------------------------------ distillation
