@@ -165,7 +165,7 @@ __global__ __launch_bounds__(1024) void rows_kernel(const T* __restrict__ logits
             float pj = 0.f;
             if (there && (uint64_t)v < (uint64_t)V) {
                 const float lp = (t[j] - tm) * inv_tau - log_ts;
-                pj = expf(lp);
+                pj = expf((t[j] - tm) * inv_tau) / ts;  // (not of lp, whose rounding grows with the list's length)
                 if (!(pj == 0.f)) kl += pj * (lp - (fmaf(Elem<T>::get(logits + row * ld + v), scale, -a.m) * kLn2 - log_s));
             }
             prob[row * top + j] = pj;
@@ -234,9 +234,9 @@ __global__ __launch_bounds__(1024) void teacher_kernel(const int64_t* __restrict
         const float tm = list_max(id, t, top, V, there);
         for (int j = lane; j < top; j += 64)
             if (there && (uint64_t)id[j] < (uint64_t)V) ts += expf((t[j] - tm) * inv_tau);
-        const float log_ts = logf(wave_sum(ts));
+        ts = wave_sum(ts);
         for (int j = lane; j < top; j += 64)
-            prob[row * top + j] = there && (uint64_t)id[j] < (uint64_t)V ? expf((t[j] - tm) * inv_tau - log_ts) : 0.f;
+            prob[row * top + j] = there && (uint64_t)id[j] < (uint64_t)V ? expf((t[j] - tm) * inv_tau) / ts : 0.f;
     }
     __shared__ float w[16];
     if (lane == 0) w[wave] = there ? 1.f : 0.f;

@@ -324,6 +324,19 @@ def test_distill_loss_is_added_to_in_place(asme, dev, n, V):
     near(g, 2 * (want.double() + 2 * x.double()), 4 * x.abs() + 4 * want.abs(), 4, "gradient")
 
 
+@pytest.mark.parametrize("top", [53, 998])
+@pytest.mark.parametrize("n,V", [(1, 2000), (512, 4096)])
+def test_distill_probabilities_of_a_long_list(asme, dev, n, V, top):
+    """equal logits: p is 1 / top, rounded once -- to 2^-24 of it, as the gradient of an item whose own q is nothing"""
+    x = torch.zeros(n, V, device=dev)
+    x[:, :top] = -60.0
+    x.requires_grad_()
+    ids = torch.arange(top, device=dev).expand(n, top)
+    (g,) = torch.autograd.grad(asme.ops.distill_cross_entropy(x, ids, torch.full((n, top), 1.7, device=dev)), x)
+    # (n is a power of two, the factor 1 / n exact; q < e^-60)
+    assert ((g[:, :top].double() * n * top + 1).abs() <= 2.0 ** -24 * (1 + 2.0 ** -20)).all()
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_distill_saves_its_gradient_where_hooks_see_it(asme, dev, dtype):
     """what the forward keeps goes through saved-tensor hooks: offloaded to the host, or formed again by a checkpoint"""
