@@ -1,5 +1,5 @@
 // Element types of the operators that take fp32 or bf16 storage (fp32 arithmetic either way): 16-byte vectors of either
-// type as floats, and the dtype codes of the C ABI.
+// type as floats, sums over lanes, and the dtype codes of the C ABI.
 #pragma once
 #include "common.h"
 
@@ -50,8 +50,31 @@ struct Elem<__bf16> {
     }
 };
 
+template <int CTRL>
+__device__ __forceinline__ float dpp_add(float x) {
+    return x + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xF, 0xF, true));
+}
+// sum over aligned groups of N lanes, in every lane (quad permutes, then mirrors of 8 and 16 lanes whose quads agree)
+template <int N>
+__device__ __forceinline__ float group_sum(float x) {
+    if constexpr (N >= 2) x = dpp_add<0xB1>(x);   // quad_perm 1 0 3 2
+    if constexpr (N >= 4) x = dpp_add<0x4E>(x);   // quad_perm 2 3 0 1
+    if constexpr (N >= 8) x = dpp_add<0x141>(x);  // row_half_mirror
+    if constexpr (N >= 16) x = dpp_add<0x140>(x); // row_mirror
+    if constexpr (N >= 32) x += __shfl_xor(x, 16, 64);
+    if constexpr (N >= 64) x += __shfl_xor(x, 32, 64);
+    return x;
+}
+
 inline bool dtype_ok(int dtype) { return dtype == kF32 || dtype == kBF16; }
 inline int64_t dtype_size(int dtype) { return dtype == kF32 ? 4 : 2; }
+
+// on 16-byte boundaries (null is)
+inline bool aligned(std::initializer_list<const void*> ps) {
+    for (const void* p : ps)
+        if ((uintptr_t)p & 15) return false;
+    return true;
+}
 
 // f(T{}) for the storage type of a checked dtype code
 template <class F>

@@ -24,19 +24,6 @@ namespace {
 
 constexpr int kMaxDim = 8192;
 
-template <int CTRL>
-__device__ __forceinline__ float dpp_add(float x) {
-    return x + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xF, 0xF, true));
-}
-// sum over aligned groups of N >= 16 lanes, in every lane (quad permutes, then mirrors of 8 and 16 lanes whose quads agree)
-template <int N>
-__device__ __forceinline__ float lanes_sum(float x) {
-    x = dpp_add<0x140>(dpp_add<0x141>(dpp_add<0x4E>(dpp_add<0xB1>(x))));
-    if constexpr (N >= 32) x += __shfl_xor(x, 16, 64);
-    if constexpr (N >= 64) x += __shfl_xor(x, 32, 64);
-    return x;
-}
-
 // A row over TPR threads of N values each, in vectors of 16 bytes.  EVEN: rows are whole vectors on their boundaries; else
 // vectors begin anywhere (global memory is read and written at any address) and the last one, part of a vector, goes
 // element by element -- a branch around a row's loads that costs even rows 8 % (16384 x 4096 bf16, backward: 211 us
@@ -113,7 +100,7 @@ struct Row {
     template <int K>
     static __device__ __forceinline__ void sum(float (&v)[K], float* red, int& flip) {
 #pragma unroll
-        for (int k = 0; k < K; ++k) v[k] = lanes_sum<(TPR < 64 ? TPR : 64)>(v[k]);
+        for (int k = 0; k < K; ++k) v[k] = group_sum<(TPR < 64 ? TPR : 64)>(v[k]);
         if constexpr (TPR > 64) {
             float* r = red + (flip & 1) * 32;
             ++flip;
@@ -435,12 +422,6 @@ __global__ __launch_bounds__(1024) void column_reduce_kernel(const float* __rest
         v += __shfl_xor(v, 32, 64);
         if (q == 0 && j < width) Elem<T>::put(out + g * width + j, v);
     }
-}
-
-bool aligned(std::initializer_list<const void*> ps) {
-    for (const void* p : ps)
-        if ((uintptr_t)p & 15) return false;
-    return true;
 }
 
 // f(Row<...>{}) for a checked dim: the fewest threads a row (at least 16) that hold it at one 16-byte vector each, 8

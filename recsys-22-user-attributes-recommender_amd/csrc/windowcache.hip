@@ -32,21 +32,6 @@ int64_t step_splits(int64_t heads, int64_t slots) {  // heads: workgroups that t
     return std::max<int64_t>(1, std::min<int64_t>({want, most, kMaxSplits}));
 }
 
-template <int CTRL>
-__device__ __forceinline__ float dpp_add(float x) {
-    return x + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xF, 0xF, true));
-}
-// sum over aligned groups of N lanes, in every lane (quad permutes, then mirrors of 8 and 16 lanes whose quads agree)
-template <int N>
-__device__ __forceinline__ float group_sum(float x) {
-    if constexpr (N >= 2) x = dpp_add<0xB1>(x);   // quad_perm 1 0 3 2
-    if constexpr (N >= 4) x = dpp_add<0x4E>(x);   // quad_perm 2 3 0 1
-    if constexpr (N >= 8) x = dpp_add<0x141>(x);  // row_half_mirror
-    if constexpr (N >= 16) x = dpp_add<0x140>(x); // row_mirror
-    if constexpr (N >= 32) x += __shfl_xor(x, 16, 64);
-    return x;
-}
-
 struct StepArgs {
     const void *q, *k, *v;
     void *cache_k, *cache_v, *out;
@@ -234,12 +219,6 @@ bool sizes_ok(int64_t batch, int64_t heads, int64_t kv_heads, int64_t D, int64_t
            slots > sinks && heads <= 65536 && batch <= (1ll << 24) && batch * heads <= (1ll << 24) &&
            slots <= (1ll << 40) / (batch * kv_heads * D);
 }
-bool aligned(std::initializer_list<const void*> ps) {
-    for (const void* p : ps)
-        if ((uintptr_t)p & 15) return false;
-    return true;
-}
-
 template <class F>
 void with_dim(int64_t D, F&& f) {
     if (D == 16) f(std::integral_constant<int, 16>{});
