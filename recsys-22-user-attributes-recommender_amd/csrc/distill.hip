@@ -15,8 +15,8 @@
 //   weight w here.  fp32 is then scaled in place (a second rounding of 2^-24, below what the row's sum leaves); bf16 is
 //   formed anew from the logits, since scaling would round it to 8 bits twice.
 // Rows are split over workgroups when there are fewer rows than the chip needs workgroups; the splits' (maximum, sum) pairs
-// are merged in a fixed order, so results do not depend on the schedule.  Statistics, probabilities and the loss are fp32;
-// a bf16 gradient is rounded once, on store.
+// are merged in a fixed order, so a schedule's results repeat bit for bit (the two differ in the order of their sums).
+// Statistics, probabilities and the loss are fp32; a bf16 gradient is rounded once, on store.
 // Measured: together, 8192 x 26747 fp32 with lists of 50, 372 us forward and backward -- 1758 MB at 4.7 TB/s, what a copy
 // reaches on this card; apart, 580 us.  64 x 10007 bf16: 30 us of kernels, of 110 that the calls and autograd take.
 #include "elem.h"

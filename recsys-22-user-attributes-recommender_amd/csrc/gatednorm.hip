@@ -14,8 +14,12 @@
 // thread (16 .. 1024 threads: a row's sums are lane moves within a wave, and one LDS exchange beyond it), and the next row
 // is on its way during its sums.  Weights stay in registers over a workgroup's rows.  Column sums: registers
 // (LDS beyond 4096 columns) over a workgroup's rows, then partial rows summed in a fixed order -- no atomics.
-// Measured (forward + backward): 16384 x 4096 bf16, gate per channel, 120 + 215 us for 403 + 671 MB (3.2 TB/s);
-// 204800 x 128 fp32, gate per sequence, 81 + 144 us for 839 MB in all (3.7 TB/s).
+// Measured (forward, whose four tensors are read or written once, and backward, whose six are): 16384 x 4096 bf16, a gate
+// per channel, 124 us for 537 MB (4.3 TB/s) and 220 for 805 (3.7); 204800 x 128 fp32, a gate per sequence or channel, 81 us
+// for 419 MB (5.2; a part comes from the cache) and 144 for 629 (4.4).  Rows that are not whole vectors, with a gate per
+// channel, take 1.6 to 3 times the copy rate's time: 3479 x 6299 bf16 101 + 121 us for 175 + 263 MB, 4050 x 2922 bf16 55 + 78
+// for 95 + 142, 303858 x 67 fp32 127 + 202 for 326 + 489; so do rows just beyond 4096 columns, 6710 x 4144 fp32 141 + 217 for
+// 445 + 667, where half of the 1024 threads hold nothing of the second vector.
 #include "elem.h"
 
 using namespace asme;

@@ -29,9 +29,9 @@
 // sequence's does not depend on what else is in its batch.  P in one term doubled the square of O's and dV's error (0.0023
 // of the output in place of 0.0017; L = 8192 below: forward 246 us, dK and dV 500); dS in one, whose terms cancel (a row of
 // it sums to 0), put dQ and dK off by 1.5 to 2 times their rounding.  Scores, softmax statistics and all sums are fp32.
-// Measured: 2 sequences of 8192, 16 heads on 4, 128 columns, window 1024 and 4 sinks, causal, bf16: forward 285 us (450
-// TFLOP/s of visible pairs, 40 % of what the library's large product reaches), dQ 376 (510), dK and dV 587 + 52 for what
-// queries outside the window see of the sinks (400).  Counters (profiles/history_ops_counters.json), of forward, dQ and
+// Measured: 2 sequences of 8192, 16 heads on 4, 128 columns, window 1024 and 4 sinks, causal, bf16: forward 279 us (460
+// TFLOP/s of visible pairs, 40 % of what the library's large product reaches), dQ 369 (520), dK and dV 574 + 52 for what
+// queries outside the window see of the sinks (410).  Counters (profiles/history_ops_counters.json), of forward, dQ and
 // dK / dV: MFMA busy 29, 29 and 27 %, vector units 36, 29 and 25 %, LDS 13, 13 and 22 %, waves waiting 37, 45 and 52 % of
 // their cycles; no bank conflicts.
 #include "elem.h"
@@ -156,7 +156,8 @@ struct Pass {
     using S = Frag<SP>;
 
     // The compiler keeps the LDS addresses of a tile's reads and writes, which are the same in every round, in registers:
-    // faster by 10 % than forming them anew (L = 8192, bf16, 128 columns) where there are registers.  fp32 rows of 128
+    // faster than forming them anew where there are registers (L = 8192, bf16, 128 columns: forward 378 us anew, 327 like
+    // this, both by events; dK and dV the same, though 37 values of its eight-wave form spill like this).  fp32 rows of 128
     // columns leave none (up to 91 spilled values); there the thread's number is made new to it in every round.
     static __device__ __forceinline__ int thread() {
         int t = threadIdx.x;
@@ -613,7 +614,7 @@ struct QueryTiles {
 // Two waves hold the same 32 keys.  Each forms P and dS of its half of the tile's queries and passes them on; each sums dK
 // and dV over all the queries, for its half of the columns.  With all columns in one wave the pass needs over 256 registers
 // at 128 columns and runs at one wave per SIMD, where the matrix and vector units take turns; with all of dV in one wave and
-// all of dK in the other, dS's second term would be a branch (800 us for L = 8192 in bf16 in place of 490).  Heads
+// all of dK in the other, dS's second term would be a branch (800 us for L = 8192 in bf16, P in one term; 500 like this).  Heads
 // of 32 columns have no halves: there a wave sums its half of the queries, and the pair adds up at the end.
 constexpr int kFarWaves = 4, kFarRows = 16 * kFarWaves;  // sinks of a workgroup of the far pass
 // where the far pass's sums of dK (0) or dV (1) of key kj begin
@@ -813,7 +814,7 @@ int padded_dim(int64_t dim) { return dim <= 32 ? 32 : (int)dim; }
 // Waves (of 32 stationary rows) per workgroup: eight share a streamed tile's way through LDS, at 256 registers each; four
 // (512 registers) where a pass's fragments and sums need more; two where the sequence has no more rows; half of them, twice
 // if need be, where each workgroup still has a CU of its own (one sequence of 2000, 4 heads of 128 columns, window 256,
-// bf16: forward 30 us, dQ 41 in 32 workgroups of eight waves, 23 and 25 in 126 of two; beyond that the tiles' way costs
+// bf16: forward 32 us, dQ 37 in 32 workgroups of eight waves, 21 and 22 in 126 of two; beyond that the tiles' way costs
 // more: 3 of 2049, 6 heads of 64, fp32, 63 us in 162 of eight, 70 in 306 of four).
 int waves(int64_t seqs, int64_t seq_len, int dtype, int dp) {  // seqs: sequences and heads
     int w = seq_len <= 64 ? 2 : dp == 32 || (dtype == kF32 && dp == 128) ? 4 : 8;
@@ -827,9 +828,10 @@ int waves_kv(int64_t seq_len, int dtype, int dp) {  // (two to 32 rows)
 // Pieces of the dK, dV passes.  Near: those that end first when the card takes its workgroups in rounds of `slots` and one
 // costs its steps and about 3 more (its keys, its sums; 4 with the rows it leaves to be added); at least 4 steps each, at
 // most 8 rounds (the partial rows' memory).  290 blocks in one piece are two rounds, the second nearly empty: 29 sequences
-// of 1181, window 307 to both sides, 128 columns in bf16 take 292 us, in 4 pieces 254.  Far: as many as give every CU two
+// of 1181, window 307 to both sides, four heads of 128 columns on one in bf16 take 345 us, in pieces 275 and 20 to add them
+// up.  Far: as many as give every CU two
 // workgroups, of at least 4 tiles; none where kAlong tiles or fewer are left to it, which the near pass takes along (256
-// ragged sequences of up to 200, 2 heads of 64, window 64, fp32: 126 us with a far pass, 105 without).
+// ragged sequences of up to 200, 2 heads of 64, window 64, fp32: 114 us with a far pass, 92 without).
 constexpr int kAlong = 4;
 void plan_kv(Args& a, int64_t batch, int dtype) {
     const int dp = padded_dim(a.dim), nw = waves_kv(a.seq_len, dtype, dp);
