@@ -78,6 +78,18 @@ def test_window_attention_in_workgroups_of_every_size(asme, dev, dtype, b, n, h,
     check_close(got, dtype, q, k, v, dout, window, sinks, causal, valid, d ** -0.5, n)
 
 
+# few keys and columns: scores are small, and what is left of an error is the factors' own rounding.  test_history_bounds.py
+# shows that check_close notices P or dS in one term, or D formed from the rounded output, at these sizes
+FEW_KEYS = [(3, 60, 2, 1, 16, 3, 1, True), (40, 130, 4, 2, 16, 2, 0, False), (3, 70, 2, 2, 32, 2, 1, True)]
+
+
+@pytest.mark.parametrize("b,n,h,kv,d,window,sinks,causal", FEW_KEYS)
+def test_window_attention_of_few_keys(asme, dev, b, n, h, kv, d, window, sinks, causal):
+    valid = torch.ones(b, n, dtype=torch.bool)
+    (q, k, v, dout), got = window_call(asme, torch.bfloat16, b, n, h, kv, d, window, sinks, causal, None, seed=40)
+    check_close(got, torch.bfloat16, q, k, v, dout, window, sinks, causal, valid, d ** -0.5, n)
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("n,h,d,window,sinks,causal", [(200, 4, 64, 40, 2, True), (130, 4, 128, 9, 1, False),
                                                        (300, 2, 32, 100, 5, True)])
