@@ -2023,7 +2023,8 @@ class _DistillFn(torch.autograd.Function):
         ctx.meta, ctx.given = (temperature, weight, logits.shape), False
         code, grad = _dtype_code(x), None
         # the gradient with the forward (csrc/distill.hip, "together") where a workgroup holds a row: at 8192 x 26747 fp32
-        # 375 us forward and backward in place of 580; 785 where an upstream factor other than 1 is left to apply
+        # 375 us forward and backward in place of 580; 785 where an upstream factor other than 1 is left to apply (bf16 206,
+        # and 404 with its gradient formed anew)
         if (ctx.needs_input_grad[0] and x.is_contiguous() and x.data_ptr() % 16 == 0
                 and _lib.load().asme_distill_xent_grad_supported(n, V, code)):
             grad = torch.empty(logits.shape, device=dev, dtype=x.dtype)
